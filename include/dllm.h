@@ -115,6 +115,94 @@ int dllm_decode_step(void* handle, const DllmStep* step, void* workspace, size_t
                      void* stream);
 int dllm_destroy(void* handle);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions of query and key heads, with the store of k and v into the
+ * paged caches (the rotary of nanovllm_dots/layers/rotary_embedding.py:6-47 and
+ * store_kvcache, layers/attention.py:10-47, for both pair layouts, part of a
+ * head and scaled frequencies).
+ * ------------------------------------------------------------------------- */
+enum { DLLM_BF16 = 0, DLLM_FP16 = 1, DLLM_FP32 = 2 };
+
+/* Strides are in elements; the last dimension is contiguous. */
+typedef struct DllmRotary {
+  int32_t dtype;                /* of q, q_out, k, v and the caches (DLLM_*) */
+  int32_t tokens;
+  int32_t q_heads, kv_heads;    /* kv_heads is not read without the store */
+  int32_t head_dim, rot_dim;    /* both even; dims [rot_dim, head_dim) are not turned */
+  int32_t interleaved;          /* pairs (2i, 2i + 1), else (i, i + rot_dim / 2) */
+  float factor;                 /* on cos and sin (attention factor; 1 for none) */
+  const uint64_t* turns;        /* [rot_dim / 2] turns a position, as a binary fraction of 2^64 */
+  const int32_t* positions;     /* [tokens] */
+  const void* q;                /* [tokens, q_heads, head_dim] */
+  void* q_out;                  /* the same shape; may be q with q's strides, else no overlap */
+  const void* k;                /* [tokens, kv_heads, head_dim]; NULL skips the store */
+  const void* v;
+  void* k_cache;                /* [num_slots, kv_heads, head_dim] */
+  void* v_cache;
+  const int32_t* slot_mapping;  /* [tokens]; -1: not stored */
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t num_slots;
+  uint32_t* err_word;           /* device word that gets the error bits (a slot past the cache) */
+} DllmRotary;
+
+/* Stream ordered, one launch, no allocation, no host synchronisation. */
+int dllm_rotary(const DllmRotary* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Append attention: the m_i = cu_seqlens_q[i + 1] - cu_seqlens_q[i] newest
+ * tokens of each sequence (their K/V is in the cache) over its context_lens[i]
+ * cached positions.  Token j of sequence i stands at position
+ * context_lens[i] - m_i + j = p and sees the keys k with
+ *     k <= p (causal), or k < prefix_lens[i];        every k without causal
+ *     k > p - window (window > 0);   k >= first_keys[token]
+ * all below context_lens[i].  With tree_masks (m_i <= 64) it sees the history
+ * k < context_lens[i] - m_i and the new tokens t whose bit t is set in its
+ * mask, whatever their order; the other masks and slopes are not used then.
+ * Scores are s = scale q.k, softcap tanh(s / softcap) if softcap > 0, minus
+ * slopes[h] |p - k| if slopes; the output is softmax(s) v, and zeros for a
+ * token that sees no key.  An infinity or NaN in a K or V row reaches the
+ * tokens that see it (V in a tile with masked keys: their rows become NaN) and
+ * no other; keys that no token sees are not read beyond the pages of those
+ * that are.  Rows of q and out past cu_seqlens_q[n] are not touched.
+ * ------------------------------------------------------------------------- */
+typedef struct DllmAppend {
+  int32_t dtype;                /* of q, caches and out: DLLM_BF16 or DLLM_FP16 */
+  int32_t tokens;               /* rows of q and out */
+  int32_t n;                    /* sequences */
+  int32_t num_heads, num_kv_heads, head_dim;   /* at most 128 query heads a kv head; 64 or 128 */
+  int32_t num_blocks, block_size, max_blocks;  /* block_size a multiple of 16 */
+  int32_t causal, window;
+  float scale, softcap;
+  const void* q;                /* [tokens, num_heads, head_dim], 16-byte aligned rows */
+  int64_t q_token_stride, q_head_stride;       /* elements, multiples of 8 */
+  const void* k_cache;          /* [num_blocks, block_size, num_kv_heads, head_dim] */
+  const void* v_cache;
+  const int32_t* cu_seqlens_q;  /* [n + 1] */
+  const int32_t* context_lens;  /* [n] */
+  const int32_t* block_table;   /* [n, max_blocks] */
+  const int32_t* prefix_lens;   /* [n] or NULL */
+  const int32_t* first_keys;    /* [tokens] or NULL */
+  const uint64_t* tree_masks;   /* [tokens] or NULL */
+  const float* slopes;          /* [num_heads] or NULL */
+  void* out;                    /* [tokens, num_heads, head_dim] */
+} DllmAppend;
+
+/* Workspace bytes for up to these bounds, 0 if the shape is not supported.
+ * Zero-fill the first 256 bytes once (the device error word); nothing else is
+ * kept from one call to the next.  Calls that may run at the same time need
+ * workspaces of their own. */
+size_t dllm_append_workspace_size(int32_t tokens, int32_t n, int32_t num_heads,
+                                  int32_t num_kv_heads, int32_t head_dim);
+
+/* Stream ordered, no allocation, no host synchronisation; the launches depend
+ * on the arguments but not on the lengths in device memory.  Lengths that make
+ * no sense, a block id out of range or a tree of more than 64 tokens set a
+ * device error bit (dllm_read_error); such a sequence's rows are zeros, or
+ * untouched where cu_seqlens_q itself is wrong, and such a block reads as zeros. */
+int dllm_append_attention(const DllmAppend* args, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

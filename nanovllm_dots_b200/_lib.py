@@ -1,6 +1,6 @@
 """ctypes binding of ``libdfm.so`` (declarations in ``include/dfm.h`` for the FM
-head, ``include/dpe.h`` for the patch encoder, ``include/dllm.h`` for the LLM
-decode attention and ``include/dvoc.h`` for the vocoder).
+head, ``include/dpe.h`` for the patch encoder, ``include/dllm.h`` for the LLM's
+decode, rotary and append attention and ``include/dvoc.h`` for the vocoder).
 
 The library is built in-tree by ``nanovllm_dots_b200.build``.  There is no
 fallback: if the shared object is missing or fails to load, every entry point
@@ -26,6 +26,7 @@ EXPORTS = ("dfm_create", "dfm_workspace_size", "dfm_pool_bytes", "dfm_step", "df
            "dpe_create", "dpe_workspace_size", "dpe_pool_bytes", "dpe_decode", "dpe_read_error",
            "dpe_destroy", "dllm_decode_workspace_size", "dllm_decode_attention", "dllm_read_error",
            "dllm_create", "dllm_step_workspace_size", "dllm_decode_step", "dllm_destroy",
+           "dllm_rotary", "dllm_append_workspace_size", "dllm_append_attention",
            "dvoc_create", "dvoc_destroy", "dvoc_conv_floats", "dvoc_bias_floats", "dvoc_act_floats",
            "dvoc_hop", "dvoc_stream_left_context", "dvoc_workspace_size", "dvoc_decode",
            "dvoc_read_error", "dvoc_num_convs", "dvoc_conv_launch")
@@ -99,6 +100,32 @@ class DllmStep(ctypes.Structure):
                 ("slot_mapping", c_void_p), ("context_lens", c_void_p), ("block_table", c_void_p),
                 ("k_caches", POINTER(c_void_p)), ("v_caches", POINTER(c_void_p)),
                 ("num_blocks", c_int32), ("out", c_void_p)]
+
+
+DLLM_BF16, DLLM_FP16, DLLM_FP32 = 0, 1, 2
+
+
+class DllmRotary(ctypes.Structure):
+    _fields_ = [("dtype", c_int32), ("tokens", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32),
+                ("head_dim", c_int32), ("rot_dim", c_int32), ("interleaved", c_int32),
+                ("factor", c_float), ("turns", c_void_p), ("positions", c_void_p), ("q", c_void_p),
+                ("q_out", c_void_p), ("k", c_void_p), ("v", c_void_p), ("k_cache", c_void_p),
+                ("v_cache", c_void_p), ("slot_mapping", c_void_p), ("q_token_stride", c_int64),
+                ("q_head_stride", c_int64), ("out_token_stride", c_int64),
+                ("out_head_stride", c_int64), ("k_token_stride", c_int64), ("k_head_stride", c_int64),
+                ("v_token_stride", c_int64), ("v_head_stride", c_int64), ("num_slots", c_int64),
+                ("err_word", c_void_p)]
+
+
+class DllmAppend(ctypes.Structure):
+    _fields_ = [("dtype", c_int32), ("tokens", c_int32), ("n", c_int32), ("num_heads", c_int32),
+                ("num_kv_heads", c_int32), ("head_dim", c_int32), ("num_blocks", c_int32),
+                ("block_size", c_int32), ("max_blocks", c_int32), ("causal", c_int32),
+                ("window", c_int32), ("scale", c_float), ("softcap", c_float), ("q", c_void_p),
+                ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("k_cache", c_void_p),
+                ("v_cache", c_void_p), ("cu_seqlens_q", c_void_p), ("context_lens", c_void_p),
+                ("block_table", c_void_p), ("prefix_lens", c_void_p), ("first_keys", c_void_p),
+                ("tree_masks", c_void_p), ("slopes", c_void_p), ("out", c_void_p)]
 
 
 DVOC_MAX_STAGES, DVOC_MAX_KERNELS = 8, 4
@@ -200,6 +227,12 @@ def lib() -> ctypes.CDLL:
     L.dllm_decode_step.restype = c_int32
     L.dllm_destroy.argtypes = [c_void_p]
     L.dllm_destroy.restype = c_int32
+    L.dllm_rotary.argtypes = [POINTER(DllmRotary), c_void_p]
+    L.dllm_rotary.restype = c_int32
+    L.dllm_append_workspace_size.argtypes = [c_int32] * 5
+    L.dllm_append_workspace_size.restype = c_size_t
+    L.dllm_append_attention.argtypes = [POINTER(DllmAppend), c_void_p, c_size_t, c_void_p]
+    L.dllm_append_attention.restype = c_int32
     L.dvoc_create.argtypes = [POINTER(DvocConfig), POINTER(DvocWeights), POINTER(c_void_p)]
     L.dvoc_create.restype = c_int32
     L.dvoc_destroy.argtypes = [c_void_p]

@@ -1,5 +1,5 @@
-"""Build the shared library (``libdfm.so``: FM head, patch encoder, LLM decode
-attention, vocoder) in-tree
+"""Build the shared library (``libdfm.so``: FM head, patch encoder, LLM decode,
+rotary and append attention, vocoder) in-tree
 with nvcc for sm_100a.
 
     python -m nanovllm_dots_b200.build
@@ -19,7 +19,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libdfm.so")
 SOURCES = ["dfm_api.cu"]
 DEPS = ["dfm_api.cu", "dpe_api.cu", "llm_api.cu", "common.cuh", "gemm.cuh", "attn_tc.cuh", "ew.cuh",
-        "pe.cuh", "llm_attn.cuh", "llm_step.cuh", "voc_api.cu", "voc.cuh"]
+        "pe.cuh", "llm_attn.cuh", "llm_step.cuh", "llm_append_api.cu", "llm_append.cuh", "llm_rotary.cuh",
+        "voc_api.cu", "voc.cuh"]
 HEADERS = [os.path.join(os.path.dirname(PKG), "include", h) for h in ("dfm.h", "dpe.h", "dllm.h", "dvoc.h")]
 
 

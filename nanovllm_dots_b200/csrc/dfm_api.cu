@@ -1003,5 +1003,8 @@ extern "C" int dfm_paged_attention_noalloc(const void* q, void* out, const void*
 // The LLM backbone's paged decode attention (include/dllm.h) shares them too.
 #include "llm_api.cu"
 
+// The LLM's rotary and append attention (include/dllm.h).
+#include "llm_append_api.cu"
+
 // The vocoder (include/dvoc.h).
 #include "voc_api.cu"

@@ -1,0 +1,945 @@
+// Append attention of the LLM backbone: new tokens of many sequences over the
+// paged K/V cache that already holds them (include/dllm.h,
+// dllm_append_attention).
+//
+// Row (token j of sequence i, query head h) sees the keys of one interval
+// [lo, hi) (causal, sliding window, bidirectional prefix and document masks all
+// are one) or, when a tree of drafted tokens is verified, the history [0, base)
+// and the drafted keys in the token's 64-bit mask:
+//   s_k = cap tanh(scale q.k / cap) - slope_h |p - k|     (cap and slope optional)
+//   o = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m),  zeros if the row sees no key.
+//
+// Work.  The G query heads of a kv head are packed with the tokens into rows,
+// row = token * G + head, RT = 128 / G tokens to a 128-row tile, so K and V are
+// read once for all of them and single tokens, trees and prompts take the same
+// path.  A unit is up to two row tiles of a sequence; its keys are taken in
+// tiles of 128, newest first (the tiles with masks first, and with a distance
+// bias the largest scores first).  The units of every kv head form one line of
+// key tiles, cut into equal shares for the persistent CTAs: a unit whose keys
+// fall into several shares leaves unnormalised partials that
+// llm_append_combine_kernel adds up in the order of the shares.
+//
+// One CTA per SM, 12 warps: two softmax warpgroups (a thread is a row), a TMA
+// warp, an MMA warp and two warps that look after V.  Each softmax warpgroup
+// works on a stream of its own (score tile S in TMEM, overwritten by the
+// probabilities P, and the accumulator O): the two row tiles of a wide unit
+// over every key tile, or the one row tile of a narrow unit over the even and
+// the odd key tiles, merged at the end.  One stream's softmax runs under the
+// other's products:
+//   S[128 x 128] = Q K^T      (Q and K from shared memory)
+//   O[128 x D]  += P V        (P from TMEM, V from shared memory)
+//
+// Keys nobody in the unit may see are not loaded (their pages may be gone) and
+// their rows of V are set to zero.  In a tile with masks, a visible row of V
+// that holds an infinity or a NaN is set to zero as well and noted: the rows
+// that see it become NaN, and no other row is touched (0 * inf in the product
+// would reach them all).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace dfm {
+
+constexpr int AP_KT = 128;          // keys per tile
+constexpr int AP_ROWS = 128;        // rows per tile (TMEM lanes)
+constexpr int AP_RING = 2;          // K tiles and V tiles in shared memory
+constexpr int AP_THREADS = 384;
+constexpr int AP_PLAN_THREADS = 1024;
+constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's key tile counts 2)
+// The running maximum of a row is raised only when a score passes it by this
+// much (log2 units): probabilities then reach 2^8, exact in fp32 and within
+// fp16's range, and O is seldom rescaled.
+constexpr float AP_TAU = 8.0f;
+
+struct ApUnit {
+  int seq, t0, ntok, row0;          // tokens [t0, t0 + ntok) of the sequence; row0: its first in q
+  int lo, hi, fmin, fmax;           // union of the rows' keys; tiles inside [fmin, fmax) have no mask
+  int base, narrow, cost, pad;      // position of token 0; one row tile only; place in the line
+  long long at;
+  long long pad2;
+};
+static_assert(sizeof(ApUnit) == 64, "unit record");
+
+struct ApHead {                     // the plan's header
+  long long line;                   // length of one kv head's line
+  long long share;                  // of one CTA
+  int units, pad;
+};
+
+struct ApParams {
+  const int* cu;                    // [n + 1]
+  const int* ctx;                   // [n]
+  const int* bt;                    // [n][max_blocks]
+  const int* prefix;                // [n] or null
+  const int* first;                 // [tokens] or null
+  const unsigned long long* tree;   // [tokens] or null
+  const float* slopes;              // [H] or null
+  void* out;                        // [tokens][H][D]
+  uint32_t* err;
+  ApHead* head;
+  ApUnit* units;
+  int* ubase;                       // [n + 1]
+  int* start;                       // [ctas + 1] unit at the start of each share
+  float* part_o;                    // [ctas][2][2][D / 4][128][4]
+  float2* part_ml;                  // [ctas][2][2][128]
+  int tokens, n, H, KVH, G, RT, max_units, ctas;
+  int num_blocks, block_size, max_blocks, box_rows;
+  int causal, window, fp16;
+  float scale_log2;                 // scale * log2(e)
+  float cap_in, cap_out;            // 2 log2(e) scale / cap and cap log2(e); cap_out 0: no cap
+};
+
+// ---------------------------------------------------------------- plan
+template <class T>
+DFM_DEV T block_exclusive_scan(T v, T* warp_sums, T& total) {   // AP_PLAN_THREADS threads
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  T x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    T w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const T y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  total = warp_sums[31];
+  const T before = warp ? warp_sums[warp - 1] : 0;
+  __syncthreads();
+  return before + x - v;
+}
+
+// Units, their keys and their places in the line, from the device's lengths.
+// A sequence whose lengths make no sense is reported: its rows are written as
+// zeros, or not at all when not even they are known.
+__global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApParams p) {
+  __shared__ int sums[32];
+  __shared__ long long lsums[32];
+  pdl_trigger();
+  pdl_wait();
+  const int t = threadIdx.x;
+  auto rows_ok = [&](int i, int& s0, int& m) {
+    s0 = p.cu[i];
+    const int s1 = p.cu[i + 1];
+    m = s1 - s0;
+    return s0 >= 0 && s1 >= s0 && s1 <= p.tokens;
+  };
+  int carry = 0;
+  for (int i0 = 0; i0 < p.n; i0 += AP_PLAN_THREADS) {
+    const int i = i0 + t;
+    int c = 0;
+    if (i < p.n) {
+      int s0, m;
+      if (rows_ok(i, s0, m)) {
+        c = (m + 2 * p.RT - 1) / (2 * p.RT);
+        const int ctx = p.ctx[i];
+        if (ctx < m || ctx > static_cast<long long>(p.max_blocks) * p.block_size || (p.tree && m > 64))
+          atomicOr(p.err, DFM_DEV_ERR_LEN);
+      } else {
+        atomicOr(p.err, DFM_DEV_ERR_LEN);
+      }
+    }
+    int total;
+    const int at = block_exclusive_scan(c, sums, total);
+    if (i < p.n) p.ubase[i] = carry + at;
+    carry += total;
+  }
+  int units = carry;
+  if (units > p.max_units) {   // rows of overlapping sequences
+    if (t == 0) atomicOr(p.err, DFM_DEV_ERR_LEN);
+    units = p.max_units;
+  }
+  __syncthreads();   // ubase, written by this block, is read below
+  long long line = 0;
+  for (int u0 = 0; u0 < units; u0 += AP_PLAN_THREADS) {
+    const int u = u0 + t;
+    ApUnit f{};
+    if (u < units) {
+      int a = 0, b = p.n - 1;    // the last sequence with ubase <= u (those without units share a value)
+      while (a < b) {
+        const int mid = (a + b + 1) >> 1;
+        if (p.ubase[mid] <= u) a = mid; else b = mid - 1;
+      }
+      int s0, m;
+      rows_ok(a, s0, m);
+      const int ctx = p.ctx[a];
+      f.seq = a;
+      f.t0 = (u - p.ubase[a]) * 2 * p.RT;
+      f.ntok = min(2 * p.RT, m - f.t0);
+      f.row0 = s0;
+      f.base = ctx - m;
+      f.narrow = f.ntok <= p.RT;
+      f.lo = f.hi = 0;
+      f.fmin = 0x7fffffff;
+      f.fmax = 0;
+      if (ctx >= m && ctx <= static_cast<long long>(p.max_blocks) * p.block_size && !(p.tree && m > 64)) {
+        if (p.tree) {
+          f.hi = ctx;
+          f.fmin = 0;
+          f.fmax = f.base;
+        } else {
+          const int pre = p.prefix ? min(p.prefix[a], ctx) : 0;
+          int lo = 0x7fffffff, hi = 0, fmin = 0, fmax = 0x7fffffff;
+          // without per-token bounds the ends of the interval rise with the token
+          const int step = p.first ? 1 : max(1, f.ntok - 1);
+          for (int j = f.t0; j < f.t0 + f.ntok; j += step) {
+            const int pos = f.base + j;
+            const int h = p.causal ? max(pos + 1, pre) : ctx;
+            int l = p.window ? max(0, pos + 1 - p.window) : 0;
+            if (p.first) l = max(l, p.first[s0 + j]);
+            if (l < h) {
+              lo = min(lo, l);
+              hi = max(hi, h);
+            }
+            fmin = max(fmin, l);
+            fmax = min(fmax, h);
+          }
+          if (hi > 0) {
+            f.lo = lo;
+            f.hi = hi;
+            f.fmin = fmin;
+            f.fmax = fmax;
+          }
+        }
+      }
+      const int tiles = f.hi > f.lo ? (f.hi + AP_KT - 1) / AP_KT - f.lo / AP_KT : 0;
+      f.cost = max(1, tiles * (f.narrow ? 1 : 2));
+    }
+    long long total;
+    f.at = line + block_exclusive_scan(static_cast<long long>(f.cost), lsums, total);
+    if (u < units) p.units[u] = f;
+    line += total;
+  }
+  long long share = (line * p.KVH + p.ctas - 1) / p.ctas;
+  if (share < AP_MIN_SHARE) share = AP_MIN_SHARE;
+  if (t == 0) {
+    p.head->line = line;
+    p.head->share = share;
+    p.head->units = units;
+  }
+  // the unit at the start of each share
+  for (int u = t; u < units; u += AP_PLAN_THREADS) {
+    const ApUnit& f = p.units[u];
+    for (int kv = 0; kv < p.KVH; ++kv) {
+      const long long a = kv * line + f.at, b = a + f.cost;
+      for (long long c = (a + share - 1) / share; c * share < b; ++c)
+        if (c <= p.ctas) p.start[c] = u;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- a CTA's segments
+// A segment: key tiles [i0, i1) of a unit (0 is the newest) for one kv head.
+struct ApSegment {
+  ApUnit f;
+  int kv, i0, i1, tiles, top;       // tiles of the whole unit; key tile of i = top - i
+  DFM_DEV bool whole() const { return i0 == 0 && i1 == tiles; }
+};
+
+struct ApWalk {
+  long long left, line;
+  int u, kv, units;
+  long long off;                    // into the unit
+
+  DFM_DEV ApWalk(const ApParams& p) {
+    line = p.head->line;
+    units = p.head->units;
+    const long long share = p.head->share, all = line * p.KVH;
+    const long long g = blockIdx.x * share;
+    left = g < all ? (g + share < all ? share : all - g) : 0;
+    if (left > 0) {
+      kv = static_cast<int>(g / line);
+      u = p.start[blockIdx.x];
+      off = g - kv * line - p.units[u].at;
+    }
+  }
+  // The next segment with work; false at the end of the share.
+  DFM_DEV bool next(const ApParams& p, ApSegment& s) {
+    while (left > 0) {
+      s.f = p.units[u];
+      s.kv = kv;
+      const int c = s.f.narrow ? 1 : 2;
+      s.tiles = s.f.hi > s.f.lo ? (s.f.hi + AP_KT - 1) / AP_KT - s.f.lo / AP_KT : 0;
+      s.top = (s.f.hi + AP_KT - 1) / AP_KT - 1;
+      const long long end = off + left < s.f.cost ? off + left : s.f.cost;
+      s.i0 = static_cast<int>((off + c - 1) / c);
+      s.i1 = min(s.tiles, static_cast<int>((end + c - 1) / c));
+      const bool zero = s.tiles == 0 && off == 0;
+      left -= end - off;
+      off = end;
+      if (end == s.f.cost) {
+        off = 0;
+        if (++u == units) {
+          u = 0;
+          ++kv;
+        }
+      }
+      if (zero) s.i0 = s.i1 = 0;
+      if (zero || s.i1 > s.i0) return true;
+    }
+    return false;
+  }
+};
+
+// ---------------------------------------------------------------- shared memory
+template <int D>
+struct ApSmem {
+  static constexpr int BOXES = D / 64;
+  static constexpr int TILE = AP_KT * D * 2;              // one K, V or Q tile
+  static constexpr int HALF = AP_KT * 128;                // its 64-dim boxes
+  static constexpr int OFF_Q = 0;                         // [2]
+  static constexpr int OFF_K = OFF_Q + 2 * TILE;          // [AP_RING]
+  static constexpr int OFF_V = OFF_K + AP_RING * TILE;    // [AP_RING]
+  static constexpr int OFF_OUT = OFF_V + AP_RING * TILE;  // [8 warps][32 rows][64 bytes]
+  static constexpr int OFF_ML = OFF_OUT + 8 * 32 * 64;   // float2 [2][128]
+  static constexpr int OFF_BAR = OFF_ML + 2 * AP_ROWS * 8;
+  static constexpr int BYTES = OFF_BAR + 512 + 1024;
+};
+static_assert(ApSmem<128>::BYTES <= 232448, "one CTA per SM");
+
+// D(tmem) (+)= A(tmem) * B(smem, MN-major), 16-bit inputs, fp32 accumulate.
+DFM_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                         uint32_t accumulate) {
+  const uint32_t z = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(
+          d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z)
+      : "memory");
+}
+
+// Wait with the time limit alone, whatever the abort flag says (the way out of
+// an aborted CTA, whose copies and products are still in flight).
+DFM_DEV void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 <= DFM_WAIT_LIMIT_NS) {
+  }
+}
+
+// Barrier over the 256 softmax threads; the AND of their predicates.
+DFM_DEV bool ap_pair_sync(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
+}
+
+DFM_DEV uint32_t ap_pack(float a, float b, bool fp16) {
+  if (fp16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return pack_bf16(a, b);
+}
+
+// The lowest n bits, n clamped to [0, 32].
+DFM_DEV uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Whether a 32-bit word of two 16-bit floats holds an infinity or a NaN.
+DFM_DEV bool ap_special(uint32_t w, uint32_t exp_lo) {
+  return (w & exp_lo) == exp_lo || (w & (exp_lo << 16)) == (exp_lo << 16);
+}
+
+// ---------------------------------------------------------------- the kernel
+// kMod: a cap or a distance bias on the scores.
+template <int D, bool kMod>
+__global__ void __launch_bounds__(AP_THREADS, 1)
+    llm_append_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const ApParams p) {
+  using S = ApSmem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem + S::OFF_Q;
+  uint8_t* sK = smem + S::OFF_K;
+  uint8_t* sV = smem + S::OFF_V;
+  float2* sML = reinterpret_cast<float2*>(smem + S::OFF_ML);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
+  uint64_t* k_empty = k_full + AP_RING;
+  uint64_t* v_full = k_empty + AP_RING;
+  uint64_t* v_ready = v_full + AP_RING;   // V without special values: arrivals of its two warps
+  uint64_t* v_empty = v_ready + AP_RING;
+  uint64_t* s_full = v_empty + AP_RING;   // [2] per stream
+  uint64_t* p_full = s_full + 2;          // [2] arrivals of the stream's four warps
+  uint64_t* o_full = p_full + 2;          // [2]
+  uint64_t* q_full = o_full + 2;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* drain = q_empty + 1;
+  uint32_t* poison = reinterpret_cast<uint32_t*>(drain + 1);   // [AP_RING][4]
+  uint32_t* tmem_slot = poison + AP_RING * 4;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((5 * AP_RING + 9) * 8 + AP_RING * 16 + 8 <= 512, "barrier area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < AP_RING; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_ready[i], 2);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch(&tm_q);
+    tma_prefetch(&tm_k);
+    tma_prefetch(&tm_v);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+  ApWalk walk(p);
+  ApSegment sg;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA
+    const int per_tile = AP_KT / p.box_rows;         // boxes along the keys
+    const int box_bytes = p.box_rows * 128;
+    int g = 0, nseg = 0;
+    bool ok = true;
+    while (ok && walk.next(p, sg)) {
+      if (sg.i1 == sg.i0) continue;
+      if (lane == 0) {
+        ok = nseg == 0 || mbar_wait(q_empty, (nseg - 1) & 1, abort_flag, p.err);
+        if (ok) {
+          const int nt = sg.f.narrow ? 1 : 2;
+          mbar_arrive_expect_tx(q_full, nt * S::BOXES * p.G * p.RT * 128);
+          for (int x = 0; x < nt; ++x)
+            for (int b = 0; b < S::BOXES; ++b)
+              tma_load_3d(sQ + x * S::TILE + b * S::HALF, &tm_q, q_full, b * 64, sg.kv * p.G,
+                          sg.f.row0 + sg.f.t0 + x * p.RT);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ++nseg;
+      const int* bt = p.bt + static_cast<size_t>(sg.f.seq) * p.max_blocks;
+      // lane = (box along the keys, 64-dim half); lanes past the tile's boxes are idle
+      const int box = lane / S::BOXES, half = lane % S::BOXES;
+      auto block_of = [&](int i) {   // the lane's cache block in tile i, -2 if nobody sees the box
+        const int key = (sg.top - i) * AP_KT + box * p.box_rows;
+        if (box >= per_tile || i >= sg.i1 || key + p.box_rows <= sg.f.lo || key >= sg.f.hi) return -2;
+        return bt[key / p.block_size];
+      };
+      int blk = block_of(sg.i0);
+      for (int i = sg.i0; ok && i < sg.i1; ++i, ++g) {
+        const int slot = g % AP_RING;
+        const int key = (sg.top - i) * AP_KT + box * p.box_rows;
+        const bool mine = blk != -2;
+        int cb = blk;
+        if (mine && (cb < 0 || cb >= p.num_blocks)) {
+          if (half == 0) atomicOr(p.err, DFM_DEV_ERR_PAGE);
+          cb = p.num_blocks;   // out of range: zeros
+        }
+        const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box_bytes;
+        blk = block_of(i + 1);
+        const int row = key % p.block_size;
+        const int dst = slot * S::TILE + half * S::HALF + box * box_bytes;
+        if (lane == 0) {
+          ok = g < AP_RING || mbar_wait(&k_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
+          if (ok) mbar_arrive_expect_tx(&k_full[slot], bytes);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (mine) tma_load_4d(sK + dst, &tm_k, &k_full[slot], half * 64, sg.kv, row, cb);
+        if (lane == 0) {
+          ok = g < AP_RING || mbar_wait(&v_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
+          if (ok) mbar_arrive_expect_tx(&v_full[slot], bytes);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) {
+          ++g;
+          break;
+        }
+        if (mine) tma_load_4d(sV + dst, &tm_v, &v_full[slot], half * 64, sg.kv, row, cb);
+      }
+    }
+    if (!ok && lane == 0) {
+      // copies that nobody waited for must land before the CTA's memory is gone
+      if (nseg > 0) mbar_drain(q_full, (nseg - 1) & 1);
+      for (int x = g > AP_RING ? g - AP_RING : 0; x < g; ++x) {
+        mbar_drain(&k_full[x % AP_RING], (x / AP_RING) & 1);
+        mbar_drain(&v_full[x % AP_RING], (x / AP_RING) & 1);
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0) {
+      const uint32_t fmt = p.fp16 ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t base = (1u << 4) | fmt | (static_cast<uint32_t>(AP_ROWS >> 4) << 24);
+      const uint32_t idesc_s = base | (static_cast<uint32_t>(AP_KT >> 3) << 17);
+      const uint32_t idesc_o = base | (static_cast<uint32_t>(D >> 3) << 17) | (1u << 16);
+      int g = 0, nseg = 0;
+      int np[2] = {0, 0};        // probability tiles taken per stream
+      bool ok = true;
+      // S_s = Q_x K^T for the K tile of ring position `at`
+      auto scores = [&](int s, int x, int at) {
+        const uint32_t q = smem_u32(sQ + x * S::TILE), k = smem_u32(sK + (at % AP_RING) * S::TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int o = (kk >> 2) * S::HALF + (kk & 3) * 32;
+          umma_bf16(tmem + s * AP_KT, umma_desc_sw128(q + o), umma_desc_sw128(k + o), idesc_s, kk > 0);
+        }
+        umma_commit(&s_full[s]);
+      };
+      auto k_wait = [&](int at) {
+        ok = ok && mbar_wait(&k_full[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err);
+        tc_fence_after();
+      };
+      // O_s += P_s V
+      auto values = [&](int s, int at, bool first) {
+        ok = ok && mbar_wait(&p_full[s], np[s] & 1, abort_flag, p.err) &&
+             mbar_wait(&v_ready[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err);
+        ++np[s];
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t v = smem_u32(sV + (at % AP_RING) * S::TILE);
+#pragma unroll
+        for (int kk = 0; kk < AP_KT / 16; ++kk)
+          umma_f16_ts(tmem + 256 + s * D, tmem + s * AP_KT + kk * 8,
+                      umma_desc_sw128_mn(v + kk * 2048, S::HALF), idesc_o, !first || kk > 0);
+      };
+      while (ok && walk.next(p, sg)) {
+        const int nt = sg.i1 - sg.i0;
+        if (nt == 0) continue;
+        ok = mbar_wait(q_full, nseg & 1, abort_flag, p.err);
+        ++nseg;
+        if (sg.f.narrow) {
+          for (int i = 0; i < 2 && i < nt; ++i) {
+            k_wait(g + i);
+            if (!ok) break;
+            scores(i, 0, g + i);
+            umma_commit(&k_empty[(g + i) % AP_RING]);
+            if (i == nt - 1) umma_commit(q_empty);
+          }
+          for (int i = 0; ok && i < nt; ++i) {
+            const int s = i & 1;
+            values(s, g + i, i < 2);
+            if (!ok) break;
+            umma_commit(&v_empty[(g + i) % AP_RING]);
+            if (i + 2 >= nt) umma_commit(&o_full[s]);
+            if (i + 2 < nt) {
+              k_wait(g + i + 2);
+              if (!ok) break;
+              scores(s, 0, g + i + 2);
+              umma_commit(&k_empty[(g + i + 2) % AP_RING]);
+              if (i + 2 == nt - 1) umma_commit(q_empty);
+            }
+          }
+        } else {
+          k_wait(g);
+          if (!ok) break;
+          scores(0, 0, g);
+          scores(1, 1, g);
+          umma_commit(&k_empty[g % AP_RING]);
+          if (nt == 1) umma_commit(q_empty);
+          for (int i = 0; ok && i < nt; ++i) {
+            for (int s = 0; s < 2; ++s) {
+              values(s, g + i, i == 0);
+              if (!ok) break;
+              if (s == 1) umma_commit(&v_empty[(g + i) % AP_RING]);
+              if (i == nt - 1) {
+                umma_commit(&o_full[s]);
+                continue;
+              }
+              if (s == 0) k_wait(g + i + 1);
+              if (!ok) break;
+              scores(s, s, g + i + 1);
+              if (s == 1) {
+                umma_commit(&k_empty[(g + i + 1) % AP_RING]);
+                if (i + 1 == nt - 1) umma_commit(q_empty);
+              }
+            }
+          }
+        }
+        g += nt;
+      }
+      if (!ok) {   // products in flight read shared memory and TMEM
+        umma_commit(drain);
+        mbar_drain(drain, 0);
+      }
+    }
+  } else if (warp >= 10) {
+    // ------------------------------------------------------------ special rows of V
+    const int w = warp - 10;
+    const uint32_t exp_lo = p.fp16 ? 0x7c00u : 0x7f80u;
+    int g = 0;
+    bool ok = true;
+    while (ok && walk.next(p, sg)) {
+      for (int i = sg.i0; i < sg.i1; ++i, ++g) {
+        const int slot = g % AP_RING;
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[slot], (g / AP_RING) & 1, abort_flag, p.err));
+        if (!ok) break;
+        const int k0 = (sg.top - i) * AP_KT;
+        if (k0 < sg.f.fmin || k0 + AP_KT > sg.f.fmax) {
+          for (int x = 0; x < 2; ++x) {
+            const int r = w * 64 + x * 32 + lane, key = k0 + r;
+            uint8_t* row = sV + slot * S::TILE + r * 128;
+            const bool seen = key >= sg.f.lo && key < sg.f.hi;
+            bool special = false;
+            if (seen) {
+#pragma unroll
+              for (int b = 0; b < S::BOXES; ++b)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                  const uint4 u = *reinterpret_cast<const uint4*>(row + b * S::HALF + ((c ^ (r & 7)) << 4));
+                  special |= ap_special(u.x, exp_lo) | ap_special(u.y, exp_lo) |
+                             ap_special(u.z, exp_lo) | ap_special(u.w, exp_lo);
+                }
+            }
+            if (!seen || special) {
+#pragma unroll
+              for (int b = 0; b < S::BOXES; ++b)
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                  *reinterpret_cast<uint4*>(row + b * S::HALF + (c << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            const uint32_t word = __ballot_sync(0xffffffffu, special);
+            if (lane == 0) poison[slot * 4 + w * 2 + x] = word;
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ready[slot]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int s = warp >> 2;                           // stream
+    const int r = (warp & 3) * 32 + lane;              // row of the tile, TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + s * AP_KT + lane_off, tO = tmem + 256 + lane_off;
+    const int tok_of = r / p.G, head_of = r % p.G;
+    uint8_t* stage = smem + S::OFF_OUT + warp * 32 * 64;
+    int g = 0, ns = 0;                                 // V tiles of the CTA, score tiles of the stream
+    int no[2] = {0, 0};                                // segments each stream had tiles in
+    bool ok = true;
+    while (walk.next(p, sg)) {
+      const int nt = sg.i1 - sg.i0;
+      const bool narrow = sg.f.narrow;
+      // this thread's row
+      const int j = sg.f.t0 + (narrow ? 0 : s * p.RT) + tok_of;
+      const bool valid = tok_of < p.RT && j < sg.f.t0 + sg.f.ntok;
+      const bool warp_valid = __any_sync(0xffffffffu, valid);
+      const int pos = sg.f.base + j;
+      int lo = 0, hi = 0;
+      unsigned long long bits = 0;
+      float slope = 0.f;
+      if (valid) {
+        if (p.tree) {
+          const int m = p.ctx[sg.f.seq] - sg.f.base;
+          bits = p.tree[sg.f.row0 + j] & (m >= 64 ? ~0ull : (1ull << m) - 1);
+          hi = sg.f.base;
+        } else {
+          const int ctx = p.ctx[sg.f.seq];
+          hi = p.causal ? max(pos + 1, p.prefix ? min(p.prefix[sg.f.seq], ctx) : 0) : ctx;
+          lo = p.window ? max(0, pos + 1 - p.window) : 0;
+          if (p.first) lo = max(lo, p.first[sg.f.row0 + j]);
+        }
+        if (kMod && p.slopes) slope = p.slopes[sg.kv * p.G + head_of] * 1.4426950408889634f;
+      }
+      float m = -INFINITY, l = 0.f;
+      const int step = narrow ? 2 : 1, i_first = narrow ? s : 0;
+#pragma unroll 1
+      for (int i = i_first; ok && i < nt; i += step, ++ns) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], ns & 1, abort_flag, p.err));
+        if (!ok) break;
+        tc_fence_after();
+        const int k0 = (sg.top - sg.i0 - i) * AP_KT;
+        const bool full = k0 >= sg.f.fmin && k0 + AP_KT <= sg.f.fmax;
+        if (!full) {
+          const int slot = (g + i) % AP_RING;
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
+          if (!ok) break;
+        }
+        if (warp_valid) {
+          float x[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c]));
+          tmem_wait_ld();
+          float scale = p.scale_log2;
+          if constexpr (kMod) {
+            if (p.cap_out > 0.f) {
+              // cap tanh(y): tanh y = 1 - 2 / (1 + e^{2y})
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  x[c][e] = p.cap_out * (1.f - __fdividef(2.f, 1.f + fast_exp2(x[c][e] * p.cap_in)));
+            } else {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[c][e] *= p.scale_log2;
+            }
+            if (p.slopes) {
+              const float d0 = static_cast<float>(pos - k0);
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  x[c][e] = fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), x[c][e]);
+            }
+            scale = 1.f;
+          }
+          if (!full) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t see = low_bits(hi - k0 - c * 32) & ~low_bits(lo - k0 - c * 32);
+              const int o = sg.f.base - k0 - c * 32;   // drafted token 0's bit in this word
+              if (bits) see |= o >= 32 || o <= -64 ? 0u
+                               : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
+              bad |= see & poison[((g + i) % AP_RING) * 4 + c];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[c][e] = (see >> e) & 1 ? x[c][e] : -INFINITY;
+            }
+            if (bad) l = __int_as_float(0x7fffffff);
+          }
+          float top[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            top[c] = x[c][0];
+#pragma unroll
+            for (int e = 1; e < 32; ++e) top[c] = fmaxf(top[c], x[c][e]);
+          }
+          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+          if (i == i_first) {
+            m = mt;
+          } else if (__any_sync(0xffffffffu, mt > m + AP_TAU)) {
+            // the stream's last product is done: this tile's scores came after it
+            const float mn = fmaxf(m, mt);
+            const float a = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+            l *= a;
+            m = mn;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(tO + s * D + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+              tmem_st32(tO + s * D + c, o);
+            }
+          }
+          const float ms = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const float a = fast_exp2(fmaf(x[c + (e >> 5)][e & 31], scale, -ms));
+              const float b = fast_exp2(fmaf(x[c + (e >> 5)][(e & 31) + 1], scale, -ms));
+              sum[(e >> 1) & 3] += a + b;
+              pk[e >> 1] = ap_pack(a, b, p.fp16);
+            }
+            tmem_st32(tS + c * 16, pk);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[s]);
+      }
+      // ------------------------------------------------ the segment's rows
+      const int n0 = narrow ? (nt + 1) / 2 : nt, n1 = narrow ? nt / 2 : nt;
+      float w0 = 1.f, w1 = 0.f;       // weights of O_0 and O_1 (narrow)
+      if (narrow) {
+        sML[s * AP_ROWS + r] = make_float2(m, l);
+        ok = ap_pair_sync(ok);
+        const float2 o = sML[(1 - s) * AP_ROWS + r];
+        const float mm = fmaxf(m, o.x);
+        const float wm = m == -INFINITY ? 0.f : fast_exp2(m - mm), wo = o.x == -INFINITY ? 0.f : fast_exp2(o.x - mm);
+        w0 = s ? wo : wm;
+        w1 = s ? wm : wo;
+        l = __fadd_rn(__fmul_rn(l, wm), __fmul_rn(o.y, wo));   // the same in both warpgroups
+        m = mm;
+      }
+      if (ok && n0 > 0 && (narrow || s == 0))
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[0], no[0] & 1, abort_flag, p.err));
+      if (ok && n1 > 0 && (narrow || s == 1))
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[1], no[1] & 1, abort_flag, p.err));
+      no[0] += n0 > 0;
+      no[1] += n1 > 0;
+      g += nt;
+      if (ok) {
+        tc_fence_after();
+        // columns of this warpgroup: all of its own tile's, or half of the shared one's
+        const int c_lo = narrow ? s * (D / 2) : 0, c_hi = narrow ? c_lo + D / 2 : D;
+        const bool whole = sg.whole();
+        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const int slot = blockIdx.x * 2 + (sg.i0 > 0 ? 0 : 1);
+        const int tile = narrow ? 0 : s;
+        float* po = p.part_o + (static_cast<size_t>(slot) * 2 + tile) * AP_ROWS * D;
+        if (!whole && (!narrow || s == 0))
+          p.part_ml[(static_cast<size_t>(slot) * 2 + tile) * AP_ROWS + r] = make_float2(m, l);
+        const long long row_off =
+            valid ? (static_cast<long long>(sg.f.row0 + j) * p.H + sg.kv * p.G + head_of) * D : -1;
+        if (warp_valid) {
+#pragma unroll 1
+          for (int c = c_lo; c < c_hi; c += 32) {
+            uint32_t o[32], o1[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = o1[e] = 0u;
+            if (narrow) {
+              if (n0 > 0) tmem_ld32(tO + c, o);
+              if (n1 > 0) tmem_ld32(tO + D + c, o1);
+            } else if (nt > 0) {
+              tmem_ld32(tO + s * D + c, o);
+            }
+            tmem_wait_ld();
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = narrow ? __uint_as_float(o[e]) * w0 + __uint_as_float(o1[e]) * w1 : __uint_as_float(o[e]);
+            if (!whole) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(po + (static_cast<size_t>((c + e) >> 2) * AP_ROWS + r) * 4) =
+                    make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+              continue;
+            }
+            // through shared memory, so that the warp writes whole rows: 32 rows of 64 bytes
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(ap_pack(v[8 * e] * inv, v[8 * e + 1] * inv, p.fp16),
+                             ap_pack(v[8 * e + 2] * inv, v[8 * e + 3] * inv, p.fp16),
+                             ap_pack(v[8 * e + 4] * inv, v[8 * e + 5] * inv, p.fp16),
+                             ap_pack(v[8 * e + 6] * inv, v[8 * e + 7] * inv, p.fp16));
+            __syncwarp();
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+              const int rr = it * 8 + (lane >> 2), e = lane & 3;
+              const long long off = __shfl_sync(0xffffffffu, row_off, rr);
+              const uint4 u = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((e ^ ((rr >> 1) & 3)) << 4));
+              if (off >= 0)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + off + c + e * 8) = u;
+            }
+            __syncwarp();
+          }
+        }
+      }
+      tc_fence_before();
+      if (narrow) ok = ap_pair_sync(ok);   // both have read O_0 and O_1
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- split units
+// Block (b, y): the unit that the end of share b cuts, if it began in share b,
+// rows and columns [y * 256, (y + 1) * 256) of its (tile, 16-dim group, row)
+// list.  out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the shares.
+template <int D>
+__global__ void __launch_bounds__(256) llm_append_combine_kernel(const ApParams p) {
+  constexpr int CB = 4;
+  pdl_trigger();
+  pdl_wait();
+  const long long line = p.head->line, share = p.head->share;
+  const int b = blockIdx.x;
+  const long long cut = (b + 1) * share;
+  if (cut >= line * p.KVH) return;
+  const int kv = static_cast<int>(cut / line);
+  const ApUnit f = p.units[p.start[b + 1]];
+  const long long begin = kv * line + f.at;
+  const int tiles = f.hi > f.lo ? (f.hi + AP_KT - 1) / AP_KT - f.lo / AP_KT : 0;
+  if (begin >= cut || begin / share != b || tiles == 0) return;
+  const int last = static_cast<int>((begin + (f.narrow ? 1 : 2) * (tiles - 1)) / share);
+  if (last == b) return;
+  const int task = blockIdx.y * 256 + threadIdx.x;
+  const int r = task % AP_ROWS, rest = task / AP_ROWS;
+  const int dg = rest % (D / 16), tile = rest / (D / 16);
+  if (tile > (f.narrow ? 0 : 1)) return;
+  const int tok = r / p.G, j = f.t0 + tile * p.RT + tok;
+  if (tok >= p.RT || j >= f.t0 + f.ntok) return;
+  float M = -INFINITY, L = 0.f, acc[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  for (int c0 = b; c0 <= last; c0 += CB) {
+    float2 ml[CB];
+    float4 o[CB][4];
+#pragma unroll
+    for (int x = 0; x < CB; ++x) {
+      const int c = c0 + x;
+      ml[x] = make_float2(-INFINITY, 0.f);
+      if (c > last) continue;
+      const size_t at = (static_cast<size_t>(c) * 2 + (c == b ? 1 : 0)) * 2 + tile;
+      ml[x] = p.part_ml[at * AP_ROWS + r];
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + at * AP_ROWS * D) + dg * 4 * AP_ROWS + r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[x][e] = src[e * AP_ROWS];
+    }
+    float Mn = M;
+#pragma unroll
+    for (int x = 0; x < CB; ++x) Mn = fmaxf(Mn, ml[x].x);
+    const float a = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
+    L *= a;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] *= a;
+#pragma unroll
+    for (int x = 0; x < CB; ++x) {
+      if (c0 + x > last) continue;
+      const float w = ml[x].x == -INFINITY ? 0.f : fast_exp2(ml[x].x - Mn);
+      L += w * ml[x].y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[4 * e] += w * o[x][e].x;
+        acc[4 * e + 1] += w * o[x][e].y;
+        acc[4 * e + 2] += w * o[x][e].z;
+        acc[4 * e + 3] += w * o[x][e].w;
+      }
+    }
+    M = Mn;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint32_t pk[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) pk[e] = ap_pack(acc[2 * e] * inv, acc[2 * e + 1] * inv, p.fp16);
+  uint4* dst = reinterpret_cast<uint4*>(
+      static_cast<uint16_t*>(p.out) +
+      (static_cast<size_t>(f.row0 + j) * p.H + kv * p.G + r % p.G) * D + dg * 16);
+  dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+  dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+}
+
+}  // namespace dfm

@@ -1,0 +1,256 @@
+// Host side of the rotary and append-attention C ABI (include/dllm.h).
+// Compiled inside dfm_api.cu's translation unit, after llm_api.cu, whose helpers
+// it uses.
+#include "llm_append.cuh"
+#include "llm_rotary.cuh"
+
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// ---------------------------------------------------------------- rotary
+template <typename T, bool INTER>
+cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t s) {
+  constexpr int VP = 16 / sizeof(T);
+  const long long heads = p.heads + (p.slots ? 2 * p.kv_heads : 0);
+  auto strides_ok = [](std::initializer_list<long long> v) {
+    for (long long x : v)
+      if (x % VP) return false;
+    return true;
+  };
+  bool vec = p.D % (2 * VP) == 0 && (p.rot / 2) % VP == 0 && aligned16(p.q) && aligned16(p.q_out) &&
+             strides_ok({p.q_ts, p.q_hs, p.o_ts, p.o_hs});
+  if (p.slots)
+    vec = vec && aligned16(p.k) && aligned16(p.v) && aligned16(p.k_cache) && aligned16(p.v_cache) &&
+          strides_ok({p.k_ts, p.k_hs, p.v_ts, p.v_hs});
+  auto blocks = [](long long threads) { return (threads + RO_THREADS - 1) / RO_THREADS; };
+  if (!vec) {
+    const long long nb = blocks(p.tokens * heads * ((p.D + 1) / 2));
+    if (nb > 0x7fffffffll) return cudaErrorInvalidValue;
+    return launch_pdl(llm_rotary_scalar_kernel<T, INTER>, dim3(static_cast<unsigned>(nb)),
+                      dim3(RO_THREADS), 0, s, p);
+  }
+  // a thread's angles serve 4 heads once there are threads enough to fill the GPU without
+  const long long lanes = p.D / (2 * VP), one = p.tokens * heads * lanes;
+  const bool four = one > 4ll * sm_count() * 2048;
+  const long long nb = blocks(four ? p.tokens * ((heads + 3) / 4) * lanes : one);
+  if (nb > 0x7fffffffll) return cudaErrorInvalidValue;
+  return launch_pdl(four ? llm_rotary_kernel<T, INTER, 4> : llm_rotary_kernel<T, INTER, 1>,
+                    dim3(static_cast<unsigned>(nb)), dim3(RO_THREADS), 0, s, p);
+}
+
+// ---------------------------------------------------------------- append attention
+struct ApWs {
+  size_t head, units, ubase, start, part_ml, part_o, total;
+};
+
+int ap_max_units(int tokens, int n, int RT) {
+  const long long u = (static_cast<long long>(tokens) + 2 * RT - 1) / (2 * RT) + n;
+  return u > 0x7fffffff ? 0 : static_cast<int>(u);
+}
+
+ApWs ap_ws(int tokens, int n, int G, int D, int ctas) {
+  auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+  ApWs w;
+  w.head = 256;   // after the error word
+  w.units = w.head + 256;
+  w.ubase = w.units + up(sizeof(ApUnit) * static_cast<size_t>(ap_max_units(tokens, n, AP_ROWS / G)));
+  w.start = w.ubase + up(4 * (static_cast<size_t>(n) + 1));
+  w.part_ml = w.start + up(4 * (static_cast<size_t>(ctas) + 1));
+  w.part_o = w.part_ml + up(static_cast<size_t>(ctas) * 4 * AP_ROWS * sizeof(float2));
+  w.total = w.part_o + static_cast<size_t>(ctas) * 4 * AP_ROWS * D * 4;
+  return w;
+}
+
+bool ap_shape_ok(int tokens, int n, int H, int KVH, int D) {
+  return tokens >= 0 && n >= 1 && H >= 1 && KVH >= 1 && H % KVH == 0 && H / KVH <= AP_ROWS &&
+         (D == 64 || D == 128) && ap_max_units(tokens, n, AP_ROWS / (H / KVH)) > 0;
+}
+
+// A paged cache as [num_blocks][block_size][kv_heads][D]: boxes of 64 dims x
+// `rows` positions of one block.
+bool map_ap_cache(CUtensorMap* m, const DllmAppend& a, const void* base, int rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t D = a.head_dim, KVH = a.num_kv_heads, bs = a.block_size;
+  cuuint64_t dims[4] = {D, KVH, bs, static_cast<cuuint64_t>(a.num_blocks)};
+  cuuint64_t strides[3] = {D * 2, KVH * D * 2, bs * KVH * D * 2};
+  cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  return fn(m, a.dtype == DLLM_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            4, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The queries as [tokens][H][D]: a box is the G heads of one kv head of RT tokens.
+bool map_ap_q(CUtensorMap* m, const DllmAppend& a, int G, int RT) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.num_heads),
+                        static_cast<cuuint64_t>(a.tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.q_head_stride) * 2,
+                           static_cast<cuuint64_t>(a.q_token_stride) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(RT)};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, a.dtype == DLLM_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            3, const_cast<void*>(a.q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+cudaError_t launch_append(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                          const ApParams& p, cudaStream_t s) {
+  static std::atomic<uint64_t> done_plain{0}, done_mod{0};
+  constexpr int smem = ApSmem<D>::BYTES;
+  const bool mod = p.cap_out > 0.f || p.slopes;
+  cudaError_t r = mod ? smem_attr_once(done_mod, llm_append_kernel<D, true>, smem)
+                      : smem_attr_once(done_plain, llm_append_kernel<D, false>, smem);
+  if (r != cudaSuccess) return r;
+  r = launch_pdl(llm_append_plan_kernel, dim3(1), dim3(AP_PLAN_THREADS), 0, s, p);
+  if (r != cudaSuccess) return r;
+  r = launch_pdl(mod ? llm_append_kernel<D, true> : llm_append_kernel<D, false>, dim3(p.ctas),
+                 dim3(AP_THREADS), smem, s, q, k, v, p);
+  if (r != cudaSuccess || p.ctas < 2) return r;
+  return launch_pdl(llm_append_combine_kernel<D>, dim3(p.ctas - 1, 2 * AP_ROWS * (D / 16) / 256),
+                    dim3(256), 0, s, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dllm_rotary(const DllmRotary* a, void* stream) {
+  if (!a) return DFM_ERR_INVALID_ARG;
+  if (a->dtype < DLLM_BF16 || a->dtype > DLLM_FP32) return DFM_ERR_UNSUPPORTED;
+  if (a->tokens < 0 || a->q_heads < 1 || a->head_dim < 2 || a->head_dim % 2 || a->rot_dim < 2 ||
+      a->rot_dim % 2 || a->rot_dim > a->head_dim)
+    return DFM_ERR_INVALID_ARG;
+  if (!a->turns || !a->positions || !a->q || !a->q_out) return DFM_ERR_INVALID_ARG;
+  if (a->k && (!a->v || !a->k_cache || !a->v_cache || !a->slot_mapping || !a->err_word ||
+               a->kv_heads < 1 || a->num_slots < 1))
+    return DFM_ERR_INVALID_ARG;
+  if (a->tokens == 0) return DFM_OK;
+  RotaryParams p{};
+  p.turns = reinterpret_cast<const unsigned long long*>(a->turns);
+  p.positions = a->positions;
+  p.q = a->q;
+  p.q_out = a->q_out;
+  p.q_ts = a->q_token_stride;
+  p.q_hs = a->q_head_stride;
+  p.o_ts = a->out_token_stride;
+  p.o_hs = a->out_head_stride;
+  if (a->q == a->q_out && (p.q_ts != p.o_ts || p.q_hs != p.o_hs)) return DFM_ERR_INVALID_ARG;
+  if (a->k) {
+    p.k = a->k;
+    p.v = a->v;
+    p.k_cache = a->k_cache;
+    p.v_cache = a->v_cache;
+    p.slots = a->slot_mapping;
+    p.k_ts = a->k_token_stride;
+    p.k_hs = a->k_head_stride;
+    p.v_ts = a->v_token_stride;
+    p.v_hs = a->v_head_stride;
+    p.kv_heads = a->kv_heads;
+    p.num_slots = a->num_slots;
+  }
+  p.err = a->err_word;
+  p.tokens = a->tokens;
+  p.heads = a->q_heads;
+  p.D = a->head_dim;
+  p.rot = a->rot_dim;
+  p.factor = a->factor;
+  p.copy_tail = a->q != a->q_out;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool in = a->interleaved != 0;
+  cudaError_t r = cudaErrorInvalidValue;
+  switch (a->dtype) {
+    case DLLM_BF16: r = in ? launch_rotary<__nv_bfloat16, true>(p, s) : launch_rotary<__nv_bfloat16, false>(p, s); break;
+    case DLLM_FP16: r = in ? launch_rotary<__half, true>(p, s) : launch_rotary<__half, false>(p, s); break;
+    case DLLM_FP32: r = in ? launch_rotary<float, true>(p, s) : launch_rotary<float, false>(p, s); break;
+  }
+  return r == cudaSuccess ? DFM_OK : DFM_ERR_CUDA;
+}
+
+size_t dllm_append_workspace_size(int32_t tokens, int32_t n, int32_t num_heads,
+                                  int32_t num_kv_heads, int32_t head_dim) {
+  if (!ap_shape_ok(tokens, n, num_heads, num_kv_heads, head_dim)) return 0;
+  return ap_ws(tokens, n, num_heads / num_kv_heads, head_dim, sm_count()).total;
+}
+
+int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  if (!a || !workspace) return DFM_ERR_INVALID_ARG;
+  if (a->dtype != DLLM_BF16 && a->dtype != DLLM_FP16) return DFM_ERR_UNSUPPORTED;
+  if (!ap_shape_ok(a->tokens, a->n, a->num_heads, a->num_kv_heads, a->head_dim))
+    return DFM_ERR_UNSUPPORTED;
+  if (!a->q || !a->k_cache || !a->v_cache || !a->cu_seqlens_q || !a->context_lens ||
+      !a->block_table || !a->out)
+    return DFM_ERR_INVALID_ARG;
+  if (a->num_blocks < 1 || a->max_blocks < 1) return DFM_ERR_INVALID_ARG;
+  if (a->block_size < 16 || a->block_size % 16) return DFM_ERR_UNSUPPORTED;
+  // positions are 32-bit, with room for a tile past the last one
+  if (static_cast<long long>(a->max_blocks) * a->block_size > 0x7fffff00ll) return DFM_ERR_UNSUPPORTED;
+  if (!(a->scale > 0.f) || !(a->softcap >= 0.f) || !(a->scale < INFINITY) || !(a->softcap < INFINITY) ||
+      a->window < 0)
+    return DFM_ERR_INVALID_ARG;
+  if (a->tree_masks && (a->prefix_lens || a->first_keys || a->slopes || a->window))
+    return DFM_ERR_UNSUPPORTED;
+  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out) ||
+      a->q_token_stride % 8 || a->q_head_stride % 8 || a->q_token_stride < 0 || a->q_head_stride < 0)
+    return DFM_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return DFM_ERR_INVALID_ARG;
+  const int G = a->num_heads / a->num_kv_heads, RT = AP_ROWS / G, ctas = sm_count();
+  const ApWs w = ap_ws(a->tokens, a->n, G, a->head_dim, ctas);
+  if (workspace_bytes < w.total) return DFM_ERR_WORKSPACE;
+  if (a->tokens == 0) return DFM_OK;
+  int rows = AP_KT;
+  while (a->block_size % rows) rows /= 2;
+  CUtensorMap mq, mk, mv;
+  if (!map_ap_q(&mq, *a, G, RT) || !map_ap_cache(&mk, *a, a->k_cache, rows) ||
+      !map_ap_cache(&mv, *a, a->v_cache, rows))
+    return DFM_ERR_CUDA;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  ApParams p{};
+  p.cu = a->cu_seqlens_q;
+  p.ctx = a->context_lens;
+  p.bt = a->block_table;
+  p.prefix = a->prefix_lens;
+  p.first = a->first_keys;
+  p.tree = reinterpret_cast<const unsigned long long*>(a->tree_masks);
+  p.slopes = a->slopes;
+  p.out = a->out;
+  p.err = reinterpret_cast<uint32_t*>(ws);
+  p.head = reinterpret_cast<ApHead*>(ws + w.head);
+  p.units = reinterpret_cast<ApUnit*>(ws + w.units);
+  p.ubase = reinterpret_cast<int*>(ws + w.ubase);
+  p.start = reinterpret_cast<int*>(ws + w.start);
+  p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  p.tokens = a->tokens;
+  p.n = a->n;
+  p.H = a->num_heads;
+  p.KVH = a->num_kv_heads;
+  p.G = G;
+  p.RT = RT;
+  p.max_units = ap_max_units(a->tokens, a->n, RT);
+  p.ctas = ctas;
+  p.num_blocks = a->num_blocks;
+  p.block_size = a->block_size;
+  p.max_blocks = a->max_blocks;
+  p.box_rows = rows;
+  p.causal = a->causal != 0;
+  p.window = a->window;
+  p.fp16 = a->dtype == DLLM_FP16;
+  const float log2e = 1.4426950408889634f;
+  p.scale_log2 = a->scale * log2e;
+  p.cap_in = a->softcap > 0.f ? 2.f * log2e * a->scale / a->softcap : 0.f;
+  p.cap_out = a->softcap * log2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t r = a->head_dim == 128 ? launch_append<128>(mq, mk, mv, p, s)
+                                           : launch_append<64>(mq, mk, mv, p, s);
+  return r == cudaSuccess ? DFM_OK : DFM_ERR_CUDA;
+}
+
+}  // extern "C"

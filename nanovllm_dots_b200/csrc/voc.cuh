@@ -50,14 +50,6 @@ DFM_DEV uint64_t umma_desc_sw64(uint32_t smem_addr) {
   return d;
 }
 
-DFM_DEV void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-
 // ---------------------------------------------------------------- conv
 constexpr int VC_BM = 128;
 constexpr int VC_BK = 32;    // channels (fp16) per 64-byte swizzle row

@@ -1,0 +1,187 @@
+"""Append attention of the LLM backbone on the B200 kernels
+(``dllm_append_attention``, ``include/dllm.h``).
+
+The reference prefills through flash-attn's variable-length call
+(``nanovllm_dots/layers/attention.py:66-86``): the new tokens of every sequence,
+packed, over the paged cache that already holds their K/V.
+``B200AppendAttention.append`` is that call with capped scores, a distance bias,
+sliding windows, bidirectional prefixes and packed documents; one new token a
+sequence is the decode step under the same options.  ``verify`` attends for
+trees of drafted tokens.  ``install_append_attention`` routes a reference
+``Attention`` module's prefill through it.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.bfloat16: _lib.DLLM_BF16, torch.float16: _lib.DLLM_FP16}
+TREE_MAX = 64     # drafted tokens of one sequence
+
+
+def tree_masks(parents) -> torch.Tensor:
+    """The masks ``verify`` takes, int64 [tokens], from each sequence's list of
+    parents: ``parents[i][t]`` is the drafted token that token t continues, or -1
+    for one that continues the history.  Bit u of a token's mask is set where
+    token u is the token itself or one of its ancestors."""
+    out = []
+    for i, row in enumerate(parents):
+        if len(row) > TREE_MAX:
+            raise ValueError(f"sequence {i}: {len(row)} drafted tokens (at most {TREE_MAX})")
+        bits = []
+        for t, up in enumerate(row):
+            if not -1 <= up < t:
+                raise ValueError(f"sequence {i}: parent {up} of token {t} does not come before it")
+            bits.append((bits[up] if up >= 0 else 0) | 1 << t)
+        out += [b - (1 << 64) if b >> 63 else b for b in bits]
+    return torch.tensor(out, dtype=torch.int64)
+
+
+class B200AppendAttention:
+    """Append attention of one model: heads, cache geometry and score options,
+    with a workspace for up to ``max_tokens`` new tokens of ``max_seqs``
+    sequences.
+
+    The workspace serves one call at a time.  Calls on one stream follow each
+    other; a call on another stream waits for the last one's stream.  A captured
+    graph keeps using the workspace: replay graphs of one object, and call it,
+    on one stream at a time, or give each an object of its own.
+    """
+
+    def __init__(self, num_heads: int, head_dim: int, scale: float, num_kv_heads: int, *,
+                 max_tokens: int, max_seqs: int, max_blocks: int, block_size: int = 256,
+                 dtype: torch.dtype = torch.bfloat16, causal: bool = True, window: int = 0,
+                 softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                 device: torch.device | str = "cuda"):
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError("B200AppendAttention runs on a CUDA device only (no CPU path)")
+        if dtype not in _DTYPES:
+            raise RuntimeError(f"unsupported append-attention type {dtype}")
+        if block_size < 16 or block_size % 16:
+            raise RuntimeError(f"block_size {block_size}: expected a multiple of 16")
+        if not scale > 0 or softcap < 0 or window < 0 or max_blocks < 1:
+            raise RuntimeError("expected a positive scale and max_blocks, no negative softcap or window")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
+        self.scale, self.softcap, self.window = float(scale), float(softcap), int(window)
+        self.causal, self.dtype = bool(causal), dtype
+        self.max_tokens, self.max_seqs = max_tokens, max_seqs
+        self.max_blocks, self.block_size = max_blocks, block_size
+        if slopes is not None:
+            if slopes.shape != (num_heads,):
+                raise RuntimeError(f"slopes: expected one for each of {num_heads} heads")
+            slopes = slopes.to(device=self.device, dtype=torch.float32).contiguous()
+        self.slopes = slopes
+        self.L = _lib.lib()
+        with torch.cuda.device(self.device):
+            self.ws_bytes = int(self.L.dllm_append_workspace_size(max_tokens, max_seqs, num_heads,
+                                                                  num_kv_heads, head_dim))
+        if self.ws_bytes == 0:
+            raise RuntimeError("unsupported append-attention shape")
+        self.workspace = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
+        self.workspace[:256].zero_()
+        self._last = torch.cuda.current_stream(self.device)   # of the zero-fill
+
+    def _int(self, name, t, dtype, shape):
+        if t.dtype != dtype or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+            raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on "
+                               f"{self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.data_ptr()
+
+    def _run(self, q, k_cache, v_cache, cu, ctx, table, prefix, first, tree, out, stream):
+        H, D, dev = self.num_heads, self.head_dim, self.device
+        if q.dim() != 3 or q.shape[1] != H or q.shape[2] != D or q.dtype != self.dtype or q.device != dev:
+            raise RuntimeError(f"q: expected a {self.dtype} tensor [tokens, {H}, {D}] on {dev}, "
+                               f"got {q.dtype} {tuple(q.shape)} on {q.device}")
+        T, n = q.shape[0], ctx.shape[0]
+        if T > self.max_tokens or not 1 <= n <= self.max_seqs:
+            raise RuntimeError(f"append of {T} tokens of {n} sequences "
+                               f"(at most {self.max_tokens} of {self.max_seqs})")
+        st, sh, sd = q.stride()
+        if sd != 1 or st % 8 or sh % 8 or q.data_ptr() % 16:
+            raise RuntimeError("q: expected contiguous head dims and 16-byte aligned heads")
+        geometry = (self.block_size, self.num_kv_heads, D)
+        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if c.dtype != self.dtype or c.device != dev or c.shape[1:] != geometry or \
+                    c.shape[0] != k_cache.shape[0] or c.shape[0] < 1 or not c.is_contiguous():
+                raise RuntimeError(f"{name}: expected a contiguous {self.dtype} tensor [num_blocks, "
+                                   f"{', '.join(map(str, geometry))}] on {dev}")
+        if table.dim() != 2 or not 1 <= table.shape[1] <= self.max_blocks:
+            raise RuntimeError(f"block_tables: expected [{n}, 1..{self.max_blocks}]")
+        s = stream if stream is not None else torch.cuda.current_stream(dev)
+        if out is None:
+            if stream is None:
+                out = torch.empty((T, H, D), dtype=self.dtype, device=dev)
+            else:     # owned by the stream that writes it
+                with torch.cuda.stream(s):
+                    out = torch.empty((T, H, D), dtype=self.dtype, device=dev)
+        elif out.dtype != self.dtype or out.device != dev or tuple(out.shape) != (T, H, D) or \
+                not out.is_contiguous():
+            raise RuntimeError(f"out: expected a contiguous {self.dtype} tensor {(T, H, D)} on {dev}")
+        i32 = torch.int32
+        a = _lib.DllmAppend(
+            _DTYPES[self.dtype], T, n, H, self.num_kv_heads, D, k_cache.shape[0], self.block_size,
+            table.shape[1], self.causal, self.window if tree is None else 0, self.scale, self.softcap,
+            q.data_ptr(), st, sh, k_cache.data_ptr(), v_cache.data_ptr(),
+            self._int("cu_seqlens_q", cu, i32, (n + 1,)), self._int("context_lens", ctx, i32, (n,)),
+            self._int("block_tables", table, i32, (n, table.shape[1])),
+            None if prefix is None else self._int("prefix_lens", prefix, i32, (n,)),
+            None if first is None else self._int("first_keys", first, i32, (T,)),
+            None if tree is None else self._int("tree_masks", tree, torch.int64, (T,)),
+            None if tree is not None or self.slopes is None else self.slopes.data_ptr(),
+            out.data_ptr())
+        if T == 0:
+            return out
+        if s != self._last and not torch.cuda.is_current_stream_capturing():
+            s.wait_stream(self._last)      # the workspace may still be in use there
+            self._last = s
+        if torch.cuda.current_device() == dev.index:
+            rc = self.L.dllm_append_attention(a, self.workspace.data_ptr(), self.ws_bytes,
+                                              ctypes.c_void_p(s.cuda_stream))
+        else:
+            with torch.cuda.device(dev):
+                rc = self.L.dllm_append_attention(a, self.workspace.data_ptr(), self.ws_bytes,
+                                                  ctypes.c_void_p(s.cuda_stream))
+        _lib.check(rc, "dllm_append_attention")
+        return out
+
+    def append(self, q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, *,
+               prefix_lens: torch.Tensor | None = None, first_keys: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """q [tokens, H, D]: the newest tokens of n sequences, packed; int32
+        cu_seqlens_q [n + 1] where each sequence's begin; int32 context_lens [n]
+        cached positions, the new tokens included; int32 block_tables [n, width].
+        prefix_lens [n]: leading positions every token of the sequence sees,
+        whatever its own; first_keys [tokens]: the first position a token sees
+        (its document's).  -> [tokens, H, D]; zeros where a token sees nothing,
+        rows past cu_seqlens_q[n] as they were."""
+        return self._run(q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, prefix_lens,
+                         first_keys, None, out, stream)
+
+    def verify(self, q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables,
+               tree_masks: torch.Tensor, *, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """``append`` for trees of drafted tokens, at most 64 a sequence, whose
+        K/V stand in the cache in the order of q.  A token sees the history
+        before them and the drafted tokens whose bits are set in its int64 mask
+        (``tree_masks(parents)``).  ``causal`` plays no part."""
+        if self.slopes is not None or self.window:
+            raise RuntimeError("verify: not supported with slopes or a window")
+        return self._run(q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, None, None,
+                         tree_masks, out, stream)
+
+    def check_errors(self) -> None:
+        """Synchronise and raise if a kernel reported a device-side error."""
+        v = _lib.c_uint32(0)
+        s = torch.cuda.current_stream(self.device)
+        s.wait_stream(self._last)
+        with torch.cuda.device(self.device):
+            _lib.check(self.L.dllm_read_error(_lib.ptr(self.workspace), _lib.c_void_p(s.cuda_stream), v),
+                       "dllm_read_error")
+        if v.value:
+            names = [nm for bit, nm in _lib.DEVERR_BITS.items() if v.value & bit]
+            raise RuntimeError(f"append attention device error: {', '.join(names)} (0x{v.value:x})")

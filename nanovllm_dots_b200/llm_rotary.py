@@ -1,0 +1,249 @@
+"""Rotary positions of the LLM backbone on the B200 kernels (``dllm_rotary``,
+``include/dllm.h``).
+
+The reference rotates whole heads in the half layout at unscaled frequencies
+(``nanovllm_dots/layers/rotary_embedding.py:6-47``) and stores k and v with a
+kernel of its own (``layers/attention.py:10-47``).  ``B200Rotary`` does both in
+one launch, in either pair layout, over part of a head, at frequencies scaled
+for contexts longer than the trained one.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.bfloat16: _lib.DLLM_BF16, torch.float16: _lib.DLLM_FP16,
+           torch.float32: _lib.DLLM_FP32}
+KINDS = ("linear", "ntk", "bands", "yarn")
+LAYOUTS = ("half", "interleaved")
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How the frequencies w_i = theta^(-2i / rot_dim) change for a context
+    ``factor`` times the ``original_max`` positions of training:
+
+    * ``linear``: w_i / factor;
+    * ``ntk``: theta becomes theta * factor^(rot_dim / (rot_dim - 2));
+    * ``bands``: waves that turn at least ``high_freq`` times in the original
+      context keep w_i, those below ``low_freq`` turns get w_i / factor, and the
+      turns between blend the two linearly;
+    * ``yarn`` (Peng et al., 2023): the blend runs over the pair index between
+      the pairs that turn ``beta_fast`` and ``beta_slow`` times, and cos and sin
+      are multiplied by 0.1 ln(factor) + 1 (``attention_factor`` overrides).
+    """
+    kind: str
+    factor: float
+    original_max: int = 0
+    low_freq: float = 1.0
+    high_freq: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float | None = None
+
+
+def rotary_frequencies(rot_dim: int, theta: float, scaling: RotaryScaling | None = None
+                       ) -> tuple[torch.Tensor, float]:
+    """(radians a position of each pair, in float64 [rot_dim / 2]; factor on cos and sin)."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim}: expected an even number of dims")
+    if not theta > 1.0 or not math.isfinite(theta):
+        raise ValueError(f"theta {theta}: expected a finite base above 1")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    inv = theta ** (-i / rot_dim)
+    if scaling is None:
+        return inv, 1.0
+    s = scaling
+    if s.kind not in KINDS:
+        raise ValueError(f"rotary scaling {s.kind!r}: expected one of {KINDS}")
+    if not s.factor >= 1.0 or not math.isfinite(s.factor):
+        raise ValueError(f"rotary scaling factor {s.factor}: expected at least 1")
+    if s.kind in ("bands", "yarn") and s.original_max < 1:
+        raise ValueError(f"rotary scaling {s.kind!r} needs original_max")
+    factor = 1.0 if s.attention_factor is None else float(s.attention_factor)
+    if s.kind == "linear":
+        return inv / s.factor, factor
+    if s.kind == "ntk":
+        if rot_dim == 2:
+            raise ValueError("rotary scaling 'ntk' needs rot_dim above 2")
+        return (theta * s.factor ** (rot_dim / (rot_dim - 2))) ** (-i / rot_dim), factor
+    if s.kind == "bands":
+        if not s.high_freq > s.low_freq:
+            raise ValueError("rotary scaling 'bands': expected high_freq above low_freq")
+        turns = s.original_max * inv / (2 * math.pi)
+        keep = ((turns - s.low_freq) / (s.high_freq - s.low_freq)).clamp(0, 1)
+    else:
+        if not s.beta_fast > s.beta_slow > 0:
+            raise ValueError("rotary scaling 'yarn': expected beta_fast above beta_slow above 0")
+
+        def pair(turns):    # the (fractional) pair that turns so often in the original context
+            return rot_dim * math.log(s.original_max / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        low = max(math.floor(pair(s.beta_fast)), 0)
+        high = min(math.ceil(pair(s.beta_slow)), rot_dim - 1)
+        keep = 1 - ((i / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
+        if s.attention_factor is None:
+            factor = 0.1 * math.log(s.factor) + 1.0
+    return inv / s.factor * (1 - keep) + inv * keep, factor
+
+
+def _turns(inv: torch.Tensor) -> torch.Tensor:
+    """Frequencies as turns a position, a binary fraction of 2^64 in int64."""
+    out = []
+    for w in inv.tolist():
+        bits = int(math.ldexp(math.fmod(w / (2 * math.pi), 1.0), 64)) & ((1 << 64) - 1)
+        out.append(bits - (1 << 64) if bits >> 63 else bits)
+    return torch.tensor(out, dtype=torch.int64)
+
+
+class B200Rotary:
+    """Rotary of one model: head size, layout and frequencies.  Rotated values
+    are computed in fp32 and rounded once; the angle is exact to 2^-31 turns at
+    every int32 position."""
+
+    def __init__(self, head_dim: int, *, theta: float = 10000.0, rot_dim: int | None = None,
+                 layout: str = "half", scaling: RotaryScaling | None = None,
+                 device: torch.device | str = "cuda"):
+        if layout not in LAYOUTS:
+            raise ValueError(f"rotary layout {layout!r}: expected one of {LAYOUTS}")
+        rot_dim = head_dim if rot_dim is None else rot_dim
+        if head_dim < 2 or head_dim % 2 or rot_dim > head_dim:
+            raise ValueError(f"head_dim {head_dim}, rot_dim {rot_dim}: expected even sizes, "
+                             "rot_dim at most head_dim")
+        inv, factor = rotary_frequencies(rot_dim, theta, scaling)
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError("B200Rotary runs on a CUDA device only (no CPU path)")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.head_dim, self.rot_dim, self.layout, self.factor = head_dim, rot_dim, layout, factor
+        self.L = _lib.lib()
+        self.turns = _turns(inv).to(self.device)
+        self.err = torch.zeros(64, dtype=torch.int32, device=self.device)
+
+    def _check(self, name, t, dtype, shape):
+        if t.dtype != dtype or t.device != self.device or tuple(t.shape) != shape:
+            raise RuntimeError(f"{name}: expected a {dtype} tensor of shape {shape} on {self.device}, "
+                               f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+    def _heads(self, name, t, dtype=None, tokens=None):
+        if t.dim() != 3 or t.shape[2] != self.head_dim or t.device != self.device:
+            raise RuntimeError(f"{name}: expected [tokens, heads, {self.head_dim}] on {self.device}, "
+                               f"got {tuple(t.shape)} on {t.device}")
+        if t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
+            raise RuntimeError(f"{name}: unsupported or mixed type {t.dtype}")
+        if tokens is not None and t.shape[0] != tokens:
+            raise RuntimeError(f"{name}: expected {tokens} tokens, got {t.shape[0]}")
+        if t.stride(2) != 1:
+            raise RuntimeError(f"{name}: expected contiguous head dims")
+
+    def _args(self, q, positions, out):
+        self._heads("q", q)
+        if positions.dtype != torch.int32 or positions.device != self.device or \
+                positions.shape != (q.shape[0],) or not positions.is_contiguous():
+            raise RuntimeError(f"positions: expected a contiguous int32 [{q.shape[0]}] on {self.device}")
+        self._heads("out", out, q.dtype, q.shape[0])
+        if out.shape != q.shape:
+            raise RuntimeError(f"out: expected shape {tuple(q.shape)}")
+        qs, os = q.stride(), out.stride()
+        same = out.data_ptr() == q.data_ptr()
+        if same and qs[:2] != os[:2]:
+            raise RuntimeError("out: rotating in place needs q's own strides")
+        if not same and _overlap(q, out):
+            raise RuntimeError("out: overlaps q without being q")
+        if q.shape[0] > 1 and os[0] == 0 or q.shape[1] > 1 and os[1] == 0:
+            raise RuntimeError("out: rows share memory")
+        a = _lib.DllmRotary(dtype=_DTYPES[q.dtype], tokens=q.shape[0], q_heads=q.shape[1],
+                            head_dim=self.head_dim, rot_dim=self.rot_dim,
+                            interleaved=self.layout == "interleaved", factor=self.factor,
+                            turns=self.turns.data_ptr(), positions=positions.data_ptr(),
+                            q=q.data_ptr(), q_out=out.data_ptr(), q_token_stride=qs[0],
+                            q_head_stride=qs[1], out_token_stride=os[0], out_head_stride=os[1],
+                            err_word=self.err.data_ptr())
+        return a
+
+    def _launch(self, a, stream):
+        s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(self.L.dllm_rotary(a, ctypes.c_void_p(s.cuda_stream)), "dllm_rotary")
+
+    def _out(self, q, out, stream):
+        if out is not None:
+            return out
+        # owned by the stream that writes it
+        with torch.cuda.stream(stream):
+            return torch.empty(q.shape, dtype=q.dtype, device=self.device)
+
+    def rotate(self, q, positions, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """q [tokens, heads, head_dim] (any token and head strides) at int32
+        positions [tokens] -> out (``out=q`` rotates in place)."""
+        out = self._out(q, out, stream)
+        if q.numel() == 0:
+            return out
+        self._launch(self._args(q, positions, out), stream)
+        return out
+
+    def rotate_store(self, q, k, v, positions, slot_mapping, k_cache, v_cache,
+                     out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """Rotates q as ``rotate`` does and writes rotated k and unrotated v
+        [tokens, kv_heads, head_dim] into the paged caches [num_blocks,
+        block_size, kv_heads, head_dim] at int32 slot_mapping [tokens] (block *
+        block_size + offset; -1 stores nothing).  Two tokens must not share a
+        slot.  A slot past the cache is not stored and reported by
+        ``check_errors``."""
+        T = q.shape[0]
+        self._heads("k", k, q.dtype, T)
+        self._heads("v", v, q.dtype, T)
+        kvh = k.shape[1]
+        if v.shape[1] != kvh or kvh < 1:
+            raise RuntimeError("k and v have different heads")
+        if slot_mapping.dtype != torch.int32 or slot_mapping.device != self.device or \
+                slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
+            raise RuntimeError(f"slot_mapping: expected a contiguous int32 [{T}] on {self.device}")
+        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if c.dtype != q.dtype or c.device != self.device or c.dim() != 4 or not c.is_contiguous() \
+                    or c.shape[2:] != (kvh, self.head_dim) or c.shape != k_cache.shape or not c.numel():
+                raise RuntimeError(f"{name}: expected a contiguous {q.dtype} [num_blocks, block_size, "
+                                   f"{kvh}, {self.head_dim}] on {self.device}")
+        out = self._out(q, out, stream)
+        if T == 0:
+            return out
+        if q.shape[1] < 1:
+            raise RuntimeError("q has no heads")
+        a = self._args(q, positions, out)
+        a.kv_heads = kvh
+        a.k, a.v = k.data_ptr(), v.data_ptr()
+        a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+        a.slot_mapping = slot_mapping.data_ptr()
+        (a.k_token_stride, a.k_head_stride), (a.v_token_stride, a.v_head_stride) = \
+            k.stride()[:2], v.stride()[:2]
+        a.num_slots = k_cache.shape[0] * k_cache.shape[1]
+        self._launch(a, stream)
+        return out
+
+    def check_errors(self) -> None:
+        """Synchronise and raise if a slot past the cache was met."""
+        v = _lib.c_uint32(0)
+        s = torch.cuda.current_stream(self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(self.L.dllm_read_error(_lib.ptr(self.err), _lib.c_void_p(s.cuda_stream), v),
+                       "dllm_read_error")
+        if v.value:
+            names = [nm for bit, nm in _lib.DEVERR_BITS.items() if v.value & bit]
+            raise RuntimeError(f"rotary device error: {', '.join(names)} (0x{v.value:x})")
+
+
+def _span(t):
+    """First and last byte of a tensor's elements."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a, b) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1

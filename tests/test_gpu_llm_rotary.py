@@ -1,0 +1,140 @@
+"""Rotary positions with the cache store (``dllm_rotary`` through ``B200Rotary``)
+against a float64 oracle; the bound of every element is derived in
+``llm_append_oracle.rotate`` (fp32 products and sums, one rounding)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from nanovllm_dots_b200.llm_rotary import B200Rotary, RotaryScaling, rotary_frequencies
+from oracle import llm_append_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def positions(T, seed=0):
+    """Positions over the whole int32 range, the ends among them."""
+    g = torch.Generator().manual_seed(seed)
+    p = (2.0 ** (torch.rand(T, generator=g, dtype=torch.float64) * 31)).long() - 1
+    p[0] = 0
+    if T > 2:
+        p[1], p[2] = 2 ** 31 - 1, 1
+    return p.to(torch.int32)
+
+
+def data(T, H, D, dtype, seed=0):
+    return torch.randn(T, H, D, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def close(got, ref, tol):
+    over = (got.double().cpu() - ref).abs() - tol
+    assert over.max() <= 0, f"{int((over > 0).sum())} of {over.numel()} are off, by up to {over.max():.3g}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("T,H,D,rot", [(1, 1, 128, 128), (5, 12, 128, 64), (64, 3, 64, 64), (7, 2, 64, 16),
+                                       (3, 2, 80, 20), (2, 1, 6, 2), (9000, 12, 128, 128), (4001, 16, 64, 32)])
+def test_rotate(T, H, D, rot, layout, dtype):
+    x, pos = data(T, H, D, dtype), positions(T)
+    inv, f = rotary_frequencies(rot, 10000.0)
+    ref, tol = O.rotate(x, pos, inv, f, rot, layout)
+    r = B200Rotary(D, rot_dim=rot, layout=layout, device=DEV)
+    xd, pd = x.to(DEV), pos.to(DEV)
+    got = r.rotate(xd, pd)
+    close(got, ref, tol)
+    assert torch.equal(xd.cpu(), x)
+    assert torch.equal(got[..., rot:].cpu(), x[..., rot:])
+    assert r.rotate(xd, pd, out=xd) is xd and torch.equal(xd, got)     # in place
+
+
+@pytest.mark.parametrize("scaling", [RotaryScaling("linear", 4.0), RotaryScaling("ntk", 8.0),
+                                     RotaryScaling("bands", 8.0, 8192), RotaryScaling("yarn", 16.0, 4096),
+                                     RotaryScaling("yarn", 2.0, 32768, attention_factor=0.5)])
+def test_scaled_frequencies(scaling):
+    x, pos = data(300, 4, 128, torch.float32), torch.arange(100000, 100300, dtype=torch.int32)
+    inv, f = rotary_frequencies(128, 1e6, scaling)
+    ref, tol = O.rotate(x, pos, inv, f, 128, "half")
+    got = B200Rotary(128, theta=1e6, scaling=scaling, device=DEV).rotate(x.to(DEV), pos.to(DEV))
+    close(got, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,KVH,D,rot,bs", [(1, 12, 2, 128, 128, 256), (64, 12, 2, 128, 128, 256),
+                                              (333, 8, 8, 64, 32, 16), (5000, 12, 2, 128, 64, 256),
+                                              (17, 3, 1, 20, 10, 48)])
+def test_rotate_and_store(T, H, KVH, D, rot, bs, dtype):
+    """q, k, v as slices of the packed projection; -1 slots store nothing; other slots stay."""
+    packed = data(T, H + 2 * KVH, D, dtype)
+    pos, blocks = positions(T, 1), -(-T // bs) + 2
+    slots = torch.randperm(blocks * bs, generator=torch.Generator().manual_seed(2))[:T].to(torch.int32)
+    slots[T // 2] = -1 if T > 1 else slots[0]
+    K0, V0 = data(blocks * bs, KVH, D, dtype, 5), data(blocks * bs, KVH, D, dtype, 6)
+    inv, f = rotary_frequencies(rot, 5e4)
+    r = B200Rotary(D, theta=5e4, rot_dim=rot, device=DEV)
+    p = packed.to(DEV)
+    K, V = (c.view(blocks, bs, KVH, D).to(DEV) for c in (K0, V0))
+    q = r.rotate_store(p[:, :H], p[:, H:H + KVH], p[:, H + KVH:], pos.to(DEV), slots.to(DEV), K, V)
+    r.check_errors()
+    close(q, *O.rotate(packed[:, :H], pos, inv, f, rot, "half"))
+    kr, kt = O.rotate(packed[:, H:H + KVH], pos, inv, f, rot, "half")
+    live = slots >= 0
+    at = slots[live].long()
+    close(K.view(-1, KVH, D)[at.to(DEV)], kr[live], kt[live])
+    assert torch.equal(V.view(-1, KVH, D).cpu()[at], packed[live, H + KVH:])
+    rest = torch.ones(blocks * bs, dtype=torch.bool)
+    rest[at] = False
+    assert torch.equal(K.view(-1, KVH, D).cpu()[rest], K0[rest])
+    assert torch.equal(V.view(-1, KVH, D).cpu()[rest], V0[rest])
+
+
+def test_odd_strides_and_alignment():
+    """Rows that are not 16-byte aligned take the element-wise kernel: same values."""
+    T, H, D = 50, 3, 64
+    x, pos = data(T, H, D, torch.bfloat16), positions(T)
+    r = B200Rotary(D, device=DEV)
+    want = r.rotate(x.to(DEV), pos.to(DEV))
+    base = torch.zeros(T, H, D + 3, dtype=torch.bfloat16, device=DEV)
+    base[..., 1:D + 1] = x.to(DEV)
+    odd = base[..., 1:D + 1]
+    assert torch.equal(r.rotate(odd, pos.to(DEV)), want)
+    flipped = x.to(DEV).transpose(0, 1).contiguous().transpose(0, 1)
+    out = torch.empty(H, T, D, dtype=torch.bfloat16, device=DEV).transpose(0, 1)
+    assert torch.equal(r.rotate(flipped, pos.to(DEV), out=out), want)
+    shared = x[:, :1].to(DEV).expand(T, H, D)        # one head read for all
+    assert torch.equal(r.rotate(shared, pos.to(DEV)), want[:, :1].expand(T, H, D))
+
+
+def test_slot_past_the_cache_is_reported():
+    r = B200Rotary(128, device=DEV)
+    qkv = data(4, 4, 128, torch.bfloat16).to(DEV)
+    K = torch.zeros(2, 16, 1, 128, dtype=torch.bfloat16, device=DEV)
+    V = torch.zeros_like(K)
+    pos = torch.arange(4, dtype=torch.int32, device=DEV)
+    slots = torch.tensor([0, 32, 5, 31], dtype=torch.int32, device=DEV)
+    r.rotate_store(qkv[:, :2], qkv[:, 2:3], qkv[:, 3:], pos, slots, K, V)
+    with pytest.raises(RuntimeError, match="page"):
+        r.check_errors()
+    r.check_errors()
+    assert int((V.view(32, -1) != 0).any(1).sum()) == 3
+
+
+def test_no_tokens_graph_and_stream():
+    r = B200Rotary(64, device=DEV)
+    x, pos = data(40, 2, 64, torch.float16).to(DEV), positions(40).to(DEV)
+    assert r.rotate(x[:0], pos[:0]).shape == (0, 2, 64)
+    want = r.rotate(x, pos)
+    out = torch.empty_like(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        r.rotate(x, pos, out=out)
+    out.zero_()
+    g.replay()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    other = r.rotate(x, pos, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(other, want)
