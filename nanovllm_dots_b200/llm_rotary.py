@@ -96,7 +96,7 @@ def _turns(inv: torch.Tensor) -> torch.Tensor:
     """Frequencies as turns a position, a binary fraction of 2^64 in int64."""
     out = []
     for w in inv.tolist():
-        bits = int(math.ldexp(math.fmod(w / (2 * math.pi), 1.0), 64)) & ((1 << 64) - 1)
+        bits = round(math.ldexp(math.fmod(w / (2 * math.pi), 1.0), 64)) & ((1 << 64) - 1)
         out.append(bits - (1 << 64) if bits >> 63 else bits)
     return torch.tensor(out, dtype=torch.int64)
 

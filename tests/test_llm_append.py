@@ -151,7 +151,8 @@ def test_turns_keep_the_angle_at_far_positions():
         for pos in (1, 12345, 2 ** 31 - 1):
             got = (pos * (t & (1 << 64) - 1)) % (1 << 64) / 2.0 ** 64 * 2 * math.pi
             gap = abs(math.remainder(got - math.fmod(pos * w, 2 * math.pi), 2 * math.pi))
-            assert gap <= pos * w * 2.0 ** -51 + 1e-12
+            # the fraction of 2^64 is rounded: half a unit a position, in radians
+            assert gap <= pos * (w * 2.0 ** -51 + math.pi * 2.0 ** -64) + 1e-12
 
 
 def test_tree_masks():
