@@ -52,6 +52,10 @@ constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's
 // much (log2 units): probabilities then reach 2^8, exact in fp32 and within
 // fp16's range, and O is seldom rescaled.
 constexpr float AP_TAU = 8.0f;
+// Registers of a thread after the split between the softmax warpgroups and the
+// third one: 88 + 2 * 208 = 3 * 168, what the block is launched with.
+constexpr int AP_REGS_FEW = 88, AP_REGS_MANY = 208, AP_REGS_LAUNCH = 168;
+static_assert(AP_REGS_FEW + 2 * AP_REGS_MANY <= 3 * AP_REGS_LAUNCH, "register split");
 
 struct ApUnit {
   int seq, t0, ntok, row0;          // tokens [t0, t0 + ntok) of the sequence; row0: its first in q
@@ -86,9 +90,11 @@ struct ApParams {
   float2* part_ml;                  // [ctas][2][2][128]
   int tokens, n, H, KVH, G, RT, max_units, ctas;
   int num_blocks, block_size, max_blocks, box_rows;
-  int causal, window, fp16;
-  float scale_log2;                 // scale * log2(e)
-  float cap_in, cap_out;            // 2 log2(e) scale / cap and cap log2(e); cap_out 0: no cap
+  int causal, window;
+  float scale_log2;                 // what makes log2 units of x (scale * log2(e) without a cap)
+  // With a cap: x = tanh(S cap_a), cap_a = scale / cap, cap_in = 2 log2(e) cap_a,
+  // scale_log2 = cap log2(e).  cap_a 0: none, x = S.
+  float cap_a, cap_in;
 };
 
 // ---------------------------------------------------------------- plan
@@ -125,6 +131,7 @@ DFM_DEV T block_exclusive_scan(T v, T* warp_sums, T& total) {   // AP_PLAN_THREA
 __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApParams p) {
   __shared__ int sums[32];
   __shared__ long long lsums[32];
+  __shared__ int near[AP_PLAN_THREADS];   // ubase of the first sequences
   pdl_trigger();
   pdl_wait();
   const int t = threadIdx.x;
@@ -151,7 +158,8 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
     }
     int total;
     const int at = block_exclusive_scan(c, sums, total);
-    if (i < p.n) p.ubase[i] = carry + at;
+    if (i < AP_PLAN_THREADS) near[i] = carry + at;
+    else if (i < p.n) p.ubase[i] = carry + at;
     carry += total;
   }
   int units = carry;
@@ -159,58 +167,81 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
     if (t == 0) atomicOr(p.err, DFM_DEV_ERR_LEN);
     units = p.max_units;
   }
-  __syncthreads();   // ubase, written by this block, is read below
+  __syncthreads();   // near and ubase, written by this block, are read below
+  auto ubase = [&](int i) { return i < AP_PLAN_THREADS ? near[i] : p.ubase[i]; };
+  auto seq_of = [&](int u) {   // the last sequence with ubase <= u (one without units shares the next one's)
+    int a = 0, b = p.n - 1;
+    while (a < b) {
+      const int mid = (a + b + 1) >> 1;
+      if (ubase(mid) <= u) a = mid; else b = mid - 1;
+    }
+    return a;
+  };
+  // [lo, hi) of a token
+  auto keys = [&](int seq, int s0, int j, int base, int ctx, int& lo, int& hi) {
+    const int pos = base + j;
+    hi = p.causal ? max(pos + 1, p.prefix ? min(p.prefix[seq], ctx) : 0) : ctx;
+    lo = p.window ? max(0, pos + 1 - p.window) : 0;
+    if (p.first) lo = max(lo, p.first[s0 + j]);
+  };
+  if (p.first) {   // every token has bounds of its own: a warp to a unit
+    for (int u = t >> 5; u < units; u += AP_PLAN_THREADS / 32) {
+      const int a = seq_of(u);
+      int s0, m;
+      rows_ok(a, s0, m);
+      const int ctx = p.ctx[a], t0 = (u - ubase(a)) * 2 * p.RT, end = min(m, t0 + 2 * p.RT);
+      int lo = 0x7fffffff, hi = 0, fmin = 0, fmax = 0x7fffffff;
+      for (int j = t0 + (t & 31); j < end; j += 32) {
+        int l, h;
+        keys(a, s0, j, ctx - m, ctx, l, h);
+        if (l < h) {
+          lo = min(lo, l);
+          hi = max(hi, h);
+        }
+        fmin = max(fmin, l);
+        fmax = min(fmax, h);
+      }
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      fmin = __reduce_max_sync(0xffffffffu, fmin);
+      fmax = __reduce_min_sync(0xffffffffu, fmax);
+      if ((t & 31) == 0) *reinterpret_cast<int4*>(&p.units[u].lo) = make_int4(lo, hi, fmin, fmax);
+    }
+    __syncthreads();
+  }
   long long line = 0;
   for (int u0 = 0; u0 < units; u0 += AP_PLAN_THREADS) {
     const int u = u0 + t;
     ApUnit f{};
     if (u < units) {
-      int a = 0, b = p.n - 1;    // the last sequence with ubase <= u (those without units share a value)
-      while (a < b) {
-        const int mid = (a + b + 1) >> 1;
-        if (p.ubase[mid] <= u) a = mid; else b = mid - 1;
-      }
+      const int a = seq_of(u);
       int s0, m;
       rows_ok(a, s0, m);
       const int ctx = p.ctx[a];
       f.seq = a;
-      f.t0 = (u - p.ubase[a]) * 2 * p.RT;
+      f.t0 = (u - ubase(a)) * 2 * p.RT;
       f.ntok = min(2 * p.RT, m - f.t0);
       f.row0 = s0;
       f.base = ctx - m;
       f.narrow = f.ntok <= p.RT;
-      f.lo = f.hi = 0;
-      f.fmin = 0x7fffffff;
-      f.fmax = 0;
-      if (ctx >= m && ctx <= static_cast<long long>(p.max_blocks) * p.block_size && !(p.tree && m > 64)) {
-        if (p.tree) {
-          f.hi = ctx;
-          f.fmin = 0;
-          f.fmax = f.base;
-        } else {
-          const int pre = p.prefix ? min(p.prefix[a], ctx) : 0;
-          int lo = 0x7fffffff, hi = 0, fmin = 0, fmax = 0x7fffffff;
-          // without per-token bounds the ends of the interval rise with the token
-          const int step = p.first ? 1 : max(1, f.ntok - 1);
-          for (int j = f.t0; j < f.t0 + f.ntok; j += step) {
-            const int pos = f.base + j;
-            const int h = p.causal ? max(pos + 1, pre) : ctx;
-            int l = p.window ? max(0, pos + 1 - p.window) : 0;
-            if (p.first) l = max(l, p.first[s0 + j]);
-            if (l < h) {
-              lo = min(lo, l);
-              hi = max(hi, h);
-            }
-            fmin = max(fmin, l);
-            fmax = min(fmax, h);
-          }
-          if (hi > 0) {
-            f.lo = lo;
-            f.hi = hi;
-            f.fmin = fmin;
-            f.fmax = fmax;
-          }
-        }
+      const bool good = ctx >= m && ctx <= static_cast<long long>(p.max_blocks) * p.block_size &&
+                        !(p.tree && m > 64);
+      if (good && p.tree) {
+        f.hi = ctx;
+        f.fmax = f.base;
+      } else if (good && p.first) {
+        const int4 b = *reinterpret_cast<const int4*>(&p.units[u].lo);
+        f.lo = b.x;
+        f.hi = b.y;
+        f.fmin = b.z;
+        f.fmax = b.w;
+      } else if (good) {   // the ends of the interval rise with the token
+        keys(a, s0, f.t0, f.base, ctx, f.lo, f.fmax);
+        keys(a, s0, f.t0 + f.ntok - 1, f.base, ctx, f.fmin, f.hi);
+      }
+      if (f.hi <= f.lo) {
+        f.lo = f.hi = f.fmax = 0;
+        f.fmin = 0x7fffffff;
       }
       const int tiles = f.hi > f.lo ? (f.hi + AP_KT - 1) / AP_KT - f.lo / AP_KT : 0;
       f.cost = max(1, tiles * (f.narrow ? 1 : 2));
@@ -320,11 +351,29 @@ DFM_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint
       : "memory");
 }
 
+// Bounded waits on the SM's clock, which is read in a few cycles (globaltimer is
+// not): about a second at the highest clock.
+constexpr long long AP_WAIT_CLOCKS = 2000000000ll;
+
+DFM_DEV bool ap_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (clock64() - t0 > AP_WAIT_CLOCKS) {
+      *abort_flag = 1;
+      atomicOr(err, DFM_DEV_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
 // Wait with the time limit alone, whatever the abort flag says (the way out of
 // an aborted CTA, whose copies and products are still in flight).
 DFM_DEV void mbar_drain(uint64_t* bar, uint32_t parity) {
-  const uint64_t t0 = globaltimer();
-  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 <= DFM_WAIT_LIMIT_NS) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity) && clock64() - t0 <= AP_WAIT_CLOCKS) {
   }
 }
 
@@ -342,25 +391,86 @@ DFM_DEV bool ap_pair_sync(bool ok) {
   return r != 0;
 }
 
-DFM_DEV uint32_t ap_pack(float a, float b, bool fp16) {
-  if (fp16) {
+template <bool kFp16>
+DFM_DEV uint32_t ap_pack(float a, float b) {
+  if constexpr (kFp16) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16(a, b);
   }
-  return pack_bf16(a, b);
+}
+
+// Two fp32 operations in one instruction.
+DFM_DEV uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+DFM_DEV void f2_split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+DFM_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+DFM_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+DFM_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // The lowest n bits, n clamped to [0, 32].
 DFM_DEV uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// Whether a 32-bit word of two 16-bit floats holds an infinity or a NaN.
-DFM_DEV bool ap_special(uint32_t w, uint32_t exp_lo) {
-  return (w & exp_lo) == exp_lo || (w & (exp_lo << 16)) == (exp_lo << 16);
+constexpr float AP_T0 = 0.999999972f, AP_T1 = -0.333329668f, AP_T2 = 0.133255161f, AP_T3 = -0.0533498438f, AP_T4 = 0.0195938116f, AP_T5 = -0.0047239585f;
+
+// tanh(S a) for 128 scores of a row.  Where every score of the warp's tile is
+// below 0.75 caps, tanh y = y q(y^2) with q the polynomial of degree 5 fitted at
+// Chebyshev nodes of [0, 0.75^2] (3e-8 relative): 3.5 instructions a score on the
+// fp32 pipe.  Else 1 - 2 / (1 + e^{2y}): two special-function operations, of
+// which an SM does 16 a clock, so that they and the softmax's exponential would
+// take three times the products' time.
+DFM_DEV void ap_tanh(float (&x)[4][32], float a, float cap_in) {
+  float big = 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 32; ++e) big = fmaxf(big, fabsf(x[c][e]));
+  // (a NaN is not above the bound and stays one in the polynomial)
+  if (__any_sync(0xffffffffu, big * a > 0.75f)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        x[c][e] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(x[c][e] * cap_in)), 1.f);
+    return;
+  }
+  const uint64_t aa = f2(a, a);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const uint64_t y = f2_mul(f2(x[c][e], x[c][e + 1]), aa), z = f2_mul(y, y);
+      uint64_t q = f2(AP_T5, AP_T5);
+      q = f2_fma(q, z, f2(AP_T4, AP_T4));
+      q = f2_fma(q, z, f2(AP_T3, AP_T3));
+      q = f2_fma(q, z, f2(AP_T2, AP_T2));
+      q = f2_fma(q, z, f2(AP_T1, AP_T1));
+      q = f2_fma(q, z, f2(AP_T0, AP_T0));
+      f2_split(f2_mul(y, q), x[c][e], x[c][e + 1]);
+    }
 }
 
 // ---------------------------------------------------------------- the kernel
 // kMod: a cap or a distance bias on the scores.
-template <int D, bool kMod>
+template <int D, bool kMod, bool kFp16>
 __global__ void __launch_bounds__(AP_THREADS, 1)
     llm_append_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const ApParams p) {
@@ -378,15 +488,15 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   uint64_t* v_ready = v_full + AP_RING;   // V without special values: arrivals of its two warps
   uint64_t* v_empty = v_ready + AP_RING;
   uint64_t* s_full = v_empty + AP_RING;   // [2] per stream
-  uint64_t* p_full = s_full + 2;          // [2] arrivals of the stream's four warps
-  uint64_t* o_full = p_full + 2;          // [2]
+  uint64_t* p_full = s_full + 2;          // [2][2] its two halves of P: arrivals of its four warps
+  uint64_t* o_full = p_full + 4;          // [2]
   uint64_t* q_full = o_full + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* drain = q_empty + 1;
   uint32_t* poison = reinterpret_cast<uint32_t*>(drain + 1);   // [AP_RING][4]
   uint32_t* tmem_slot = poison + AP_RING * 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((5 * AP_RING + 9) * 8 + AP_RING * 16 + 8 <= 512, "barrier area");
+  static_assert((5 * AP_RING + 11) * 8 + AP_RING * 16 + 8 <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -399,7 +509,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(q_full, 1);
@@ -421,9 +532,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
   pdl_wait();
+
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AP_REGS_FEW));
   ApWalk walk(p);
   ApSegment sg;
-
   if (warp == 8) {
     // ------------------------------------------------------------ TMA
     const int per_tile = AP_KT / p.box_rows;         // boxes along the keys
@@ -433,7 +546,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     while (ok && walk.next(p, sg)) {
       if (sg.i1 == sg.i0) continue;
       if (lane == 0) {
-        ok = nseg == 0 || mbar_wait(q_empty, (nseg - 1) & 1, abort_flag, p.err);
+        ok = nseg == 0 || ap_wait(q_empty, (nseg - 1) & 1, abort_flag, p.err);
         if (ok) {
           const int nt = sg.f.narrow ? 1 : 2;
           mbar_arrive_expect_tx(q_full, nt * S::BOXES * p.G * p.RT * 128);
@@ -468,14 +581,14 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         const int row = key % p.block_size;
         const int dst = slot * S::TILE + half * S::HALF + box * box_bytes;
         if (lane == 0) {
-          ok = g < AP_RING || mbar_wait(&k_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
+          ok = g < AP_RING || ap_wait(&k_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
           if (ok) mbar_arrive_expect_tx(&k_full[slot], bytes);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         if (mine) tma_load_4d(sK + dst, &tm_k, &k_full[slot], half * 64, sg.kv, row, cb);
         if (lane == 0) {
-          ok = g < AP_RING || mbar_wait(&v_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
+          ok = g < AP_RING || ap_wait(&v_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
           if (ok) mbar_arrive_expect_tx(&v_full[slot], bytes);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -497,7 +610,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA
     if (lane == 0) {
-      const uint32_t fmt = p.fp16 ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t fmt = kFp16 ? 0u : (1u << 7) | (1u << 10);
       const uint32_t base = (1u << 4) | fmt | (static_cast<uint32_t>(AP_ROWS >> 4) << 24);
       const uint32_t idesc_s = base | (static_cast<uint32_t>(AP_KT >> 3) << 17);
       const uint32_t idesc_o = base | (static_cast<uint32_t>(D >> 3) << 17) | (1u << 16);
@@ -515,26 +628,29 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         umma_commit(&s_full[s]);
       };
       auto k_wait = [&](int at) {
-        ok = ok && mbar_wait(&k_full[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err);
+        ok = ok && ap_wait(&k_full[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err);
         tc_fence_after();
       };
-      // O_s += P_s V
+      // O_s += P_s V, half a key tile at a time
       auto values = [&](int s, int at, bool first) {
-        ok = ok && mbar_wait(&p_full[s], np[s] & 1, abort_flag, p.err) &&
-             mbar_wait(&v_ready[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err);
-        ++np[s];
-        if (!ok) return;
-        tc_fence_after();
         const uint32_t v = smem_u32(sV + (at % AP_RING) * S::TILE);
+        for (int h = 0; ok && h < 2; ++h) {
+          ok = ap_wait(&p_full[2 * s + h], np[s] & 1, abort_flag, p.err) &&
+               (h > 0 || ap_wait(&v_ready[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err));
+          if (!ok) return;
+          tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < AP_KT / 16; ++kk)
-          umma_f16_ts(tmem + 256 + s * D, tmem + s * AP_KT + kk * 8,
-                      umma_desc_sw128_mn(v + kk * 2048, S::HALF), idesc_o, !first || kk > 0);
+          for (int kk = 0; kk < AP_KT / 32; ++kk)
+            umma_f16_ts(tmem + 256 + s * D, tmem + s * AP_KT + h * 32 + kk * 8,
+                        umma_desc_sw128_mn(v + h * (AP_KT / 2) * 128 + kk * 2048, S::HALF), idesc_o,
+                        !first || h > 0 || kk > 0);
+        }
+        ++np[s];
       };
       while (ok && walk.next(p, sg)) {
         const int nt = sg.i1 - sg.i0;
         if (nt == 0) continue;
-        ok = mbar_wait(q_full, nseg & 1, abort_flag, p.err);
+        ok = ap_wait(q_full, nseg & 1, abort_flag, p.err);
         ++nseg;
         if (sg.f.narrow) {
           for (int i = 0; i < 2 && i < nt; ++i) {
@@ -591,33 +707,37 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         mbar_drain(drain, 0);
       }
     }
-  } else if (warp >= 10) {
+  } else {
     // ------------------------------------------------------------ special rows of V
     const int w = warp - 10;
-    const uint32_t exp_lo = p.fp16 ? 0x7c00u : 0x7f80u;
+    const uint32_t inf2 = kFp16 ? 0x7c007c00u : 0x7f807f80u;
     int g = 0;
     bool ok = true;
     while (ok && walk.next(p, sg)) {
       for (int i = sg.i0; i < sg.i1; ++i, ++g) {
         const int slot = g % AP_RING;
-        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[slot], (g / AP_RING) & 1, abort_flag, p.err));
+        ok = __all_sync(0xffffffffu, ap_wait(&v_full[slot], (g / AP_RING) & 1, abort_flag, p.err));
         if (!ok) break;
         const int k0 = (sg.top - i) * AP_KT;
         if (k0 < sg.f.fmin || k0 + AP_KT > sg.f.fmax) {
+          // where all rows see the same keys, a special value is all rows' own
+          const bool split = max(k0, sg.f.lo) < sg.f.fmin || min(k0 + AP_KT, sg.f.hi) > sg.f.fmax;
           for (int x = 0; x < 2; ++x) {
             const int r = w * 64 + x * 32 + lane, key = k0 + r;
             uint8_t* row = sV + slot * S::TILE + r * 128;
             const bool seen = key >= sg.f.lo && key < sg.f.hi;
             bool special = false;
-            if (seen) {
+            if (seen && split) {
+              uint32_t top = 0;    // per half word, the largest magnitude's bits
 #pragma unroll
               for (int b = 0; b < S::BOXES; ++b)
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                   const uint4 u = *reinterpret_cast<const uint4*>(row + b * S::HALF + ((c ^ (r & 7)) << 4));
-                  special |= ap_special(u.x, exp_lo) | ap_special(u.y, exp_lo) |
-                             ap_special(u.z, exp_lo) | ap_special(u.w, exp_lo);
+                  top = __vimax3_u16x2(top, u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
+                  top = __vimax3_u16x2(top, u.z & 0x7fff7fffu, u.w & 0x7fff7fffu);
                 }
+              special = (top & 0xffffu) >= (inf2 & 0xffffu) || (top >> 16) >= (inf2 >> 16);
             }
             if (!seen || special) {
 #pragma unroll
@@ -635,8 +755,12 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (lane == 0) mbar_arrive(&v_ready[slot]);
       }
     }
+  }
   } else {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AP_REGS_MANY));
+    ApWalk walk(p);
+    ApSegment sg;
     const int s = warp >> 2;                           // stream
     const int r = (warp & 3) * 32 + lane;              // row of the tile, TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -668,51 +792,67 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           lo = p.window ? max(0, pos + 1 - p.window) : 0;
           if (p.first) lo = max(lo, p.first[sg.f.row0 + j]);
         }
-        if (kMod && p.slopes) slope = p.slopes[sg.kv * p.G + head_of] * 1.4426950408889634f;
+        // in units of x
+        if (kMod && p.slopes) slope = p.slopes[sg.kv * p.G + head_of] * (1.4426950408889634f / p.scale_log2);
       }
       float m = -INFINITY, l = 0.f;
       const int step = narrow ? 2 : 1, i_first = narrow ? s : 0;
 #pragma unroll 1
       for (int i = i_first; ok && i < nt; i += step, ++ns) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], ns & 1, abort_flag, p.err));
+        ok = __all_sync(0xffffffffu, ap_wait(&s_full[s], ns & 1, abort_flag, p.err));
         if (!ok) break;
         tc_fence_after();
         const int k0 = (sg.top - sg.i0 - i) * AP_KT;
         const bool full = k0 >= sg.f.fmin && k0 + AP_KT <= sg.f.fmax;
         if (!full) {
           const int slot = (g + i) % AP_RING;
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
+          ok = __all_sync(0xffffffffu, ap_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
           if (!ok) break;
         }
         if (warp_valid) {
+          // x scale + shift is the score in log2 units
           float x[4][32];
+          float top = -INFINITY;
+          auto tops = [&](const float (&v)[32]) {
+            float t0 = v[0], t1 = v[1];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c]));
+            for (int e = 2; e < 32; e += 2) {
+              t0 = fmaxf(t0, v[e]);
+              t1 = fmaxf(t1, v[e + 1]);
+            }
+            top = fmaxf(top, fmaxf(t0, t1));
+          };
+          float shift = 0.f;
+          tmem_ld32(tS, reinterpret_cast<uint32_t(&)[32]>(x[0]));
           tmem_wait_ld();
-          float scale = p.scale_log2;
+#pragma unroll
+          for (int c = 1; c < 4; ++c) {
+            tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c]));
+            if (!kMod && full) tops(x[c - 1]);
+            tmem_wait_ld();
+          }
           if constexpr (kMod) {
-            if (p.cap_out > 0.f) {
-              // cap tanh(y): tanh y = 1 - 2 / (1 + e^{2y})
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  x[c][e] = p.cap_out * (1.f - __fdividef(2.f, 1.f + fast_exp2(x[c][e] * p.cap_in)));
-            } else {
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int e = 0; e < 32; ++e) x[c][e] *= p.scale_log2;
-            }
+            if (p.cap_a > 0.f) ap_tanh(x, p.cap_a, p.cap_in);
             if (p.slopes) {
-              const float d0 = static_cast<float>(pos - k0);
+              if (k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix)) {
+                // every key the row may see is at or before it: |p - k| = (p - k0) - c
+                shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
+                const uint64_t sl = f2(slope, slope);
 #pragma unroll
-              for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  x[c][e] = fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), x[c][e]);
+                  for (int e = 0; e < 32; e += 2)
+                    f2_split(f2_fma(sl, f2(c * 32 + e, c * 32 + e + 1), f2(x[c][e], x[c][e + 1])), x[c][e],
+                             x[c][e + 1]);
+              } else {
+                const float d0 = static_cast<float>(pos - k0);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                  for (int e = 0; e < 32; ++e)
+                    x[c][e] = fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), x[c][e]);
+              }
             }
-            scale = 1.f;
           }
           if (!full) {
             uint32_t bad = 0;
@@ -728,14 +868,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
             if (bad) l = __int_as_float(0x7fffffff);
           }
-          float top[4];
+          if (kMod || !full) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            top[c] = x[c][0];
-#pragma unroll
-            for (int e = 1; e < 32; ++e) top[c] = fmaxf(top[c], x[c][e]);
+            for (int c = 0; c < 4; ++c) tops(x[c]);
+          } else {
+            tops(x[3]);
           }
-          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+          const float mt = fmaf(top, p.scale_log2, shift);
           if (i == i_first) {
             m = mt;
           } else if (__any_sync(0xffffffffu, mt > m + AP_TAU)) {
@@ -754,26 +893,36 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               tmem_st32(tO + s * D + c, o);
             }
           }
-          const float ms = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float ms = shift - (m == -INFINITY ? 0.f : m);
+          const uint64_t sc = f2(p.scale_log2, p.scale_log2), sh = f2(ms, ms);
+          uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-          for (int c = 0; c < 4; c += 2) {
+          for (int h = 0; h < 2; ++h) {
             uint32_t pk[32];
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
-              const float a = fast_exp2(fmaf(x[c + (e >> 5)][e & 31], scale, -ms));
-              const float b = fast_exp2(fmaf(x[c + (e >> 5)][(e & 31) + 1], scale, -ms));
-              sum[(e >> 1) & 3] += a + b;
-              pk[e >> 1] = ap_pack(a, b, p.fp16);
+              float& xa = x[2 * h + (e >> 5)][e & 31];
+              float& xb = x[2 * h + (e >> 5)][(e & 31) + 1];
+              float a, b;
+              f2_split(f2_fma(f2(xa, xb), sc, sh), a, b);
+              a = fast_exp2(a);
+              b = fast_exp2(b);
+              sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], f2(a, b));
+              pk[e >> 1] = ap_pack<kFp16>(a, b);
             }
-            tmem_st32(tS + c * 16, pk);
+            tmem_st32(tS + h * 32, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_wait_st();
+          float a, b;
+          f2_split(f2_add(sum[0], sum[1]), a, b);
+          l += a + b;
+        } else if (lane == 0) {   // nobody reads this warp's rows
+          mbar_arrive(&p_full[2 * s]);
+          mbar_arrive(&p_full[2 * s + 1]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[s]);
       }
       // ------------------------------------------------ the segment's rows
       const int n0 = narrow ? (nt + 1) / 2 : nt, n1 = narrow ? nt / 2 : nt;
@@ -790,9 +939,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         m = mm;
       }
       if (ok && n0 > 0 && (narrow || s == 0))
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[0], no[0] & 1, abort_flag, p.err));
+        ok = __all_sync(0xffffffffu, ap_wait(&o_full[0], no[0] & 1, abort_flag, p.err));
       if (ok && n1 > 0 && (narrow || s == 1))
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[1], no[1] & 1, abort_flag, p.err));
+        ok = __all_sync(0xffffffffu, ap_wait(&o_full[1], no[1] & 1, abort_flag, p.err));
       no[0] += n0 > 0;
       no[1] += n1 > 0;
       g += nt;
@@ -837,10 +986,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(ap_pack(v[8 * e] * inv, v[8 * e + 1] * inv, p.fp16),
-                             ap_pack(v[8 * e + 2] * inv, v[8 * e + 3] * inv, p.fp16),
-                             ap_pack(v[8 * e + 4] * inv, v[8 * e + 5] * inv, p.fp16),
-                             ap_pack(v[8 * e + 6] * inv, v[8 * e + 7] * inv, p.fp16));
+                  make_uint4(ap_pack<kFp16>(v[8 * e] * inv, v[8 * e + 1] * inv),
+                             ap_pack<kFp16>(v[8 * e + 2] * inv, v[8 * e + 3] * inv),
+                             ap_pack<kFp16>(v[8 * e + 4] * inv, v[8 * e + 5] * inv),
+                             ap_pack<kFp16>(v[8 * e + 6] * inv, v[8 * e + 7] * inv));
             __syncwarp();
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
@@ -870,7 +1019,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 // Block (b, y): the unit that the end of share b cuts, if it began in share b,
 // rows and columns [y * 256, (y + 1) * 256) of its (tile, 16-dim group, row)
 // list.  out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the shares.
-template <int D>
+template <int D, bool kFp16>
 __global__ void __launch_bounds__(256) llm_append_combine_kernel(const ApParams p) {
   constexpr int CB = 4;
   pdl_trigger();
@@ -934,7 +1083,7 @@ __global__ void __launch_bounds__(256) llm_append_combine_kernel(const ApParams 
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint32_t pk[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) pk[e] = ap_pack(acc[2 * e] * inv, acc[2 * e + 1] * inv, p.fp16);
+  for (int e = 0; e < 8; ++e) pk[e] = ap_pack<kFp16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   uint4* dst = reinterpret_cast<uint4*>(
       static_cast<uint16_t*>(p.out) +
       (static_cast<size_t>(f.row0 + j) * p.H + kv * p.G + r % p.G) * D + dg * 16);

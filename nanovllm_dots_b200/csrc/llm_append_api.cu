@@ -99,22 +99,37 @@ bool map_ap_q(CUtensorMap* m, const DllmAppend& a, int G, int RT) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, bool kMod, bool kFp16>
 cudaError_t launch_append(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                           const ApParams& p, cudaStream_t s) {
-  static std::atomic<uint64_t> done_plain{0}, done_mod{0};
+  static std::atomic<uint64_t> done{0};
+  static std::atomic<int> regs{0};
   constexpr int smem = ApSmem<D>::BYTES;
-  const bool mod = p.cap_out > 0.f || p.slopes;
-  cudaError_t r = mod ? smem_attr_once(done_mod, llm_append_kernel<D, true>, smem)
-                      : smem_attr_once(done_plain, llm_append_kernel<D, false>, smem);
+  auto fn = llm_append_kernel<D, kMod, kFp16>;
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes at;
+    const cudaError_t r = cudaFuncGetAttributes(&at, fn);
+    if (r != cudaSuccess) return r;
+    regs.store(at.numRegs, std::memory_order_relaxed);
+  }
+  // with fewer registers at launch the softmax warps would wait for theirs for ever
+  if (regs.load(std::memory_order_relaxed) < AP_REGS_LAUNCH) return cudaErrorInvalidConfiguration;
+  cudaError_t r = smem_attr_once(done, fn, smem);
   if (r != cudaSuccess) return r;
   r = launch_pdl(llm_append_plan_kernel, dim3(1), dim3(AP_PLAN_THREADS), 0, s, p);
   if (r != cudaSuccess) return r;
-  r = launch_pdl(mod ? llm_append_kernel<D, true> : llm_append_kernel<D, false>, dim3(p.ctas),
-                 dim3(AP_THREADS), smem, s, q, k, v, p);
+  r = launch_pdl(fn, dim3(p.ctas), dim3(AP_THREADS), smem, s, q, k, v, p);
   if (r != cudaSuccess || p.ctas < 2) return r;
-  return launch_pdl(llm_append_combine_kernel<D>, dim3(p.ctas - 1, 2 * AP_ROWS * (D / 16) / 256),
+  return launch_pdl(llm_append_combine_kernel<D, kFp16>, dim3(p.ctas - 1, 2 * AP_ROWS * (D / 16) / 256),
                     dim3(256), 0, s, p);
+}
+
+template <int D>
+cudaError_t launch_append(bool mod, bool fp16, const CUtensorMap& q, const CUtensorMap& k,
+                          const CUtensorMap& v, const ApParams& p, cudaStream_t s) {
+  if (mod)
+    return fp16 ? launch_append<D, true, true>(q, k, v, p, s) : launch_append<D, true, false>(q, k, v, p, s);
+  return fp16 ? launch_append<D, false, true>(q, k, v, p, s) : launch_append<D, false, false>(q, k, v, p, s);
 }
 
 }  // namespace
@@ -242,14 +257,14 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.box_rows = rows;
   p.causal = a->causal != 0;
   p.window = a->window;
-  p.fp16 = a->dtype == DLLM_FP16;
   const float log2e = 1.4426950408889634f;
-  p.scale_log2 = a->scale * log2e;
-  p.cap_in = a->softcap > 0.f ? 2.f * log2e * a->scale / a->softcap : 0.f;
-  p.cap_out = a->softcap * log2e;
+  p.cap_a = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
+  p.cap_in = 2.f * log2e * p.cap_a;
+  p.scale_log2 = (a->softcap > 0.f ? a->softcap : a->scale) * log2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t r = a->head_dim == 128 ? launch_append<128>(mq, mk, mv, p, s)
-                                           : launch_append<64>(mq, mk, mv, p, s);
+  const bool mod = a->softcap > 0.f || a->slopes, fp16 = a->dtype == DLLM_FP16;
+  const cudaError_t r = a->head_dim == 128 ? launch_append<128>(mod, fp16, mq, mk, mv, p, s)
+                                           : launch_append<64>(mod, fp16, mq, mk, mv, p, s);
   return r == cudaSuccess ? DFM_OK : DFM_ERR_CUDA;
 }
 
