@@ -52,10 +52,8 @@ constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's
 // much (log2 units): probabilities then reach 2^8, exact in fp32 and within
 // fp16's range, and O is seldom rescaled.
 constexpr float AP_TAU = 8.0f;
-// Registers of a thread after the split between the softmax warpgroups and the
-// third one: 88 + 2 * 208 = 3 * 168, what the block is launched with.
-constexpr int AP_REGS_FEW = 88, AP_REGS_MANY = 208, AP_REGS_LAUNCH = 168;
-static_assert(AP_REGS_FEW + 2 * AP_REGS_MANY <= 3 * AP_REGS_LAUNCH, "register split");
+// Of AP_EXP_OF pairs of exponentials, AP_EXP_POLY go to the fp32 pipe.
+constexpr int AP_EXP_POLY = 1, AP_EXP_OF = 4;
 
 struct ApUnit {
   int seq, t0, ntok, row0;          // tokens [t0, t0 + ntok) of the sequence; row0: its first in q
@@ -338,6 +336,16 @@ struct ApSmem {
 };
 static_assert(ApSmem<128>::BYTES <= 232448, "one CTA per SM");
 
+DFM_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // D(tmem) (+)= A(tmem) * B(smem, MN-major), 16-bit inputs, fp32 accumulate.
 DFM_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                          uint32_t accumulate) {
@@ -401,6 +409,22 @@ DFM_DEV uint32_t ap_pack(float a, float b) {
   }
 }
 
+// 32 TMEM columns of this thread's lane, asynchronously: x is there after
+// ap_landed, whose operands keep the compiler from using it earlier.
+DFM_DEV void ap_load(uint32_t taddr, float (&x)[32]) {
+  tmem_ld32(taddr, reinterpret_cast<uint32_t(&)[32]>(x));
+}
+DFM_DEV void ap_landed(float (&x)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]),
+                 "+f"(x[7]), "+f"(x[8]), "+f"(x[9]), "+f"(x[10]), "+f"(x[11]), "+f"(x[12]), "+f"(x[13]),
+                 "+f"(x[14]), "+f"(x[15]), "+f"(x[16]), "+f"(x[17]), "+f"(x[18]), "+f"(x[19]), "+f"(x[20]),
+                 "+f"(x[21]), "+f"(x[22]), "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]),
+                 "+f"(x[28]), "+f"(x[29]), "+f"(x[30]), "+f"(x[31])
+               :
+               : "memory");
+}
+
 // Two fp32 operations in one instruction.
 DFM_DEV uint64_t f2(float a, float b) {
   uint64_t r;
@@ -431,41 +455,71 @@ DFM_DEV uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n
 
 constexpr float AP_T0 = 0.999999972f, AP_T1 = -0.333329668f, AP_T2 = 0.133255161f, AP_T3 = -0.0533498438f, AP_T4 = 0.0195938116f, AP_T5 = -0.0047239585f;
 
-// tanh(S a) for 128 scores of a row.  Where every score of the warp's tile is
+// 2^x of two scores on the fp32 pipe: x = n + f with n the nearest integer, 2^f by
+// the polynomial of degree 5 fitted at Chebyshev nodes of [-1/2, 1/2] (1e-7
+// relative), times 2^n, which for n = -127 comes out as an exact 0 (masked scores are
+// -inf); a NaN stays one.
+constexpr float AP_E0 = 1.00000008f, AP_E1 = 0.693147207f, AP_E2 = 0.240221073f, AP_E3 = 0.055503272f, AP_E4 = 0.00967604193f, AP_E5 = 0.00134004369f;
+DFM_DEV void ap_exp2_pair(uint64_t x, float& a, float& b) {
+  constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer
+  f2_split(x, a, b);
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(-127.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(b), "f"(-127.f));
+  const uint64_t y = f2(a, b), t = f2_add(y, f2(kRound, kRound));
+  const uint64_t f = f2_add(y, f2_fma(t, f2(-1.f, -1.f), f2(kRound, kRound)));
+  uint64_t q = f2(AP_E5, AP_E5);
+  q = f2_fma(q, f, f2(AP_E4, AP_E4));
+  q = f2_fma(q, f, f2(AP_E3, AP_E3));
+  q = f2_fma(q, f, f2(AP_E2, AP_E2));
+  q = f2_fma(q, f, f2(AP_E1, AP_E1));
+  q = f2_fma(q, f, f2(AP_E0, AP_E0));
+  float ta, tb;
+  f2_split(t, ta, tb);
+  // kRound's low bits are zero: t's hold n, and (n << 23) + the bits of 1 is 2^n
+  q = f2_mul(q, f2(__uint_as_float((__float_as_uint(ta) << 23) + 0x3f800000u),
+                   __uint_as_float((__float_as_uint(tb) << 23) + 0x3f800000u)));
+  f2_split(q, a, b);
+}
+
+// tanh(S a) for 32 scores of a row.  Where every score of the warp's chunk is
 // below 0.75 caps, tanh y = y q(y^2) with q the polynomial of degree 5 fitted at
 // Chebyshev nodes of [0, 0.75^2] (3e-8 relative): 3.5 instructions a score on the
 // fp32 pipe.  Else 1 - 2 / (1 + e^{2y}): two special-function operations, of
 // which an SM does 16 a clock, so that they and the softmax's exponential would
 // take three times the products' time.
-DFM_DEV void ap_tanh(float (&x)[4][32], float a, float cap_in) {
+DFM_DEV void ap_tanh(float (&x)[32], float a, float cap_in) {
   float big = 0.f;
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int e = 0; e < 32; ++e) big = fmaxf(big, fabsf(x[c][e]));
+  for (int e = 0; e < 32; ++e) big = fmaxf(big, fabsf(x[e]));
   // (a NaN is not above the bound and stays one in the polynomial)
   if (__any_sync(0xffffffffu, big * a > 0.75f)) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-        x[c][e] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(x[c][e] * cap_in)), 1.f);
+    for (int e = 0; e < 32; ++e)
+      x[e] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(x[e] * cap_in)), 1.f);
     return;
   }
   const uint64_t aa = f2(a, a);
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int e = 0; e < 32; e += 2) {
+    const uint64_t y = f2_mul(f2(x[e], x[e + 1]), aa), z = f2_mul(y, y);
+    uint64_t q = f2(AP_T5, AP_T5);
+    q = f2_fma(q, z, f2(AP_T4, AP_T4));
+    q = f2_fma(q, z, f2(AP_T3, AP_T3));
+    q = f2_fma(q, z, f2(AP_T2, AP_T2));
+    q = f2_fma(q, z, f2(AP_T1, AP_T1));
+    q = f2_fma(q, z, f2(AP_T0, AP_T0));
+    f2_split(f2_mul(y, q), x[e], x[e + 1]);
+  }
+}
+
+DFM_DEV float ap_max32(const float (&x)[32], float top) {
+  float t0 = top, t1 = x[0];
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      const uint64_t y = f2_mul(f2(x[c][e], x[c][e + 1]), aa), z = f2_mul(y, y);
-      uint64_t q = f2(AP_T5, AP_T5);
-      q = f2_fma(q, z, f2(AP_T4, AP_T4));
-      q = f2_fma(q, z, f2(AP_T3, AP_T3));
-      q = f2_fma(q, z, f2(AP_T2, AP_T2));
-      q = f2_fma(q, z, f2(AP_T1, AP_T1));
-      q = f2_fma(q, z, f2(AP_T0, AP_T0));
-      f2_split(f2_mul(y, q), x[c][e], x[c][e + 1]);
-    }
+  for (int e = 1; e < 31; e += 2) {
+    t0 = fmaxf(t0, x[e]);
+    t1 = fmaxf(t1, x[e + 1]);
+  }
+  return fmaxf(fmaxf(t0, t1), x[31]);
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -534,7 +588,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   pdl_wait();
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AP_REGS_FEW));
   ApWalk walk(p);
   ApSegment sg;
   if (warp == 8) {
@@ -564,21 +617,22 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       auto block_of = [&](int i) {   // the lane's cache block in tile i, -2 if nobody sees the box
         const int key = (sg.top - i) * AP_KT + box * p.box_rows;
         if (box >= per_tile || i >= sg.i1 || key + p.box_rows <= sg.f.lo || key >= sg.f.hi) return -2;
-        return bt[key / p.block_size];
+        const int b = bt[key / p.block_size];
+        return b < 0 ? -1 : b;
       };
       int blk = block_of(sg.i0);
       for (int i = sg.i0; ok && i < sg.i1; ++i, ++g) {
         const int slot = g % AP_RING;
         const int key = (sg.top - i) * AP_KT + box * p.box_rows;
+        const int row = key % p.block_size;
         const bool mine = blk != -2;
         int cb = blk;
         if (mine && (cb < 0 || cb >= p.num_blocks)) {
           if (half == 0) atomicOr(p.err, DFM_DEV_ERR_PAGE);
           cb = p.num_blocks;   // out of range: zeros
         }
-        const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box_bytes;
         blk = block_of(i + 1);
-        const int row = key % p.block_size;
+        const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box_bytes;
         const int dst = slot * S::TILE + half * S::HALF + box * box_bytes;
         if (lane == 0) {
           ok = g < AP_RING || ap_wait(&k_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
@@ -609,69 +663,86 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA
-    if (lane == 0) {
+    // The whole warp walks and waits, so that descriptors are built in uniform
+    // registers; one elected lane issues.
+    {
       const uint32_t fmt = kFp16 ? 0u : (1u << 7) | (1u << 10);
       const uint32_t base = (1u << 4) | fmt | (static_cast<uint32_t>(AP_ROWS >> 4) << 24);
       const uint32_t idesc_s = base | (static_cast<uint32_t>(AP_KT >> 3) << 17);
       const uint32_t idesc_o = base | (static_cast<uint32_t>(D >> 3) << 17) | (1u << 16);
+      const bool leader = elect_one();
+      const uint64_t dq = umma_desc_sw128(smem_u32(sQ)), dk = umma_desc_sw128(smem_u32(sK)),
+                     dv = umma_desc_sw128_mn(smem_u32(sV), S::HALF);
       int g = 0, nseg = 0;
       int np[2] = {0, 0};        // probability tiles taken per stream
       bool ok = true;
+      auto commit = [&](uint64_t* bar) {
+        if (leader) umma_commit(bar);
+      };
       // S_s = Q_x K^T for the K tile of ring position `at`
       auto scores = [&](int s, int x, int at) {
-        const uint32_t q = smem_u32(sQ + x * S::TILE), k = smem_u32(sK + (at % AP_RING) * S::TILE);
+        const uint64_t q = dq + x * (S::TILE >> 4), k = dk + (at % AP_RING) * (S::TILE >> 4);
+        const uint32_t d = tmem + s * AP_KT;
+        if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const int o = (kk >> 2) * S::HALF + (kk & 3) * 32;
-          umma_bf16(tmem + s * AP_KT, umma_desc_sw128(q + o), umma_desc_sw128(k + o), idesc_s, kk > 0);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            constexpr int H16 = S::HALF >> 4;
+            umma_bf16(d, q + (kk >> 2) * H16 + (kk & 3) * 2, k + (kk >> 2) * H16 + (kk & 3) * 2, idesc_s,
+                      kk > 0);
+          }
+          umma_commit(&s_full[s]);
         }
-        umma_commit(&s_full[s]);
       };
       auto k_wait = [&](int at) {
         ok = ok && ap_wait(&k_full[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err);
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       };
       // O_s += P_s V, half a key tile at a time
       auto values = [&](int s, int at, bool first) {
-        const uint32_t v = smem_u32(sV + (at % AP_RING) * S::TILE);
-        for (int h = 0; ok && h < 2; ++h) {
-          ok = ap_wait(&p_full[2 * s + h], np[s] & 1, abort_flag, p.err) &&
+        const uint64_t v = dv + (at % AP_RING) * (S::TILE >> 4);
+        const uint32_t d = tmem + 256 + s * D, a = tmem + s * AP_KT;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && ap_wait(&p_full[2 * s + h], np[s] & 1, abort_flag, p.err) &&
                (h > 0 || ap_wait(&v_ready[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err));
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           tc_fence_after();
+          if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < AP_KT / 32; ++kk)
-            umma_f16_ts(tmem + 256 + s * D, tmem + s * AP_KT + h * 32 + kk * 8,
-                        umma_desc_sw128_mn(v + h * (AP_KT / 2) * 128 + kk * 2048, S::HALF), idesc_o,
-                        !first || h > 0 || kk > 0);
+            for (int kk = 0; kk < AP_KT / 32; ++kk)
+              umma_f16_ts(d, a + h * 32 + kk * 8, v + (h * (AP_KT / 2) * 128 + kk * 2048) / 16, idesc_o,
+                          !first || h > 0 || kk > 0);
+          }
         }
         ++np[s];
       };
       while (ok && walk.next(p, sg)) {
         const int nt = sg.i1 - sg.i0;
         if (nt == 0) continue;
-        ok = ap_wait(q_full, nseg & 1, abort_flag, p.err);
+        ok = __all_sync(0xffffffffu, ap_wait(q_full, nseg & 1, abort_flag, p.err));
         ++nseg;
         if (sg.f.narrow) {
           for (int i = 0; i < 2 && i < nt; ++i) {
             k_wait(g + i);
             if (!ok) break;
             scores(i, 0, g + i);
-            umma_commit(&k_empty[(g + i) % AP_RING]);
-            if (i == nt - 1) umma_commit(q_empty);
+            commit(&k_empty[(g + i) % AP_RING]);
+            if (i == nt - 1) commit(q_empty);
           }
           for (int i = 0; ok && i < nt; ++i) {
             const int s = i & 1;
             values(s, g + i, i < 2);
             if (!ok) break;
-            umma_commit(&v_empty[(g + i) % AP_RING]);
-            if (i + 2 >= nt) umma_commit(&o_full[s]);
+            commit(&v_empty[(g + i) % AP_RING]);
+            if (i + 2 >= nt) commit(&o_full[s]);
             if (i + 2 < nt) {
               k_wait(g + i + 2);
               if (!ok) break;
               scores(s, 0, g + i + 2);
-              umma_commit(&k_empty[(g + i + 2) % AP_RING]);
-              if (i + 2 == nt - 1) umma_commit(q_empty);
+              commit(&k_empty[(g + i + 2) % AP_RING]);
+              if (i + 2 == nt - 1) commit(q_empty);
             }
           }
         } else {
@@ -679,23 +750,23 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if (!ok) break;
           scores(0, 0, g);
           scores(1, 1, g);
-          umma_commit(&k_empty[g % AP_RING]);
-          if (nt == 1) umma_commit(q_empty);
+          commit(&k_empty[g % AP_RING]);
+          if (nt == 1) commit(q_empty);
           for (int i = 0; ok && i < nt; ++i) {
             for (int s = 0; s < 2; ++s) {
               values(s, g + i, i == 0);
               if (!ok) break;
-              if (s == 1) umma_commit(&v_empty[(g + i) % AP_RING]);
+              if (s == 1) commit(&v_empty[(g + i) % AP_RING]);
               if (i == nt - 1) {
-                umma_commit(&o_full[s]);
+                commit(&o_full[s]);
                 continue;
               }
               if (s == 0) k_wait(g + i + 1);
               if (!ok) break;
               scores(s, s, g + i + 1);
               if (s == 1) {
-                umma_commit(&k_empty[(g + i + 1) % AP_RING]);
-                if (i + 1 == nt - 1) umma_commit(q_empty);
+                commit(&k_empty[(g + i + 1) % AP_RING]);
+                if (i + 1 == nt - 1) commit(q_empty);
               }
             }
           }
@@ -703,8 +774,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         g += nt;
       }
       if (!ok) {   // products in flight read shared memory and TMEM
-        umma_commit(drain);
-        mbar_drain(drain, 0);
+        commit(drain);
+        if (leader) mbar_drain(drain, 0);
       }
     }
   } else {
@@ -758,7 +829,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   }
   } else {
     // ------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AP_REGS_MANY));
     ApWalk walk(p);
     ApSegment sg;
     const int s = warp >> 2;                           // stream
@@ -810,69 +880,64 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if (!ok) break;
         }
         if (warp_valid) {
-          // x scale + shift is the score in log2 units
-          float x[4][32];
-          float top = -INFINITY;
-          auto tops = [&](const float (&v)[32]) {
-            float t0 = v[0], t1 = v[1];
-#pragma unroll
-            for (int e = 2; e < 32; e += 2) {
-              t0 = fmaxf(t0, v[e]);
-              t1 = fmaxf(t1, v[e + 1]);
+          // Two passes over the row's 128 scores in TMEM, 32 at a time so that the
+          // code stays small: the maximum (with a cap, a bias or masks, the
+          // changed scores x go back to TMEM), then the probabilities.
+          // x scale + shift is the score in log2 units.
+          float shift = 0.f, top = -INFINITY;
+          float xa[32], xb[32];
+          auto ld = [&](float (&x)[32], int c) { ap_load(tS + c * 32, x); };
+          if (!kMod && full) {
+            ld(xa, 0);
+#pragma unroll 1
+            for (int c = 0; c < 4; c += 2) {
+              ap_landed(xa);
+              ld(xb, c + 1);
+              top = ap_max32(xa, top);
+              ap_landed(xb);
+              if (c == 0) ld(xa, 2);
+              top = ap_max32(xb, top);
             }
-            top = fmaxf(top, fmaxf(t0, t1));
-          };
-          float shift = 0.f;
-          tmem_ld32(tS, reinterpret_cast<uint32_t(&)[32]>(x[0]));
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 1; c < 4; ++c) {
-            tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c]));
-            if (!kMod && full) tops(x[c - 1]);
-            tmem_wait_ld();
-          }
-          if constexpr (kMod) {
-            if (p.cap_a > 0.f) ap_tanh(x, p.cap_a, p.cap_in);
-            if (p.slopes) {
-              if (k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix)) {
-                // every key the row may see is at or before it: |p - k| = (p - k0) - c
-                shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
-                const uint64_t sl = f2(slope, slope);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                  for (int e = 0; e < 32; e += 2)
-                    f2_split(f2_fma(sl, f2(c * 32 + e, c * 32 + e + 1), f2(x[c][e], x[c][e + 1])), x[c][e],
-                             x[c][e + 1]);
-              } else {
-                const float d0 = static_cast<float>(pos - k0);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                  for (int e = 0; e < 32; ++e)
-                    x[c][e] = fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), x[c][e]);
-              }
-            }
-          }
-          if (!full) {
+          } else {
+            const bool behind = k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix);
+            if (kMod && p.slopes && behind) shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
             uint32_t bad = 0;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
-              uint32_t see = low_bits(hi - k0 - c * 32) & ~low_bits(lo - k0 - c * 32);
-              const int o = sg.f.base - k0 - c * 32;   // drafted token 0's bit in this word
-              if (bits) see |= o >= 32 || o <= -64 ? 0u
-                               : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
-              bad |= see & poison[((g + i) % AP_RING) * 4 + c];
+              ld(xa, c);
+              ap_landed(xa);
+              if constexpr (kMod) {
+                if (p.cap_a > 0.f) ap_tanh(xa, p.cap_a, p.cap_in);
+                if (p.slopes) {
+                  const float c0 = static_cast<float>(c * 32);
+                  if (behind) {   // every key the row sees is at or before it: |p - k| = (p - k0) - c
+                    const uint64_t sl = f2(slope, slope), base = f2(c0, c0);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[c][e] = (see >> e) & 1 ? x[c][e] : -INFINITY;
+                    for (int e = 0; e < 32; e += 2)
+                      f2_split(f2_fma(sl, f2_add(base, f2(e, e + 1)), f2(xa[e], xa[e + 1])), xa[e], xa[e + 1]);
+                  } else {
+                    const float d0 = static_cast<float>(pos - k0) - c0;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                      xa[e] = fmaf(-slope, fabsf(d0 - static_cast<float>(e)), xa[e]);
+                  }
+                }
+              }
+              if (!full) {
+                const int kc = k0 + c * 32;
+                uint32_t see = low_bits(hi - kc) & ~low_bits(lo - kc);
+                const int o = sg.f.base - kc;   // drafted token 0's bit in this word
+                if (bits) see |= o >= 32 || o <= -64 ? 0u
+                                 : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
+                bad |= see & poison[((g + i) % AP_RING) * 4 + c];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) xa[e] = (see >> e) & 1 ? xa[e] : -INFINITY;
+              }
+              top = ap_max32(xa, top);
+              tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(xa));
             }
             if (bad) l = __int_as_float(0x7fffffff);
-          }
-          if (kMod || !full) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tops(x[c]);
-          } else {
-            tops(x[3]);
+            tmem_wait_st();
           }
           const float mt = fmaf(top, p.scale_log2, shift);
           if (i == i_first) {
@@ -885,31 +950,44 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             m = mn;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(tO + s * D + c, o);
-              tmem_wait_ld();
+              ap_load(tO + s * D + c, xb);
+              ap_landed(xb);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-              tmem_st32(tO + s * D + c, o);
+              for (int e = 0; e < 32; ++e) xb[e] *= a;
+              tmem_st32(tO + s * D + c, reinterpret_cast<uint32_t(&)[32]>(xb));
             }
           }
           const float ms = shift - (m == -INFINITY ? 0.f : m);
           const uint64_t sc = f2(p.scale_log2, p.scale_log2), sh = f2(ms, ms);
-          uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+          uint64_t sum0 = f2(0.f, 0.f), sum1 = f2(0.f, 0.f);
+          uint32_t pk[32];
+          auto probabilities = [&](const float (&x)[32], int at) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t pk[32];
-#pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-              float& xa = x[2 * h + (e >> 5)][e & 31];
-              float& xb = x[2 * h + (e >> 5)][(e & 31) + 1];
+            for (int e = 0; e < 32; e += 2) {
               float a, b;
-              f2_split(f2_fma(f2(xa, xb), sc, sh), a, b);
-              a = fast_exp2(a);
-              b = fast_exp2(b);
-              sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], f2(a, b));
-              pk[e >> 1] = ap_pack<kFp16>(a, b);
+              const uint64_t y = f2_fma(f2(x[e], x[e + 1]), sc, sh);
+              if ((e >> 1) % AP_EXP_OF < AP_EXP_POLY) {
+                ap_exp2_pair(y, a, b);
+              } else {
+                f2_split(y, a, b);
+                a = fast_exp2(a);
+                b = fast_exp2(b);
+              }
+              if (e & 2) sum1 = f2_add(sum1, f2(a, b));
+              else sum0 = f2_add(sum0, f2(a, b));
+              pk[at + (e >> 1)] = ap_pack<kFp16>(a, b);
             }
+          };
+          ld(xa, 0);
+          // (P's chunks lie on scores that have been read)
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            ap_landed(xa);
+            ld(xb, 2 * h + 1);
+            probabilities(xa, 0);
+            ap_landed(xb);
+            if (h == 0) ld(xa, 2);
+            probabilities(xb, 16);
             tmem_st32(tS + h * 32, pk);
             tmem_wait_st();
             tc_fence_before();
@@ -917,7 +995,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
           }
           float a, b;
-          f2_split(f2_add(sum[0], sum[1]), a, b);
+          f2_split(f2_add(sum0, sum1), a, b);
           l += a + b;
         } else if (lane == 0) {   // nobody reads this warp's rows
           mbar_arrive(&p_full[2 * s]);
@@ -961,20 +1039,20 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (warp_valid) {
 #pragma unroll 1
           for (int c = c_lo; c < c_hi; c += 32) {
-            uint32_t o[32], o1[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = o1[e] = 0u;
-            if (narrow) {
-              if (n0 > 0) tmem_ld32(tO + c, o);
-              if (n1 > 0) tmem_ld32(tO + D + c, o1);
-            } else if (nt > 0) {
-              tmem_ld32(tO + s * D + c, o);
-            }
-            tmem_wait_ld();
             float v[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              v[e] = narrow ? __uint_as_float(o[e]) * w0 + __uint_as_float(o1[e]) * w1 : __uint_as_float(o[e]);
+            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+            if (nt > 0) {
+              ap_load(tO + (narrow ? 0 : s * D) + c, v);
+              ap_landed(v);
+            }
+            if (narrow && n1 > 0) {
+              float o1[32];
+              ap_load(tO + D + c, o1);
+              ap_landed(o1);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], w0, o1[e] * w1);
+            }
             if (!whole) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)

@@ -103,17 +103,8 @@ template <int D, bool kMod, bool kFp16>
 cudaError_t launch_append(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                           const ApParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  static std::atomic<int> regs{0};
   constexpr int smem = ApSmem<D>::BYTES;
   auto fn = llm_append_kernel<D, kMod, kFp16>;
-  if (regs.load(std::memory_order_relaxed) == 0) {
-    cudaFuncAttributes at;
-    const cudaError_t r = cudaFuncGetAttributes(&at, fn);
-    if (r != cudaSuccess) return r;
-    regs.store(at.numRegs, std::memory_order_relaxed);
-  }
-  // with fewer registers at launch the softmax warps would wait for theirs for ever
-  if (regs.load(std::memory_order_relaxed) < AP_REGS_LAUNCH) return cudaErrorInvalidConfiguration;
   cudaError_t r = smem_attr_once(done, fn, smem);
   if (r != cudaSuccess) return r;
   r = launch_pdl(llm_append_plan_kernel, dim3(1), dim3(AP_PLAN_THREADS), 0, s, p);
