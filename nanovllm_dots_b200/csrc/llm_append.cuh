@@ -45,8 +45,10 @@ namespace dfm {
 constexpr int AP_KT = 128;          // keys per tile
 constexpr int AP_ROWS = 128;        // rows per tile (TMEM lanes)
 constexpr int AP_RING = 2;          // K tiles and V tiles in shared memory
-constexpr int AP_THREADS = 384;
+constexpr int AP_SOFT_WARPS = 8;
+constexpr int AP_THREADS = 32 * (AP_SOFT_WARPS + 4);
 constexpr int AP_PLAN_THREADS = 1024;
+constexpr int AP_NEAR_SEQS = 256, AP_NEAR_UNITS = 512;   // what a CTA plans by itself
 constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's key tile counts 2)
 // The running maximum of a row is raised only when a score passes it by this
 // much (log2 units): probabilities then reach 2^8, exact in fp32 and within
@@ -58,16 +60,21 @@ constexpr int AP_EXP_POLY = 1, AP_EXP_OF = 4;
 struct ApUnit {
   int seq, t0, ntok, row0;          // tokens [t0, t0 + ntok) of the sequence; row0: its first in q
   int lo, hi, fmin, fmax;           // union of the rows' keys; tiles inside [fmin, fmax) have no mask
-  int base, narrow, cost, pad;      // position of token 0; one row tile only; place in the line
-  long long at;
-  long long pad2;
+  int base, narrow;                 // position of token 0; one row tile only
+  int at, pad;                      // place in the line
+  DFM_DEV int tiles() const { return hi > lo ? (hi + AP_KT - 1) / AP_KT - lo / AP_KT : 0; }
+  DFM_DEV int weight() const { return narrow ? 1 : 2; }            // of a key tile
+  DFM_DEV int cost() const { return max(1, tiles() * weight()); }  // in the line
 };
-static_assert(sizeof(ApUnit) == 64, "unit record");
+static_assert(sizeof(ApUnit) == 48, "unit record");
 
 struct ApHead {                     // the plan's header
-  long long line;                   // length of one kv head's line
-  long long share;                  // of one CTA
-  int units, pad;
+  int line, share, units, pad;      // length of one kv head's line, of one CTA's share
+};
+
+struct ApCut {                      // the unit that the end of a share cuts
+  int row, ntok, narrow, kv;        // its first token's row in q
+  int last, pad[3];                 // last share it reaches into; -1: no unit of this share is cut
 };
 
 struct ApParams {
@@ -80,85 +87,214 @@ struct ApParams {
   const float* slopes;              // [H] or null
   void* out;                        // [tokens][H][D]
   uint32_t* err;
-  ApHead* head;
+  ApHead* head;                     // head .. start: of the plan kernel, unused with near_plan
   ApUnit* units;
-  int* ubase;                       // [n + 1]
+  int* ubase;                       // [n]
   int* start;                       // [ctas + 1] unit at the start of each share
+  ApCut* cuts;                      // [ctas]
   float* part_o;                    // [ctas][2][2][D / 4][128][4]
   float2* part_ml;                  // [ctas][2][2][128]
-  int tokens, n, H, KVH, G, RT, max_units, ctas;
+  int tokens, n, H, KVH, G, RT, max_units, ctas, near_plan;
   int num_blocks, block_size, max_blocks, box_rows;
   int causal, window;
-  float scale_log2;                 // what makes log2 units of x (scale * log2(e) without a cap)
-  // With a cap: x = tanh(S cap_a), cap_a = scale / cap, cap_in = 2 log2(e) cap_a,
-  // scale_log2 = cap log2(e).  cap_a 0: none, x = S.
-  float cap_a, cap_in;
+  float scale_log2;                 // scale * log2(e)
+  // With a cap (cap_a 0: none): cap_a = scale / cap, cap_b its inverse, cap_in =
+  // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a.
+  float cap_a, cap_b, cap_in, cap_q[3];
 };
 
 // ---------------------------------------------------------------- plan
-template <class T>
-DFM_DEV T block_exclusive_scan(T v, T* warp_sums, T& total) {   // AP_PLAN_THREADS threads
+// Sums of two values over the threads before this one and over all of the
+// block's kWarps warps.
+template <int kWarps>
+DFM_DEV int2 block_scan(int2 v, int2* warp_sums, int2& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T x = v;
+  int2 x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    const int a = __shfl_up_sync(0xffffffffu, x.x, o), b = __shfl_up_sync(0xffffffffu, x.y, o);
+    if (lane >= o) {
+      x.x += a;
+      x.y += b;
+    }
   }
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    T w = warp_sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const T y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    warp_sums[lane] = w;
-  }
+  int2 w = lane < kWarps ? warp_sums[lane] : make_int2(0, 0);
+  const bool mine = lane < warp;
+  const int2 before = make_int2(__reduce_add_sync(0xffffffffu, mine ? w.x : 0),
+                                __reduce_add_sync(0xffffffffu, mine ? w.y : 0));
+  total = make_int2(__reduce_add_sync(0xffffffffu, w.x), __reduce_add_sync(0xffffffffu, w.y));
   __syncthreads();
-  total = warp_sums[31];
-  const T before = warp ? warp_sums[warp - 1] : 0;
-  __syncthreads();
-  return before + x - v;
+  return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
 }
 
-// Units, their keys and their places in the line, from the device's lengths.
-// A sequence whose lengths make no sense is reported: its rows are written as
-// zeros, or not at all when not even they are known.
+// Rows [s0, s0 + m) of sequence i; whether they make sense.
+DFM_DEV bool ap_rows(const ApParams& p, int i, int& s0, int& m) {
+  s0 = p.cu[i];
+  const int s1 = p.cu[i + 1];
+  m = s1 - s0;
+  return s0 >= 0 && s1 >= s0 && s1 <= p.tokens;
+}
+
+// Whether ctx cached positions with m new tokens make sense.
+DFM_DEV bool ap_length(const ApParams& p, int m, int ctx) {
+  return ctx >= m && ctx <= static_cast<long long>(p.max_blocks) * p.block_size && !(p.tree && m > 64);
+}
+
+// [lo, hi) of new token j (row s0 + j of q) without a tree; pre: the sequence's prefix.
+DFM_DEV void ap_keys(const ApParams& p, int s0, int j, int base, int ctx, int pre, int& lo, int& hi) {
+  const int pos = base + j;
+  hi = p.causal ? max(pos + 1, min(pre, ctx)) : ctx;
+  lo = p.window ? max(0, pos + 1 - p.window) : 0;
+  if (p.first) lo = max(lo, p.first[s0 + j]);
+}
+
+// The unit at token t0 of a sequence; with per-token bounds (p.first) lo .. fmax
+// are the caller's.
+DFM_DEV ApUnit ap_unit(const ApParams& p, int seq, int s0, int m, int ctx, int pre, int t0) {
+  ApUnit f;
+  f.seq = seq;
+  f.t0 = t0;
+  f.ntok = min(2 * p.RT, m - t0);
+  f.row0 = s0;
+  f.base = ctx - m;
+  f.narrow = f.ntok <= p.RT;
+  f.lo = f.hi = f.fmax = 0;
+  f.fmin = 0x7fffffff;
+  f.at = 0;
+  if (ap_length(p, m, ctx)) {
+    if (p.tree) {
+      f.hi = ctx;
+      f.fmin = 0;
+      f.fmax = f.base;
+    } else if (!p.first) {   // the ends of the interval rise with the token
+      ap_keys(p, s0, t0, f.base, ctx, pre, f.lo, f.fmax);
+      ap_keys(p, s0, t0 + f.ntok - 1, f.base, ctx, pre, f.fmin, f.hi);
+    }
+  }
+  return f;
+}
+
+DFM_DEV int ap_share(const ApParams& p, int line) {
+  return max(AP_MIN_SHARE, (line * p.KVH + p.ctas - 1) / p.ctas);
+}
+
+// The plan of a batch small enough for every CTA to make it in its own shared
+// memory: that takes about a microsecond, a kernel of its own three.
+struct ApNear {
+  int s0[AP_NEAR_SEQS], m[AP_NEAR_SEQS], ctx[AP_NEAR_SEQS], pre[AP_NEAR_SEQS], ubase[AP_NEAR_SEQS];
+  int at[AP_NEAR_UNITS];
+  uint16_t seq[AP_NEAR_UNITS];
+  int2 sums[AP_THREADS / 32];
+  int line, units;
+
+  // The last place of an ascending list with list[place] <= x; a whole warp.
+  static DFM_DEV int last_at_most(const int* list, int n, int x) {
+    const int lane = threadIdx.x & 31;
+    int a = 0;
+    for (int step = 32; step > 0; step = step == 32 ? 1 : 0) {   // blocks of 32, then within one
+      int k = 0;
+      for (int i0 = 0; step == 32 && i0 < n; i0 += 1024) {
+        const int i = i0 + lane * 32;
+        k += __popc(__ballot_sync(0xffffffffu, i < n && list[i] <= x));
+      }
+      if (step == 32) a = (k - 1) * 32;
+      else a += __popc(__ballot_sync(0xffffffffu, a + lane < n && list[a + lane] <= x)) - 1;
+    }
+    return a;
+  }
+  DFM_DEV ApUnit unit(const ApParams& p, int u) const {
+    const int i = seq[u];
+    ApUnit f = ap_unit(p, i, s0[i], m[i], ctx[i], pre[i], (u - ubase[i]) * 2 * p.RT);
+    f.at = at[u];
+    return f;
+  }
+  // All AP_THREADS threads.
+  DFM_DEV void make(const ApParams& p) {
+    const int t = threadIdx.x;
+    int c = 0, cost = 0, s = 0, k = 0, x = 0, pr = 0;
+    if (t < p.n) {
+      const bool rows = ap_rows(p, t, s, k);
+      x = p.ctx[t];
+      if (p.prefix) pr = p.prefix[t];
+      if (rows) c = (k + 2 * p.RT - 1) / (2 * p.RT);
+      if (blockIdx.x == 0 && !(rows && ap_length(p, k, x))) atomicOr(p.err, DFM_DEV_ERR_LEN);
+      if (c > 0) cost = ap_unit(p, t, s, k, x, pr, 0).cost();
+      s0[t] = s;
+      m[t] = k;
+      ctx[t] = x;
+      pre[t] = pr;
+    }
+    const bool several = __syncthreads_or(c > 1);
+    int2 all;
+    const int2 before = block_scan<AP_THREADS / 32>(make_int2(c, cost), sums, all);
+    if (t < p.n) ubase[t] = before.x;
+    if (all.x > p.max_units) {   // rows of overlapping sequences
+      if (blockIdx.x == 0 && t == 0) atomicOr(p.err, DFM_DEV_ERR_LEN);
+      all.x = p.max_units;
+    }
+    if (!several) {              // a unit to a sequence: their places are known
+      if (c > 0 && before.x < all.x) {
+        seq[before.x] = static_cast<uint16_t>(t);
+        at[before.x] = before.y;
+      }
+    } else {
+      __syncthreads();
+      all.y = 0;
+      for (int u0 = 0; u0 < all.x; u0 += AP_THREADS) {
+        const int u = u0 + t;
+        cost = 0;
+        if (u < all.x) {
+          int a = 0, b = p.n - 1;   // the last sequence with ubase <= u (one without units shares the next one's)
+          while (a < b) {
+            const int mid = (a + b + 1) >> 1;
+            if (ubase[mid] <= u) a = mid; else b = mid - 1;
+          }
+          seq[u] = static_cast<uint16_t>(a);
+          cost = ap_unit(p, a, s0[a], m[a], ctx[a], pre[a], (u - ubase[a]) * 2 * p.RT).cost();
+        }
+        int2 sum;
+        const int2 place = block_scan<AP_THREADS / 32>(make_int2(cost, 0), sums, sum);
+        if (u < all.x) at[u] = all.y + place.x;
+        all.y += sum.x;
+      }
+    }
+    if (t == 0) {
+      line = all.y;
+      units = all.x;
+    }
+    __syncthreads();
+  }
+};
+static_assert(AP_NEAR_SEQS <= AP_THREADS, "a thread to a sequence");
+
+// The plan of larger batches, and of per-token bounds: units, their keys and
+// their places in the line, from the device's lengths.  A sequence whose lengths
+// make no sense is reported: its rows are written as zeros, or not at all when
+// not even they are known.
 __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApParams p) {
-  __shared__ int sums[32];
-  __shared__ long long lsums[32];
+  __shared__ int2 sums[32];
   __shared__ int near[AP_PLAN_THREADS];   // ubase of the first sequences
+  constexpr int W = AP_PLAN_THREADS / 32;
   pdl_trigger();
   pdl_wait();
   const int t = threadIdx.x;
-  auto rows_ok = [&](int i, int& s0, int& m) {
-    s0 = p.cu[i];
-    const int s1 = p.cu[i + 1];
-    m = s1 - s0;
-    return s0 >= 0 && s1 >= s0 && s1 <= p.tokens;
-  };
   int carry = 0;
   for (int i0 = 0; i0 < p.n; i0 += AP_PLAN_THREADS) {
     const int i = i0 + t;
     int c = 0;
     if (i < p.n) {
       int s0, m;
-      if (rows_ok(i, s0, m)) {
-        c = (m + 2 * p.RT - 1) / (2 * p.RT);
-        const int ctx = p.ctx[i];
-        if (ctx < m || ctx > static_cast<long long>(p.max_blocks) * p.block_size || (p.tree && m > 64))
-          atomicOr(p.err, DFM_DEV_ERR_LEN);
-      } else {
-        atomicOr(p.err, DFM_DEV_ERR_LEN);
-      }
+      const bool rows = ap_rows(p, i, s0, m);
+      if (rows) c = (m + 2 * p.RT - 1) / (2 * p.RT);
+      if (!(rows && ap_length(p, m, p.ctx[i]))) atomicOr(p.err, DFM_DEV_ERR_LEN);
     }
-    int total;
-    const int at = block_exclusive_scan(c, sums, total);
+    int2 total;
+    const int at = block_scan<W>(make_int2(c, 0), sums, total).x;
     if (i < AP_PLAN_THREADS) near[i] = carry + at;
     else if (i < p.n) p.ubase[i] = carry + at;
-    carry += total;
+    carry += total.x;
   }
   int units = carry;
   if (units > p.max_units) {   // rows of overlapping sequences
@@ -175,23 +311,17 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
     }
     return a;
   };
-  // [lo, hi) of a token
-  auto keys = [&](int seq, int s0, int j, int base, int ctx, int& lo, int& hi) {
-    const int pos = base + j;
-    hi = p.causal ? max(pos + 1, p.prefix ? min(p.prefix[seq], ctx) : 0) : ctx;
-    lo = p.window ? max(0, pos + 1 - p.window) : 0;
-    if (p.first) lo = max(lo, p.first[s0 + j]);
-  };
   if (p.first) {   // every token has bounds of its own: a warp to a unit
-    for (int u = t >> 5; u < units; u += AP_PLAN_THREADS / 32) {
+    for (int u = t >> 5; u < units; u += W) {
       const int a = seq_of(u);
       int s0, m;
-      rows_ok(a, s0, m);
-      const int ctx = p.ctx[a], t0 = (u - ubase(a)) * 2 * p.RT, end = min(m, t0 + 2 * p.RT);
+      ap_rows(p, a, s0, m);
+      const int ctx = p.ctx[a], pre = p.prefix ? p.prefix[a] : 0;
+      const int t0 = (u - ubase(a)) * 2 * p.RT, end = min(m, t0 + 2 * p.RT);
       int lo = 0x7fffffff, hi = 0, fmin = 0, fmax = 0x7fffffff;
       for (int j = t0 + (t & 31); j < end; j += 32) {
         int l, h;
-        keys(a, s0, j, ctx - m, ctx, l, h);
+        ap_keys(p, s0, j, ctx - m, ctx, pre, l, h);
         if (l < h) {
           lo = min(lo, l);
           hi = max(hi, h);
@@ -207,50 +337,35 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
     }
     __syncthreads();
   }
-  long long line = 0;
+  int line = 0;
   for (int u0 = 0; u0 < units; u0 += AP_PLAN_THREADS) {
     const int u = u0 + t;
-    ApUnit f{};
+    ApUnit f;
+    int cost = 0;
     if (u < units) {
       const int a = seq_of(u);
       int s0, m;
-      rows_ok(a, s0, m);
+      ap_rows(p, a, s0, m);
       const int ctx = p.ctx[a];
-      f.seq = a;
-      f.t0 = (u - ubase(a)) * 2 * p.RT;
-      f.ntok = min(2 * p.RT, m - f.t0);
-      f.row0 = s0;
-      f.base = ctx - m;
-      f.narrow = f.ntok <= p.RT;
-      const bool good = ctx >= m && ctx <= static_cast<long long>(p.max_blocks) * p.block_size &&
-                        !(p.tree && m > 64);
-      if (good && p.tree) {
-        f.hi = ctx;
-        f.fmax = f.base;
-      } else if (good && p.first) {
+      f = ap_unit(p, a, s0, m, ctx, p.prefix ? p.prefix[a] : 0, (u - ubase(a)) * 2 * p.RT);
+      if (p.first && ap_length(p, m, ctx)) {
         const int4 b = *reinterpret_cast<const int4*>(&p.units[u].lo);
         f.lo = b.x;
         f.hi = b.y;
         f.fmin = b.z;
         f.fmax = b.w;
-      } else if (good) {   // the ends of the interval rise with the token
-        keys(a, s0, f.t0, f.base, ctx, f.lo, f.fmax);
-        keys(a, s0, f.t0 + f.ntok - 1, f.base, ctx, f.fmin, f.hi);
       }
-      if (f.hi <= f.lo) {
-        f.lo = f.hi = f.fmax = 0;
-        f.fmin = 0x7fffffff;
-      }
-      const int tiles = f.hi > f.lo ? (f.hi + AP_KT - 1) / AP_KT - f.lo / AP_KT : 0;
-      f.cost = max(1, tiles * (f.narrow ? 1 : 2));
+      cost = f.cost();
     }
-    long long total;
-    f.at = line + block_exclusive_scan(static_cast<long long>(f.cost), lsums, total);
-    if (u < units) p.units[u] = f;
-    line += total;
+    int2 total;
+    const int at = line + block_scan<W>(make_int2(cost, 0), sums, total).x;
+    if (u < units) {
+      f.at = at;
+      p.units[u] = f;
+    }
+    line += total.x;
   }
-  long long share = (line * p.KVH + p.ctas - 1) / p.ctas;
-  if (share < AP_MIN_SHARE) share = AP_MIN_SHARE;
+  const int share = ap_share(p, line);
   if (t == 0) {
     p.head->line = line;
     p.head->share = share;
@@ -258,11 +373,10 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
   }
   // the unit at the start of each share
   for (int u = t; u < units; u += AP_PLAN_THREADS) {
-    const ApUnit& f = p.units[u];
+    const ApUnit f = p.units[u];
     for (int kv = 0; kv < p.KVH; ++kv) {
-      const long long a = kv * line + f.at, b = a + f.cost;
-      for (long long c = (a + share - 1) / share; c * share < b; ++c)
-        if (c <= p.ctas) p.start[c] = u;
+      const int a = kv * line + f.at, b = a + f.cost();
+      for (int c = (a + share - 1) / share; c * share < b; ++c) p.start[c] = u;
     }
   }
 }
@@ -276,37 +390,38 @@ struct ApSegment {
 };
 
 struct ApWalk {
-  long long left, line;
+  const ApNear& near;
+  int left, line, share, off;       // off: into the unit
   int u, kv, units;
-  long long off;                    // into the unit
 
-  DFM_DEV ApWalk(const ApParams& p) {
-    line = p.head->line;
-    units = p.head->units;
-    const long long share = p.head->share, all = line * p.KVH;
-    const long long g = blockIdx.x * share;
-    left = g < all ? (g + share < all ? share : all - g) : 0;
+  DFM_DEV ApWalk(const ApParams& p, const ApNear& nr) : near(nr) {
+    line = p.near_plan ? near.line : p.head->line;
+    units = p.near_plan ? near.units : p.head->units;
+    share = p.near_plan ? ap_share(p, line) : p.head->share;
+    const int all = line * p.KVH, g = blockIdx.x * share;
+    left = max(0, min(share, all - g));
     if (left > 0) {
-      kv = static_cast<int>(g / line);
-      u = p.start[blockIdx.x];
-      off = g - kv * line - p.units[u].at;
+      kv = g / line;
+      const int r = g - kv * line;
+      u = p.near_plan ? ApNear::last_at_most(near.at, units, r) : p.start[blockIdx.x];
+      off = r - (p.near_plan ? near.at[u] : p.units[u].at);
     }
   }
   // The next segment with work; false at the end of the share.
   DFM_DEV bool next(const ApParams& p, ApSegment& s) {
     while (left > 0) {
-      s.f = p.units[u];
+      s.f = p.near_plan ? near.unit(p, u) : p.units[u];
       s.kv = kv;
-      const int c = s.f.narrow ? 1 : 2;
-      s.tiles = s.f.hi > s.f.lo ? (s.f.hi + AP_KT - 1) / AP_KT - s.f.lo / AP_KT : 0;
+      const int wide = 1 - s.f.narrow, cost = s.f.cost();   // a wide unit's tile counts 2
+      s.tiles = s.f.tiles();
       s.top = (s.f.hi + AP_KT - 1) / AP_KT - 1;
-      const long long end = off + left < s.f.cost ? off + left : s.f.cost;
-      s.i0 = static_cast<int>((off + c - 1) / c);
-      s.i1 = min(s.tiles, static_cast<int>((end + c - 1) / c));
+      const int end = min(off + left, cost);
+      s.i0 = (off + wide) >> wide;
+      s.i1 = min(s.tiles, (end + wide) >> wide);
       const bool zero = s.tiles == 0 && off == 0;
       left -= end - off;
       off = end;
-      if (end == s.f.cost) {
+      if (end == cost) {
         off = 0;
         if (++u == units) {
           u = 0;
@@ -326,12 +441,14 @@ struct ApSmem {
   static constexpr int BOXES = D / 64;
   static constexpr int TILE = AP_KT * D * 2;              // one K, V or Q tile
   static constexpr int HALF = AP_KT * 128;                // its 64-dim boxes
+  static constexpr int STAGE = 32 * 64;                   // a warp's 32 rows of 32 values
   static constexpr int OFF_Q = 0;                         // [2]
   static constexpr int OFF_K = OFF_Q + 2 * TILE;          // [AP_RING]
   static constexpr int OFF_V = OFF_K + AP_RING * TILE;    // [AP_RING]
-  static constexpr int OFF_OUT = OFF_V + AP_RING * TILE;  // [8 warps][32 rows][64 bytes]
-  static constexpr int OFF_ML = OFF_OUT + 8 * 32 * 64;   // float2 [2][128]
-  static constexpr int OFF_BAR = OFF_ML + 2 * AP_ROWS * 8;
+  static constexpr int OFF_OUT = OFF_V + AP_RING * TILE;  // [softmax warps]
+  static constexpr int OFF_ML = OFF_OUT + AP_SOFT_WARPS * STAGE;     // float2 [2 streams][128]
+  static constexpr int OFF_NEAR = OFF_ML + 2 * AP_ROWS * 8;
+  static constexpr int OFF_BAR = OFF_NEAR + (static_cast<int>(sizeof(ApNear)) + 15) / 16 * 16;
   static constexpr int BYTES = OFF_BAR + 512 + 1024;
 };
 static_assert(ApSmem<128>::BYTES <= 232448, "one CTA per SM");
@@ -385,16 +502,16 @@ DFM_DEV void mbar_drain(uint64_t* bar, uint32_t parity) {
   }
 }
 
-// Barrier over the 256 softmax threads; the AND of their predicates.
-DFM_DEV bool ap_pair_sync(bool ok) {
+// Barrier `id` over `threads` threads (whole warps); the AND of their predicates.
+DFM_DEV bool ap_meet(int id, int threads, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 256, p;\n\t"
+      "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(static_cast<uint32_t>(ok))
+      : "r"(static_cast<uint32_t>(ok)), "r"(id), "r"(threads)
       : "memory");
   return r != 0;
 }
@@ -425,6 +542,17 @@ DFM_DEV void ap_landed(float (&x)[32]) {
                : "memory");
 }
 
+// 0 x + sum for two 16-bit values.
+template <bool kFp16>
+DFM_DEV uint32_t ap_zero_times(uint32_t x, uint32_t sum) {
+  uint32_t r;
+  if constexpr (kFp16)
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(sum));
+  else
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(sum));
+  return r;
+}
+
 // Two fp32 operations in one instruction.
 DFM_DEV uint64_t f2(float a, float b) {
   uint64_t r;
@@ -453,8 +581,6 @@ DFM_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
 // The lowest n bits, n clamped to [0, 32].
 DFM_DEV uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
-constexpr float AP_T0 = 0.999999972f, AP_T1 = -0.333329668f, AP_T2 = 0.133255161f, AP_T3 = -0.0533498438f, AP_T4 = 0.0195938116f, AP_T5 = -0.0047239585f;
-
 // 2^x of two scores on the fp32 pipe: x = n + f with n the nearest integer, 2^f by
 // the polynomial of degree 5 fitted at Chebyshev nodes of [-1/2, 1/2] (1e-7
 // relative), times 2^n, which for n = -127 comes out as an exact 0 (masked scores are
@@ -481,32 +607,32 @@ DFM_DEV void ap_exp2_pair(uint64_t x, float& a, float& b) {
   f2_split(q, a, b);
 }
 
-// tanh(S a) for 32 scores of a row.  Where every score of the warp's chunk is
-// below 0.75 caps, tanh y = y q(y^2) with q the polynomial of degree 5 fitted at
-// Chebyshev nodes of [0, 0.75^2] (3e-8 relative): 3.5 instructions a score on the
-// fp32 pipe.  Else 1 - 2 / (1 + e^{2y}): two special-function operations, of
-// which an SM does 16 a clock, so that they and the softmax's exponential would
+// x = (cap / scale) tanh(S scale / cap) of 32 scores of a row (x scale is the
+// capped score).  Where every score of the warp's chunk is below half the cap,
+// tanh y = y q(y^2) with q the cubic fitted at Chebyshev nodes of [0, 1/4] (6e-7
+// relative), its coefficients scaled so that x = S q(S^2): 2.5 instructions a score
+// on the fp32 pipe.  Else 1 - 2 / (1 + e^{2y}): two special-function operations,
+// of which an SM does 16 a clock, so that they and the softmax's exponential would
 // take three times the products' time.
-DFM_DEV void ap_tanh(float (&x)[32], float a, float cap_in) {
+constexpr float AP_T0 = 0.999999464f, AP_T1 = -0.33326377f, AP_T2 = 0.131909163f, AP_T3 = -0.0444185946f;
+DFM_DEV void ap_cap(float (&x)[32], const ApParams& p) {
   float big = 0.f;
 #pragma unroll
   for (int e = 0; e < 32; ++e) big = fmaxf(big, fabsf(x[e]));
   // (a NaN is not above the bound and stays one in the polynomial)
-  if (__any_sync(0xffffffffu, big * a > 0.75f)) {
+  if (__any_sync(0xffffffffu, big * p.cap_a > 0.5f)) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      x[e] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(x[e] * cap_in)), 1.f);
+    for (int e = 0; e < 32; ++e) {
+      const float r = __fdividef(1.f, 1.f + fast_exp2(x[e] * p.cap_in));
+      x[e] = fmaf(-2.f * p.cap_b, r, p.cap_b);
+    }
     return;
   }
-  const uint64_t aa = f2(a, a);
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
-    const uint64_t y = f2_mul(f2(x[e], x[e + 1]), aa), z = f2_mul(y, y);
-    uint64_t q = f2(AP_T5, AP_T5);
-    q = f2_fma(q, z, f2(AP_T4, AP_T4));
-    q = f2_fma(q, z, f2(AP_T3, AP_T3));
-    q = f2_fma(q, z, f2(AP_T2, AP_T2));
-    q = f2_fma(q, z, f2(AP_T1, AP_T1));
+    const uint64_t y = f2(x[e], x[e + 1]), z = f2_mul(y, y);
+    uint64_t q = f2_fma(f2(p.cap_q[2], p.cap_q[2]), z, f2(p.cap_q[1], p.cap_q[1]));
+    q = f2_fma(q, z, f2(p.cap_q[0], p.cap_q[0]));
     q = f2_fma(q, z, f2(AP_T0, AP_T0));
     f2_split(f2_mul(y, q), x[e], x[e + 1]);
   }
@@ -527,7 +653,7 @@ DFM_DEV float ap_max32(const float (&x)[32], float top) {
 template <int D, bool kMod, bool kFp16>
 __global__ void __launch_bounds__(AP_THREADS, 1)
     llm_append_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v, const ApParams p) {
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ApParams p) {
   using S = ApSmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -536,6 +662,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   uint8_t* sK = smem + S::OFF_K;
   uint8_t* sV = smem + S::OFF_V;
   float2* sML = reinterpret_cast<float2*>(smem + S::OFF_ML);
+  ApNear& near = *reinterpret_cast<ApNear*>(smem + S::OFF_NEAR);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint64_t* k_empty = k_full + AP_RING;
   uint64_t* v_full = k_empty + AP_RING;
@@ -576,7 +703,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     tma_prefetch(&tm_k);
     tma_prefetch(&tm_v);
   }
-  if (warp == 9) {
+  if (warp == AP_SOFT_WARPS + 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -586,11 +713,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
   pdl_wait();
-
-  if (warp >= 8) {
-  ApWalk walk(p);
+  if (p.near_plan) near.make(p);
+  ApWalk walk(p, near);
   ApSegment sg;
-  if (warp == 8) {
+
+  if (warp == AP_SOFT_WARPS) {
     // ------------------------------------------------------------ TMA
     const int per_tile = AP_KT / p.box_rows;         // boxes along the keys
     const int box_bytes = p.box_rows * 128;
@@ -598,6 +725,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     bool ok = true;
     while (ok && walk.next(p, sg)) {
       if (sg.i1 == sg.i0) continue;
+      const int* bt = p.bt + static_cast<size_t>(sg.f.seq) * p.max_blocks;
+      // lane = (box along the keys, 64-dim half); lanes past the tile's boxes are idle
+      const int box = lane / S::BOXES, half = lane % S::BOXES;
+      auto block_of = [&](int i) {   // the lane's cache block in tile i, -2 if nobody sees the box
+        const int key = (sg.top - i) * AP_KT + box * p.box_rows;
+        if (box >= per_tile || i >= sg.i1 || key + p.box_rows <= sg.f.lo || key >= sg.f.hi) return -2;
+        const int b = bt[key / p.block_size];
+        return b < 0 ? -1 : b;
+      };
+      int blk = block_of(sg.i0);
       if (lane == 0) {
         ok = nseg == 0 || ap_wait(q_empty, (nseg - 1) & 1, abort_flag, p.err);
         if (ok) {
@@ -611,16 +748,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       ++nseg;
-      const int* bt = p.bt + static_cast<size_t>(sg.f.seq) * p.max_blocks;
-      // lane = (box along the keys, 64-dim half); lanes past the tile's boxes are idle
-      const int box = lane / S::BOXES, half = lane % S::BOXES;
-      auto block_of = [&](int i) {   // the lane's cache block in tile i, -2 if nobody sees the box
-        const int key = (sg.top - i) * AP_KT + box * p.box_rows;
-        if (box >= per_tile || i >= sg.i1 || key + p.box_rows <= sg.f.lo || key >= sg.f.hi) return -2;
-        const int b = bt[key / p.block_size];
-        return b < 0 ? -1 : b;
-      };
-      int blk = block_of(sg.i0);
       for (int i = sg.i0; ok && i < sg.i1; ++i, ++g) {
         const int slot = g % AP_RING;
         const int key = (sg.top - i) * AP_KT + box * p.box_rows;
@@ -661,7 +788,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         mbar_drain(&v_full[x % AP_RING], (x / AP_RING) & 1);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == AP_SOFT_WARPS + 1) {
     // ------------------------------------------------------------ MMA
     // The whole warp walks and waits, so that descriptors are built in uniform
     // registers; one elected lane issues.
@@ -778,10 +905,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (leader) mbar_drain(drain, 0);
       }
     }
-  } else {
+  } else if (warp > AP_SOFT_WARPS) {
     // ------------------------------------------------------------ special rows of V
-    const int w = warp - 10;
-    const uint32_t inf2 = kFp16 ? 0x7c007c00u : 0x7f807f80u;
+    const int w = warp - AP_SOFT_WARPS - 2;
     int g = 0;
     bool ok = true;
     while (ok && walk.next(p, sg)) {
@@ -799,23 +925,20 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             const bool seen = key >= sg.f.lo && key < sg.f.hi;
             bool special = false;
             if (seen && split) {
-              uint32_t top = 0;    // per half word, the largest magnitude's bits
-#pragma unroll
-              for (int b = 0; b < S::BOXES; ++b)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                  const uint4 u = *reinterpret_cast<const uint4*>(row + b * S::HALF + ((c ^ (r & 7)) << 4));
-                  top = __vimax3_u16x2(top, u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
-                  top = __vimax3_u16x2(top, u.z & 0x7fff7fffu, u.w & 0x7fff7fffu);
-                }
-              special = (top & 0xffffu) >= (inf2 & 0xffffu) || (top >> 16) >= (inf2 >> 16);
+              // 0 x is NaN for an infinity or a NaN, and stays in the sum
+              uint32_t sum = 0;
+#pragma unroll 4
+              for (int c = 0; c < 8 * S::BOXES; ++c) {
+                const uint4 u = *reinterpret_cast<const uint4*>(row + (c >> 3) * S::HALF + (((c & 7) ^ (r & 7)) << 4));
+                sum = ap_zero_times<kFp16>(u.x, ap_zero_times<kFp16>(u.y, sum));
+                sum = ap_zero_times<kFp16>(u.z, ap_zero_times<kFp16>(u.w, sum));
+              }
+              special = (sum & 0x7fff7fffu) != 0;
             }
             if (!seen || special) {
-#pragma unroll
-              for (int b = 0; b < S::BOXES; ++b)
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                  *reinterpret_cast<uint4*>(row + b * S::HALF + (c << 4)) = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+              for (int c = 0; c < 8 * S::BOXES; ++c)
+                *reinterpret_cast<uint4*>(row + (c >> 3) * S::HALF + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
             }
             const uint32_t word = __ballot_sync(0xffffffffu, special);
             if (lane == 0) poison[slot * 4 + w * 2 + x] = word;
@@ -826,20 +949,19 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (lane == 0) mbar_arrive(&v_ready[slot]);
       }
     }
-  }
   } else {
     // ------------------------------------------------------------ softmax
-    ApWalk walk(p);
-    ApSegment sg;
     const int s = warp >> 2;                           // stream
     const int r = (warp & 3) * 32 + lane;              // row of the tile, TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + s * AP_KT + lane_off, tO = tmem + 256 + lane_off;
     const int tok_of = r / p.G, head_of = r % p.G;
-    uint8_t* stage = smem + S::OFF_OUT + warp * 32 * 64;
+    uint8_t* stage = smem + S::OFF_OUT + warp * S::STAGE;
     int g = 0, ns = 0;                                 // V tiles of the CTA, score tiles of the stream
     int no[2] = {0, 0};                                // segments each stream had tiles in
     bool ok = true;
+    ApCut cut;
+    cut.last = -1;
     while (walk.next(p, sg)) {
       const int nt = sg.i1 - sg.i0;
       const bool narrow = sg.f.narrow;
@@ -857,14 +979,19 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           bits = p.tree[sg.f.row0 + j] & (m >= 64 ? ~0ull : (1ull << m) - 1);
           hi = sg.f.base;
         } else {
-          const int ctx = p.ctx[sg.f.seq];
-          hi = p.causal ? max(pos + 1, p.prefix ? min(p.prefix[sg.f.seq], ctx) : 0) : ctx;
-          lo = p.window ? max(0, pos + 1 - p.window) : 0;
-          if (p.first) lo = max(lo, p.first[sg.f.row0 + j]);
+          ap_keys(p, sg.f.row0, j, sg.f.base, p.ctx[sg.f.seq], p.prefix ? p.prefix[sg.f.seq] : 0, lo, hi);
         }
         // in units of x
         if (kMod && p.slopes) slope = p.slopes[sg.kv * p.G + head_of] * (1.4426950408889634f / p.scale_log2);
       }
+      // which of the 32 keys from kc on the row sees
+      auto sees = [&](int kc) {
+        uint32_t see = low_bits(hi - kc) & ~low_bits(lo - kc);
+        const int o = sg.f.base - kc;   // drafted token 0's bit in this word
+        if (bits) see |= o >= 32 || o <= -64 ? 0u
+                         : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
+        return see;
+      };
       float m = -INFINITY, l = 0.f;
       const int step = narrow ? 2 : 1, i_first = narrow ? s : 0;
 #pragma unroll 1
@@ -874,11 +1001,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         tc_fence_after();
         const int k0 = (sg.top - sg.i0 - i) * AP_KT;
         const bool full = k0 >= sg.f.fmin && k0 + AP_KT <= sg.f.fmax;
-        if (!full) {
-          const int slot = (g + i) % AP_RING;
-          ok = __all_sync(0xffffffffu, ap_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
-          if (!ok) break;
-        }
         if (warp_valid) {
           // Two passes over the row's 128 scores in TMEM, 32 at a time so that the
           // code stays small: the maximum (with a cap, a bias or masks, the
@@ -901,13 +1023,14 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           } else {
             const bool behind = k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix);
             if (kMod && p.slopes && behind) shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
-            uint32_t bad = 0;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               ld(xa, c);
+              const uint32_t see = full ? ~0u : sees(k0 + c * 32);
+              const bool masked = __any_sync(0xffffffffu, see != ~0u);
               ap_landed(xa);
               if constexpr (kMod) {
-                if (p.cap_a > 0.f) ap_tanh(xa, p.cap_a, p.cap_in);
+                if (p.cap_a > 0.f) ap_cap(xa, p);
                 if (p.slopes) {
                   const float c0 = static_cast<float>(c * 32);
                   if (behind) {   // every key the row sees is at or before it: |p - k| = (p - k0) - c
@@ -923,20 +1046,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                   }
                 }
               }
-              if (!full) {
-                const int kc = k0 + c * 32;
-                uint32_t see = low_bits(hi - kc) & ~low_bits(lo - kc);
-                const int o = sg.f.base - kc;   // drafted token 0's bit in this word
-                if (bits) see |= o >= 32 || o <= -64 ? 0u
-                                 : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
-                bad |= see & poison[((g + i) % AP_RING) * 4 + c];
+              if (masked) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) xa[e] = (see >> e) & 1 ? xa[e] : -INFINITY;
               }
               top = ap_max32(xa, top);
-              tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(xa));
+              if (kMod || masked) tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(xa));
             }
-            if (bad) l = __int_as_float(0x7fffffff);
             tmem_wait_st();
           }
           const float mt = fmaf(top, p.scale_log2, shift);
@@ -997,6 +1113,14 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           float a, b;
           f2_split(f2_add(sum0, sum1), a, b);
           l += a + b;
+          if (!full) {   // special values of V that this row sees
+            const int slot = (g + i) % AP_RING;
+            ok = __all_sync(0xffffffffu, ap_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
+            if (!ok) break;
+            uint32_t bad = 0;
+            for (int c = 0; c < 4; ++c) bad |= poison[slot * 4 + c] & sees(k0 + c * 32);
+            if (bad) l = __int_as_float(0x7fffffff);
+          }
         } else if (lane == 0) {   // nobody reads this warp's rows
           mbar_arrive(&p_full[2 * s]);
           mbar_arrive(&p_full[2 * s + 1]);
@@ -1007,7 +1131,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       float w0 = 1.f, w1 = 0.f;       // weights of O_0 and O_1 (narrow)
       if (narrow) {
         sML[s * AP_ROWS + r] = make_float2(m, l);
-        ok = ap_pair_sync(ok);
+        ok = ap_meet(1, 32 * AP_SOFT_WARPS, ok);
         const float2 o = sML[(1 - s) * AP_ROWS + r];
         const float mm = fmaxf(m, o.x);
         const float wm = m == -INFINITY ? 0.f : fast_exp2(m - mm), wo = o.x == -INFINITY ? 0.f : fast_exp2(o.x - mm);
@@ -1054,6 +1178,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], w0, o1[e] * w1);
             }
             if (!whole) {
+              if (!valid) continue;
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
                 *reinterpret_cast<float4*>(po + (static_cast<size_t>((c + e) >> 2) * AP_ROWS + r) * 4) =
@@ -1081,13 +1206,21 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           }
         }
       }
+      if (sg.i0 == 0 && !sg.whole()) {     // the end of the share cuts this unit
+        cut.row = sg.f.row0 + sg.f.t0;
+        cut.ntok = sg.f.ntok;
+        cut.narrow = sg.f.narrow;
+        cut.kv = sg.kv;
+        cut.last = (sg.kv * walk.line + sg.f.at + (2 - sg.f.narrow) * (sg.tiles - 1)) / walk.share;
+      }
       tc_fence_before();
-      if (narrow) ok = ap_pair_sync(ok);   // both have read O_0 and O_1
+      if (narrow) ok = ap_meet(1, 32 * AP_SOFT_WARPS, ok);   // both have read O_0 and O_1
     }
+    if (threadIdx.x == 0) p.cuts[blockIdx.x] = cut;
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == AP_SOFT_WARPS + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -1095,30 +1228,23 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 
 // ---------------------------------------------------------------- split units
 // Block (b, y): the unit that the end of share b cuts, if it began in share b,
-// rows and columns [y * 256, (y + 1) * 256) of its (tile, 16-dim group, row)
-// list.  out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the shares.
+// items [y * 256, (y + 1) * 256) of its (tile, 16-dim group, row) list.
+// out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the shares, in their order.
 template <int D, bool kFp16>
 __global__ void __launch_bounds__(256) llm_append_combine_kernel(const ApParams p) {
   constexpr int CB = 4;
   pdl_trigger();
   pdl_wait();
-  const long long line = p.head->line, share = p.head->share;
   const int b = blockIdx.x;
-  const long long cut = (b + 1) * share;
-  if (cut >= line * p.KVH) return;
-  const int kv = static_cast<int>(cut / line);
-  const ApUnit f = p.units[p.start[b + 1]];
-  const long long begin = kv * line + f.at;
-  const int tiles = f.hi > f.lo ? (f.hi + AP_KT - 1) / AP_KT - f.lo / AP_KT : 0;
-  if (begin >= cut || begin / share != b || tiles == 0) return;
-  const int last = static_cast<int>((begin + (f.narrow ? 1 : 2) * (tiles - 1)) / share);
-  if (last == b) return;
+  const ApCut f = p.cuts[b];
+  const int last = f.last;
+  if (last <= b) return;
   const int task = blockIdx.y * 256 + threadIdx.x;
   const int r = task % AP_ROWS, rest = task / AP_ROWS;
   const int dg = rest % (D / 16), tile = rest / (D / 16);
   if (tile > (f.narrow ? 0 : 1)) return;
-  const int tok = r / p.G, j = f.t0 + tile * p.RT + tok;
-  if (tok >= p.RT || j >= f.t0 + f.ntok) return;
+  const int tok = r / p.G, j = tile * p.RT + tok;
+  if (tok >= p.RT || j >= f.ntok) return;
   float M = -INFINITY, L = 0.f, acc[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -1164,7 +1290,7 @@ __global__ void __launch_bounds__(256) llm_append_combine_kernel(const ApParams 
   for (int e = 0; e < 8; ++e) pk[e] = ap_pack<kFp16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   uint4* dst = reinterpret_cast<uint4*>(
       static_cast<uint16_t*>(p.out) +
-      (static_cast<size_t>(f.row0 + j) * p.H + kv * p.G + r % p.G) * D + dg * 16);
+      (static_cast<size_t>(f.row + j) * p.H + f.kv * p.G + r % p.G) * D + dg * 16);
   dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
   dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
 }

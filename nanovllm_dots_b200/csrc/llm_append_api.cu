@@ -41,7 +41,7 @@ cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t s) {
 
 // ---------------------------------------------------------------- append attention
 struct ApWs {
-  size_t head, units, ubase, start, part_ml, part_o, total;
+  size_t head, units, ubase, start, cuts, part_ml, part_o, total;
 };
 
 int ap_max_units(int tokens, int n, int RT) {
@@ -56,7 +56,8 @@ ApWs ap_ws(int tokens, int n, int G, int D, int ctas) {
   w.units = w.head + 256;
   w.ubase = w.units + up(sizeof(ApUnit) * static_cast<size_t>(ap_max_units(tokens, n, AP_ROWS / G)));
   w.start = w.ubase + up(4 * (static_cast<size_t>(n) + 1));
-  w.part_ml = w.start + up(4 * (static_cast<size_t>(ctas) + 1));
+  w.cuts = w.start + up(4 * (static_cast<size_t>(ctas) + 1));
+  w.part_ml = w.cuts + up(sizeof(ApCut) * static_cast<size_t>(ctas));
   w.part_o = w.part_ml + up(static_cast<size_t>(ctas) * 4 * AP_ROWS * sizeof(float2));
   w.total = w.part_o + static_cast<size_t>(ctas) * 4 * AP_ROWS * D * 4;
   return w;
@@ -107,8 +108,10 @@ cudaError_t launch_append(const CUtensorMap& q, const CUtensorMap& k, const CUte
   auto fn = llm_append_kernel<D, kMod, kFp16>;
   cudaError_t r = smem_attr_once(done, fn, smem);
   if (r != cudaSuccess) return r;
-  r = launch_pdl(llm_append_plan_kernel, dim3(1), dim3(AP_PLAN_THREADS), 0, s, p);
-  if (r != cudaSuccess) return r;
+  if (!p.near_plan) {
+    r = launch_pdl(llm_append_plan_kernel, dim3(1), dim3(AP_PLAN_THREADS), 0, s, p);
+    if (r != cudaSuccess) return r;
+  }
   r = launch_pdl(fn, dim3(p.ctas), dim3(AP_THREADS), smem, s, q, k, v, p);
   if (r != cudaSuccess || p.ctas < 2) return r;
   return launch_pdl(llm_append_combine_kernel<D, kFp16>, dim3(p.ctas - 1, 2 * AP_ROWS * (D / 16) / 256),
@@ -211,6 +214,10 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   const ApWs w = ap_ws(a->tokens, a->n, G, a->head_dim, ctas);
   if (workspace_bytes < w.total) return DFM_ERR_WORKSPACE;
   if (a->tokens == 0) return DFM_OK;
+  // places in the line of key tiles are 32-bit
+  const long long tiles = static_cast<long long>(a->max_blocks) * a->block_size / AP_KT + 2;
+  if (2 * tiles * ap_max_units(a->tokens, a->n, RT) > 0x7fffffffll / a->num_kv_heads - 2 * ctas)
+    return DFM_ERR_UNSUPPORTED;
   int rows = AP_KT;
   while (a->block_size % rows) rows /= 2;
   CUtensorMap mq, mk, mv;
@@ -232,6 +239,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.units = reinterpret_cast<ApUnit*>(ws + w.units);
   p.ubase = reinterpret_cast<int*>(ws + w.ubase);
   p.start = reinterpret_cast<int*>(ws + w.start);
+  p.cuts = reinterpret_cast<ApCut*>(ws + w.cuts);
   p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + w.part_o);
   p.tokens = a->tokens;
@@ -242,6 +250,8 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.RT = RT;
   p.max_units = ap_max_units(a->tokens, a->n, RT);
   p.ctas = ctas;
+  // each CTA plans by itself where that fits its shared memory
+  p.near_plan = !a->first_keys && a->n <= AP_NEAR_SEQS && p.max_units <= AP_NEAR_UNITS;
   p.num_blocks = a->num_blocks;
   p.block_size = a->block_size;
   p.max_blocks = a->max_blocks;
@@ -249,9 +259,16 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.causal = a->causal != 0;
   p.window = a->window;
   const float log2e = 1.4426950408889634f;
-  p.cap_a = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
-  p.cap_in = 2.f * log2e * p.cap_a;
-  p.scale_log2 = (a->softcap > 0.f ? a->softcap : a->scale) * log2e;
+  p.scale_log2 = a->scale * log2e;
+  if (a->softcap > 0.f) {
+    p.cap_a = a->scale / a->softcap;
+    p.cap_b = a->softcap / a->scale;
+    p.cap_in = 2.f * log2e * p.cap_a;
+    const float z = p.cap_a * p.cap_a;
+    p.cap_q[0] = AP_T1 * z;
+    p.cap_q[1] = AP_T2 * z * z;
+    p.cap_q[2] = AP_T3 * z * z * z;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool mod = a->softcap > 0.f || a->slopes, fp16 = a->dtype == DLLM_FP16;
   const cudaError_t r = a->head_dim == 128 ? launch_append<128>(mod, fp16, mq, mk, mv, p, s)
