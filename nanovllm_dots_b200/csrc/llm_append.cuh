@@ -48,6 +48,8 @@ constexpr int AP_RING = 2;          // K tiles and V tiles in shared memory
 constexpr int AP_SOFT_WARPS = 8;
 constexpr int AP_THREADS = 32 * (AP_SOFT_WARPS + 4);
 constexpr int AP_PLAN_THREADS = 1024;
+constexpr int AP_COMBINE_THREADS = 256, AP_COMBINE_BLOCKS = 2;   // blocks to an SM
+constexpr int AP_MAX_CTAS = 256;    // most SMs the shares go to
 constexpr int AP_NEAR_SEQS = 256, AP_NEAR_UNITS = 512;   // what a CTA plans by itself
 constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's key tile counts 2)
 // The running maximum of a row is raised only when a score passes it by this
@@ -77,6 +79,22 @@ struct ApCut {                      // the unit that the end of a share cuts
   int last, pad[3];                 // last share it reaches into; -1: no unit of this share is cut
 };
 
+// n / d for 0 <= n < 2^31: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d), m d
+// is above 2^(31 + s) by less than d <= 2^s, so n m / 2^(31 + s) has n / d's floor.
+struct ApDiv {
+  uint32_t m, s;
+  int d, pad;
+  void set(int by) {
+    d = by;
+    s = 0;
+    while ((1ll << s) < by) ++s;
+    m = static_cast<uint32_t>(((1ull << (31 + s)) + by - 1) / by);
+  }
+  DFM_DEV int operator()(int n) const {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<uint32_t>(n)) * m) >> (31 + s));
+  }
+};
+
 struct ApParams {
   const int* cu;                    // [n + 1]
   const int* ctx;                   // [n]
@@ -97,6 +115,7 @@ struct ApParams {
   int tokens, n, H, KVH, G, RT, max_units, ctas, near_plan;
   int num_blocks, block_size, max_blocks, box_rows;
   int causal, window;
+  ApDiv by_g, by_unit, by_ctas, by_block;   // G, 2 RT, ctas, block_size
   float scale_log2;                 // scale * log2(e)
   // With a cap (cap_a 0: none): cap_a = scale / cap, cap_b its inverse, cap_in =
   // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a.
@@ -177,7 +196,7 @@ DFM_DEV ApUnit ap_unit(const ApParams& p, int seq, int s0, int m, int ctx, int p
 }
 
 DFM_DEV int ap_share(const ApParams& p, int line) {
-  return max(AP_MIN_SHARE, (line * p.KVH + p.ctas - 1) / p.ctas);
+  return max(AP_MIN_SHARE, p.by_ctas(line * p.KVH + p.ctas - 1));
 }
 
 // The plan of a batch small enough for every CTA to make it in its own shared
@@ -187,23 +206,9 @@ struct ApNear {
   int at[AP_NEAR_UNITS];
   uint16_t seq[AP_NEAR_UNITS];
   int2 sums[AP_THREADS / 32];
-  int line, units;
+  int line, units, share;
+  int first, kv, off;   // where this CTA's share starts: unit, kv head, place in the unit
 
-  // The last place of an ascending list with list[place] <= x; a whole warp.
-  static DFM_DEV int last_at_most(const int* list, int n, int x) {
-    const int lane = threadIdx.x & 31;
-    int a = 0;
-    for (int step = 32; step > 0; step = step == 32 ? 1 : 0) {   // blocks of 32, then within one
-      int k = 0;
-      for (int i0 = 0; step == 32 && i0 < n; i0 += 1024) {
-        const int i = i0 + lane * 32;
-        k += __popc(__ballot_sync(0xffffffffu, i < n && list[i] <= x));
-      }
-      if (step == 32) a = (k - 1) * 32;
-      else a += __popc(__ballot_sync(0xffffffffu, a + lane < n && list[a + lane] <= x)) - 1;
-    }
-    return a;
-  }
   DFM_DEV ApUnit unit(const ApParams& p, int u) const {
     const int i = seq[u];
     ApUnit f = ap_unit(p, i, s0[i], m[i], ctx[i], pre[i], (u - ubase[i]) * 2 * p.RT);
@@ -213,12 +218,12 @@ struct ApNear {
   // All AP_THREADS threads.
   DFM_DEV void make(const ApParams& p) {
     const int t = threadIdx.x;
-    int c = 0, cost = 0, s = 0, k = 0, x = 0, pr = 0;
+    int c = 0, cost = 0;
     if (t < p.n) {
+      int s, k;
       const bool rows = ap_rows(p, t, s, k);
-      x = p.ctx[t];
-      if (p.prefix) pr = p.prefix[t];
-      if (rows) c = (k + 2 * p.RT - 1) / (2 * p.RT);
+      const int x = p.ctx[t], pr = p.prefix ? p.prefix[t] : 0;
+      if (rows) c = min(p.by_unit(k + 2 * p.RT - 1), AP_NEAR_UNITS);
       if (blockIdx.x == 0 && !(rows && ap_length(p, k, x))) atomicOr(p.err, DFM_DEV_ERR_LEN);
       if (c > 0) cost = ap_unit(p, t, s, k, x, pr, 0).cost();
       s0[t] = s;
@@ -226,43 +231,72 @@ struct ApNear {
       ctx[t] = x;
       pre[t] = pr;
     }
-    const bool several = __syncthreads_or(c > 1);
+    // units, and above bit 20 the sequences that have some; places if each has one
     int2 all;
-    const int2 before = block_scan<AP_THREADS / 32>(make_int2(c, cost), sums, all);
-    if (t < p.n) ubase[t] = before.x;
-    if (all.x > p.max_units) {   // rows of overlapping sequences
+    const int2 before = block_scan<AP_THREADS / 32>(make_int2(c | (c > 0) << 20, cost), sums, all);
+    const int base = before.x & 0xfffff;
+    int total = all.x & 0xfffff, place = before.y, u = base;
+    const bool several = total != all.x >> 20;
+    if (t < p.n) ubase[t] = base;
+    if (total > p.max_units) {   // rows of overlapping sequences
       if (blockIdx.x == 0 && t == 0) atomicOr(p.err, DFM_DEV_ERR_LEN);
-      all.x = p.max_units;
+      total = p.max_units;
     }
-    if (!several) {              // a unit to a sequence: their places are known
-      if (c > 0 && before.x < all.x) {
-        seq[before.x] = static_cast<uint16_t>(t);
-        at[before.x] = before.y;
+    int of = t;
+    bool mine = c > 0 && u < total;
+    auto settle = [&]() {        // this thread's unit u of sequence `of` has its place
+      if (!mine) return;
+      seq[u] = static_cast<uint16_t>(of);
+      at[u] = place;
+    };
+    auto start = [&]() {         // the share starts in this thread's unit
+      const int sh = ap_share(p, all.y), g = blockIdx.x * sh;
+      if (t == 0) {
+        line = all.y;
+        units = total;
+        share = sh;
       }
+      if (!mine || g >= all.y * p.KVH) return;
+      const int h = g / all.y, o = g - h * all.y - place;
+      if (o < 0 || o >= cost) return;
+      first = u;
+      kv = h;
+      off = o;
+    };
+    if (!several) {              // a unit to a sequence
+      settle();
+      start();
     } else {
       __syncthreads();
       all.y = 0;
-      for (int u0 = 0; u0 < all.x; u0 += AP_THREADS) {
-        const int u = u0 + t;
+#pragma unroll 1
+      for (int u0 = 0; u0 < total; u0 += AP_THREADS) {
+        u = u0 + t;
+        mine = u < total;
         cost = 0;
-        if (u < all.x) {
+        if (mine) {
           int a = 0, b = p.n - 1;   // the last sequence with ubase <= u (one without units shares the next one's)
           while (a < b) {
             const int mid = (a + b + 1) >> 1;
             if (ubase[mid] <= u) a = mid; else b = mid - 1;
           }
-          seq[u] = static_cast<uint16_t>(a);
+          of = a;
           cost = ap_unit(p, a, s0[a], m[a], ctx[a], pre[a], (u - ubase[a]) * 2 * p.RT).cost();
         }
         int2 sum;
-        const int2 place = block_scan<AP_THREADS / 32>(make_int2(cost, 0), sums, sum);
-        if (u < all.x) at[u] = all.y + place.x;
+        place = all.y + block_scan<AP_THREADS / 32>(make_int2(cost, 0), sums, sum).x;
+        settle();
         all.y += sum.x;
       }
-    }
-    if (t == 0) {
-      line = all.y;
-      units = all.x;
+      __syncthreads();
+      for (u = t; u < total; u += AP_THREADS) {
+        mine = true;
+        place = at[u];
+        cost = (u + 1 < total ? at[u + 1] : all.y) - place;
+        start();
+      }
+      mine = false;
+      start();
     }
     __syncthreads();
   }
@@ -287,7 +321,7 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
     if (i < p.n) {
       int s0, m;
       const bool rows = ap_rows(p, i, s0, m);
-      if (rows) c = (m + 2 * p.RT - 1) / (2 * p.RT);
+      if (rows) c = p.by_unit(m + 2 * p.RT - 1);
       if (!(rows && ap_length(p, m, p.ctx[i]))) atomicOr(p.err, DFM_DEV_ERR_LEN);
     }
     int2 total;
@@ -395,16 +429,26 @@ struct ApWalk {
   int u, kv, units;
 
   DFM_DEV ApWalk(const ApParams& p, const ApNear& nr) : near(nr) {
-    line = p.near_plan ? near.line : p.head->line;
-    units = p.near_plan ? near.units : p.head->units;
-    share = p.near_plan ? ap_share(p, line) : p.head->share;
+    if (p.near_plan) {
+      line = near.line;
+      units = near.units;
+      share = near.share;
+    } else {
+      line = p.head->line;
+      units = p.head->units;
+      share = p.head->share;
+    }
     const int all = line * p.KVH, g = blockIdx.x * share;
     left = max(0, min(share, all - g));
-    if (left > 0) {
+    if (left == 0) return;
+    if (p.near_plan) {
+      u = near.first;
+      kv = near.kv;
+      off = near.off;
+    } else {
       kv = g / line;
-      const int r = g - kv * line;
-      u = p.near_plan ? ApNear::last_at_most(near.at, units, r) : p.start[blockIdx.x];
-      off = r - (p.near_plan ? near.at[u] : p.units[u].at);
+      u = p.start[blockIdx.x];
+      off = g - kv * line - p.units[u].at;
     }
   }
   // The next segment with work; false at the end of the share.
@@ -731,7 +775,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       auto block_of = [&](int i) {   // the lane's cache block in tile i, -2 if nobody sees the box
         const int key = (sg.top - i) * AP_KT + box * p.box_rows;
         if (box >= per_tile || i >= sg.i1 || key + p.box_rows <= sg.f.lo || key >= sg.f.hi) return -2;
-        const int b = bt[key / p.block_size];
+        const int b = bt[p.by_block(key)];
         return b < 0 ? -1 : b;
       };
       int blk = block_of(sg.i0);
@@ -751,7 +795,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       for (int i = sg.i0; ok && i < sg.i1; ++i, ++g) {
         const int slot = g % AP_RING;
         const int key = (sg.top - i) * AP_KT + box * p.box_rows;
-        const int row = key % p.block_size;
+        const int row = key - p.by_block(key) * p.block_size;
         const bool mine = blk != -2;
         int cb = blk;
         if (mine && (cb < 0 || cb >= p.num_blocks)) {
@@ -955,7 +999,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     const int r = (warp & 3) * 32 + lane;              // row of the tile, TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + s * AP_KT + lane_off, tO = tmem + 256 + lane_off;
-    const int tok_of = r / p.G, head_of = r % p.G;
+    const int tok_of = p.by_g(r), head_of = r - tok_of * p.G;
     uint8_t* stage = smem + S::OFF_OUT + warp * S::STAGE;
     int g = 0, ns = 0;                                 // V tiles of the CTA, score tiles of the stream
     int no[2] = {0, 0};                                // segments each stream had tiles in
@@ -1227,72 +1271,121 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 }
 
 // ---------------------------------------------------------------- split units
-// Block (b, y): the unit that the end of share b cuts, if it began in share b,
-// items [y * 256, (y + 1) * 256) of its (tile, 16-dim group, row) list.
-// out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the shares, in their order.
+// Joins the units that lie in several shares:
+//   out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the shares j.
+// An item is 8 dims of 32 rows, which lie next to each other in the partials.  A
+// load of another SM's partial takes over a microsecond, so the items of all cuts
+// are spread evenly over one wave of blocks, and where there are few, 2 or 4
+// warps take an item's shares in turn (their sums are added in the warps' order).
 template <int D, bool kFp16>
-__global__ void __launch_bounds__(256) llm_append_combine_kernel(const ApParams p) {
-  constexpr int CB = 4;
+__global__ void __launch_bounds__(AP_COMBINE_THREADS, AP_COMBINE_BLOCKS)
+    llm_append_combine_kernel(const ApParams p) {
+  constexpr int CB = 4, DG = D / 8, WARPS = AP_COMBINE_THREADS / 32;
+  __shared__ float part[WARPS][10][32];
+  __shared__ int2 sums[WARPS];
+  __shared__ ApCut cuts[AP_MAX_CTAS];
+  __shared__ int starts[AP_MAX_CTAS];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x;
-  const ApCut f = p.cuts[b];
-  const int last = f.last;
-  if (last <= b) return;
-  const int task = blockIdx.y * 256 + threadIdx.x;
-  const int r = task % AP_ROWS, rest = task / AP_ROWS;
-  const int dg = rest % (D / 16), tile = rest / (D / 16);
-  if (tile > (f.narrow ? 0 : 1)) return;
-  const int tok = r / p.G, j = tile * p.RT + tok;
-  if (tok >= p.RT || j >= f.ntok) return;
-  float M = -INFINITY, L = 0.f, acc[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-  for (int c0 = b; c0 <= last; c0 += CB) {
-    float2 ml[CB];
-    float4 o[CB][4];
-#pragma unroll
-    for (int x = 0; x < CB; ++x) {
-      const int c = c0 + x;
-      ml[x] = make_float2(-INFINITY, 0.f);
-      if (c > last) continue;
-      const size_t at = (static_cast<size_t>(c) * 2 + (c == b ? 1 : 0)) * 2 + tile;
-      ml[x] = p.part_ml[at * AP_ROWS + r];
-      const float4* src = reinterpret_cast<const float4*>(p.part_o + at * AP_ROWS * D) + dg * 4 * AP_ROWS + r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[x][e] = src[e * AP_ROWS];
-    }
-    float Mn = M;
-#pragma unroll
-    for (int x = 0; x < CB; ++x) Mn = fmaxf(Mn, ml[x].x);
-    const float a = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
-    L *= a;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] *= a;
-#pragma unroll
-    for (int x = 0; x < CB; ++x) {
-      if (c0 + x > last) continue;
-      const float w = ml[x].x == -INFINITY ? 0.f : fast_exp2(ml[x].x - Mn);
-      L += w * ml[x].y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[4 * e] += w * o[x][e].x;
-        acc[4 * e + 1] += w * o[x][e].y;
-        acc[4 * e + 2] += w * o[x][e].z;
-        acc[4 * e + 3] += w * o[x][e].w;
-      }
-    }
-    M = Mn;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  auto row_groups = [&](int tokens) { return (tokens * p.G + 31) >> 5; };
+  int n = 0;
+  if (t < p.ctas) {
+    const ApCut c = p.cuts[t];
+    if (c.last > t) n = (row_groups(min(c.ntok, p.RT)) + row_groups(c.ntok - min(c.ntok, p.RT))) * DG;
+    cuts[t] = c;
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint32_t pk[8];
+  int2 all;
+  const int begin = block_scan<WARPS>(make_int2(n, 0), sums, all).x;
+  if (t < p.ctas) starts[t] = begin;
+  __syncthreads();
+  const int items = all.x;
+  if (items == 0) return;
+  const int room = gridDim.x * WARPS;
+  const int team = items * 4 <= room ? 4 : items * 2 <= room ? 2 : 1;   // warps to an item
+  const int k = warp % team, at_once = WARPS / team;
+  for (int i0 = blockIdx.x * at_once; i0 < items; i0 += gridDim.x * at_once) {
+    const int it = min(i0 + warp / team, items - 1);
+    int b = 0;                  // the last cut that starts at or before the item
+    for (int hi = p.ctas - 1; b < hi;) {
+      const int mid = (b + hi + 1) >> 1;
+      if (starts[mid] <= it) b = mid; else hi = mid - 1;
+    }
+    const ApCut f = cuts[b];
+    const int item = it - starts[b], dg = item % DG, rg = item / DG;
+    const int first = min(f.ntok, p.RT), groups1 = row_groups(first), tile = rg >= groups1;
+    const int r = (tile ? rg - groups1 : rg) * 32 + lane;
+    const bool mine = i0 + warp / team < items && r < (tile ? f.ntok - first : first) * p.G;
+    float M = -INFINITY, L = 0.f, acc[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) pk[e] = ap_pack<kFp16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  uint4* dst = reinterpret_cast<uint4*>(
-      static_cast<uint16_t*>(p.out) +
-      (static_cast<size_t>(f.row + j) * p.H + f.kv * p.G + r % p.G) * D + dg * 16);
-  dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-  dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int c0 = b + k; mine && c0 <= f.last; c0 += CB * team) {
+      float2 ml[CB];
+      float4 o[CB][2];
+#pragma unroll
+      for (int x = 0; x < CB; ++x) {
+        const int c = c0 + x * team;
+        const bool in = c <= f.last;
+        const size_t at = (static_cast<size_t>(c) * 2 + (c > b ? 0 : 1)) * 2 + tile;
+        const float4* src = reinterpret_cast<const float4*>(p.part_o + at * AP_ROWS * D) + dg * 2 * AP_ROWS + r;
+        ml[x] = in ? p.part_ml[at * AP_ROWS + r] : make_float2(-INFINITY, 0.f);
+        o[x][0] = in ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+        o[x][1] = in ? src[AP_ROWS] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float Mn = M;
+#pragma unroll
+      for (int x = 0; x < CB; ++x) Mn = fmaxf(Mn, ml[x].x);
+      const float a = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
+      L *= a;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= a;
+#pragma unroll
+      for (int x = 0; x < CB; ++x) {
+        const float wt = ml[x].x == -INFINITY ? 0.f : fast_exp2(ml[x].x - Mn);
+        L += wt * ml[x].y;
+        acc[0] += wt * o[x][0].x;
+        acc[1] += wt * o[x][0].y;
+        acc[2] += wt * o[x][0].z;
+        acc[3] += wt * o[x][0].w;
+        acc[4] += wt * o[x][1].x;
+        acc[5] += wt * o[x][1].y;
+        acc[6] += wt * o[x][1].z;
+        acc[7] += wt * o[x][1].w;
+      }
+      M = Mn;
+    }
+    if (team > 1) {
+      part[warp][8][lane] = M;
+      part[warp][9][lane] = L;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part[warp][e][lane] = acc[e];
+      __syncthreads();
+      if (k == 0) {
+        float Mn = M;
+        for (int x = 1; x < team; ++x) Mn = fmaxf(Mn, part[warp + x][8][lane]);
+        const float a = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
+        L *= a;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] *= a;
+        for (int x = 1; x < team; ++x) {
+          const float mx = part[warp + x][8][lane];
+          const float wt = mx == -INFINITY ? 0.f : fast_exp2(mx - Mn);
+          L += wt * part[warp + x][9][lane];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += wt * part[warp + x][e][lane];
+        }
+      }
+      __syncthreads();
+    }
+    if (!mine || k != 0) continue;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int tok = p.by_g(r), j = tile * p.RT + tok;
+    *reinterpret_cast<uint4*>(
+        static_cast<uint16_t*>(p.out) +
+        (static_cast<size_t>(f.row + j) * p.H + f.kv * p.G + r - tok * p.G) * D + dg * 8) =
+        make_uint4(ap_pack<kFp16>(acc[0] * inv, acc[1] * inv), ap_pack<kFp16>(acc[2] * inv, acc[3] * inv),
+                   ap_pack<kFp16>(acc[4] * inv, acc[5] * inv), ap_pack<kFp16>(acc[6] * inv, acc[7] * inv));
+  }
 }
 
 }  // namespace dfm

@@ -63,6 +63,9 @@ ApWs ap_ws(int tokens, int n, int G, int D, int ctas) {
   return w;
 }
 
+// CTAs of the append kernel: one to an SM.
+int ap_ctas() { return sm_count() < AP_MAX_CTAS ? sm_count() : AP_MAX_CTAS; }
+
 bool ap_shape_ok(int tokens, int n, int H, int KVH, int D) {
   return tokens >= 0 && n >= 1 && H >= 1 && KVH >= 1 && H % KVH == 0 && H / KVH <= AP_ROWS &&
          (D == 64 || D == 128) && ap_max_units(tokens, n, AP_ROWS / (H / KVH)) > 0;
@@ -114,8 +117,8 @@ cudaError_t launch_append(const CUtensorMap& q, const CUtensorMap& k, const CUte
   }
   r = launch_pdl(fn, dim3(p.ctas), dim3(AP_THREADS), smem, s, q, k, v, p);
   if (r != cudaSuccess || p.ctas < 2) return r;
-  return launch_pdl(llm_append_combine_kernel<D, kFp16>, dim3(p.ctas - 1, 2 * AP_ROWS * (D / 16) / 256),
-                    dim3(256), 0, s, p);
+  return launch_pdl(llm_append_combine_kernel<D, kFp16>, dim3(p.ctas * AP_COMBINE_BLOCKS),
+                    dim3(AP_COMBINE_THREADS), 0, s, p);
 }
 
 template <int D>
@@ -185,7 +188,7 @@ int dllm_rotary(const DllmRotary* a, void* stream) {
 size_t dllm_append_workspace_size(int32_t tokens, int32_t n, int32_t num_heads,
                                   int32_t num_kv_heads, int32_t head_dim) {
   if (!ap_shape_ok(tokens, n, num_heads, num_kv_heads, head_dim)) return 0;
-  return ap_ws(tokens, n, num_heads / num_kv_heads, head_dim, sm_count()).total;
+  return ap_ws(tokens, n, num_heads / num_kv_heads, head_dim, ap_ctas()).total;
 }
 
 int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace_bytes,
@@ -210,7 +213,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
       a->q_token_stride % 8 || a->q_head_stride % 8 || a->q_token_stride < 0 || a->q_head_stride < 0)
     return DFM_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return DFM_ERR_INVALID_ARG;
-  const int G = a->num_heads / a->num_kv_heads, RT = AP_ROWS / G, ctas = sm_count();
+  const int G = a->num_heads / a->num_kv_heads, RT = AP_ROWS / G, ctas = ap_ctas();
   const ApWs w = ap_ws(a->tokens, a->n, G, a->head_dim, ctas);
   if (workspace_bytes < w.total) return DFM_ERR_WORKSPACE;
   if (a->tokens == 0) return DFM_OK;
@@ -256,6 +259,10 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.block_size = a->block_size;
   p.max_blocks = a->max_blocks;
   p.box_rows = rows;
+  p.by_g.set(G);
+  p.by_unit.set(2 * RT);
+  p.by_ctas.set(ctas);
+  p.by_block.set(a->block_size);
   p.causal = a->causal != 0;
   p.window = a->window;
   const float log2e = 1.4426950408889634f;
