@@ -59,14 +59,12 @@ constexpr float AP_TAU = 8.0f;
 // Of AP_EXP_OF pairs of exponentials, AP_EXP_POLY go to the fp32 pipe.
 constexpr int AP_EXP_POLY = 1, AP_EXP_OF = 4;
 
-struct ApUnit {
+struct __align__(16) ApUnit {
   int seq, t0, ntok, row0;          // tokens [t0, t0 + ntok) of the sequence; row0: its first in q
   int lo, hi, fmin, fmax;           // union of the rows' keys; tiles inside [fmin, fmax) have no mask
-  int base, narrow;                 // position of token 0; one row tile only
-  int at, pad;                      // place in the line
+  int base, m, pre, at;             // position of token 0; the sequence's tokens and prefix; place in the line
   DFM_DEV int tiles() const { return hi > lo ? (hi + AP_KT - 1) / AP_KT - lo / AP_KT : 0; }
-  DFM_DEV int weight() const { return narrow ? 1 : 2; }            // of a key tile
-  DFM_DEV int cost() const { return max(1, tiles() * weight()); }  // in the line
+  DFM_DEV int cost(int rt) const { return max(1, tiles() << (ntok > rt)); }   // a wide unit's tile counts 2
 };
 static_assert(sizeof(ApUnit) == 48, "unit record");
 
@@ -110,7 +108,7 @@ struct ApParams {
   int* ubase;                       // [n]
   int* start;                       // [ctas + 1] unit at the start of each share
   ApCut* cuts;                      // [ctas]
-  float* part_o;                    // [ctas][2][2][D / 4][128][4]
+  float* part_o;                    // [ctas][2][2][D / 8][128][8]
   float2* part_ml;                  // [ctas][2][2][128]
   int tokens, n, H, KVH, G, RT, max_units, ctas, near_plan;
   int num_blocks, block_size, max_blocks, box_rows;
@@ -178,7 +176,8 @@ DFM_DEV ApUnit ap_unit(const ApParams& p, int seq, int s0, int m, int ctx, int p
   f.ntok = min(2 * p.RT, m - t0);
   f.row0 = s0;
   f.base = ctx - m;
-  f.narrow = f.ntok <= p.RT;
+  f.m = m;
+  f.pre = pre;
   f.lo = f.hi = f.fmax = 0;
   f.fmin = 0x7fffffff;
   f.at = 0;
@@ -202,58 +201,51 @@ DFM_DEV int ap_share(const ApParams& p, int line) {
 // The plan of a batch small enough for every CTA to make it in its own shared
 // memory: that takes about a microsecond, a kernel of its own three.
 struct ApNear {
-  int s0[AP_NEAR_SEQS], m[AP_NEAR_SEQS], ctx[AP_NEAR_SEQS], pre[AP_NEAR_SEQS], ubase[AP_NEAR_SEQS];
-  int at[AP_NEAR_UNITS];
-  uint16_t seq[AP_NEAR_UNITS];
+  ApUnit units[AP_NEAR_UNITS];
   int2 sums[AP_THREADS / 32];
-  int line, units, share;
+  int line, count, share;
   int first, kv, off;   // where this CTA's share starts: unit, kv head, place in the unit
 
-  DFM_DEV ApUnit unit(const ApParams& p, int u) const {
-    const int i = seq[u];
-    ApUnit f = ap_unit(p, i, s0[i], m[i], ctx[i], pre[i], (u - ubase[i]) * 2 * p.RT);
-    f.at = at[u];
-    return f;
-  }
+  // Scratch of make(), which is over before the memory is used for anything else.
+  struct Seqs {
+    int s0[AP_NEAR_SEQS], m[AP_NEAR_SEQS], ctx[AP_NEAR_SEQS], pre[AP_NEAR_SEQS], ubase[AP_NEAR_SEQS];
+  };
+
   // All AP_THREADS threads.
-  DFM_DEV void make(const ApParams& p) {
+  DFM_DEV void make(const ApParams& p, Seqs& q) {
     const int t = threadIdx.x;
     int c = 0, cost = 0;
+    ApUnit f;
     if (t < p.n) {
       int s, k;
       const bool rows = ap_rows(p, t, s, k);
       const int x = p.ctx[t], pr = p.prefix ? p.prefix[t] : 0;
       if (rows) c = min(p.by_unit(k + 2 * p.RT - 1), AP_NEAR_UNITS);
       if (blockIdx.x == 0 && !(rows && ap_length(p, k, x))) atomicOr(p.err, DFM_DEV_ERR_LEN);
-      if (c > 0) cost = ap_unit(p, t, s, k, x, pr, 0).cost();
-      s0[t] = s;
-      m[t] = k;
-      ctx[t] = x;
-      pre[t] = pr;
+      if (c > 0) {
+        f = ap_unit(p, t, s, k, x, pr, 0);
+        cost = f.cost(p.RT);
+      }
+      q.s0[t] = s;
+      q.m[t] = k;
+      q.ctx[t] = x;
+      q.pre[t] = pr;
     }
     // units, and above bit 20 the sequences that have some; places if each has one
     int2 all;
     const int2 before = block_scan<AP_THREADS / 32>(make_int2(c | (c > 0) << 20, cost), sums, all);
-    const int base = before.x & 0xfffff;
-    int total = all.x & 0xfffff, place = before.y, u = base;
+    int u = before.x & 0xfffff, place = before.y, total = all.x & 0xfffff;
     const bool several = total != all.x >> 20;
-    if (t < p.n) ubase[t] = base;
+    if (t < p.n) q.ubase[t] = u;
     if (total > p.max_units) {   // rows of overlapping sequences
       if (blockIdx.x == 0 && t == 0) atomicOr(p.err, DFM_DEV_ERR_LEN);
       total = p.max_units;
     }
-    int of = t;
-    bool mine = c > 0 && u < total;
-    auto settle = [&]() {        // this thread's unit u of sequence `of` has its place
-      if (!mine) return;
-      seq[u] = static_cast<uint16_t>(of);
-      at[u] = place;
-    };
-    auto start = [&]() {         // the share starts in this thread's unit
+    auto start = [&](bool mine) {   // the share starts in this thread's unit u
       const int sh = ap_share(p, all.y), g = blockIdx.x * sh;
       if (t == 0) {
         line = all.y;
-        units = total;
+        count = total;
         share = sh;
       }
       if (!mine || g >= all.y * p.KVH) return;
@@ -264,40 +256,45 @@ struct ApNear {
       off = o;
     };
     if (!several) {              // a unit to a sequence
-      settle();
-      start();
+      const bool mine = c > 0 && u < total;
+      if (mine) {
+        f.at = place;
+        units[u] = f;
+      }
+      start(mine);
     } else {
       __syncthreads();
       all.y = 0;
 #pragma unroll 1
       for (int u0 = 0; u0 < total; u0 += AP_THREADS) {
         u = u0 + t;
-        mine = u < total;
         cost = 0;
-        if (mine) {
+        if (u < total) {
           int a = 0, b = p.n - 1;   // the last sequence with ubase <= u (one without units shares the next one's)
           while (a < b) {
             const int mid = (a + b + 1) >> 1;
-            if (ubase[mid] <= u) a = mid; else b = mid - 1;
+            if (q.ubase[mid] <= u) a = mid; else b = mid - 1;
           }
-          of = a;
-          cost = ap_unit(p, a, s0[a], m[a], ctx[a], pre[a], (u - ubase[a]) * 2 * p.RT).cost();
+          f = ap_unit(p, a, q.s0[a], q.m[a], q.ctx[a], q.pre[a], (u - q.ubase[a]) * 2 * p.RT);
+          cost = f.cost(p.RT);
         }
         int2 sum;
         place = all.y + block_scan<AP_THREADS / 32>(make_int2(cost, 0), sums, sum).x;
-        settle();
+        if (u < total) {
+          f.at = place;
+          units[u] = f;
+        }
         all.y += sum.x;
       }
       __syncthreads();
       for (u = t; u < total; u += AP_THREADS) {
-        mine = true;
-        place = at[u];
-        cost = (u + 1 < total ? at[u + 1] : all.y) - place;
-        start();
+        place = units[u].at;
+        cost = units[u].cost(p.RT);
+        start(true);
       }
-      mine = false;
-      start();
+      start(false);
     }
+    fence_proxy_async_smem();   // the scratch lies where copies will land
     __syncthreads();
   }
 };
@@ -389,7 +386,7 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
         f.fmin = b.z;
         f.fmax = b.w;
       }
-      cost = f.cost();
+      cost = f.cost(p.RT);
     }
     int2 total;
     const int at = line + block_scan<W>(make_int2(cost, 0), sums, total).x;
@@ -409,7 +406,7 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
   for (int u = t; u < units; u += AP_PLAN_THREADS) {
     const ApUnit f = p.units[u];
     for (int kv = 0; kv < p.KVH; ++kv) {
-      const int a = kv * line + f.at, b = a + f.cost();
+      const int a = kv * line + f.at, b = a + f.cost(p.RT);
       for (int c = (a + share - 1) / share; c * share < b; ++c) p.start[c] = u;
     }
   }
@@ -420,6 +417,7 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
 struct ApSegment {
   ApUnit f;
   int kv, i0, i1, tiles, top;       // tiles of the whole unit; key tile of i = top - i
+  bool narrow;                      // one row tile only
   DFM_DEV bool whole() const { return i0 == 0 && i1 == tiles; }
 };
 
@@ -431,7 +429,7 @@ struct ApWalk {
   DFM_DEV ApWalk(const ApParams& p, const ApNear& nr) : near(nr) {
     if (p.near_plan) {
       line = near.line;
-      units = near.units;
+      units = near.count;
       share = near.share;
     } else {
       line = p.head->line;
@@ -454,9 +452,10 @@ struct ApWalk {
   // The next segment with work; false at the end of the share.
   DFM_DEV bool next(const ApParams& p, ApSegment& s) {
     while (left > 0) {
-      s.f = p.near_plan ? near.unit(p, u) : p.units[u];
+      s.f = p.near_plan ? near.units[u] : p.units[u];
       s.kv = kv;
-      const int wide = 1 - s.f.narrow, cost = s.f.cost();   // a wide unit's tile counts 2
+      s.narrow = s.f.ntok <= p.RT;
+      const int wide = !s.narrow, cost = s.f.cost(p.RT);
       s.tiles = s.f.tiles();
       s.top = (s.f.hi + AP_KT - 1) / AP_KT - 1;
       const int end = min(off + left, cost);
@@ -485,17 +484,16 @@ struct ApSmem {
   static constexpr int BOXES = D / 64;
   static constexpr int TILE = AP_KT * D * 2;              // one K, V or Q tile
   static constexpr int HALF = AP_KT * 128;                // its 64-dim boxes
-  static constexpr int STAGE = 32 * 64;                   // a warp's 32 rows of 32 values
   static constexpr int OFF_Q = 0;                         // [2]
   static constexpr int OFF_K = OFF_Q + 2 * TILE;          // [AP_RING]
   static constexpr int OFF_V = OFF_K + AP_RING * TILE;    // [AP_RING]
-  static constexpr int OFF_OUT = OFF_V + AP_RING * TILE;  // [softmax warps]
-  static constexpr int OFF_ML = OFF_OUT + AP_SOFT_WARPS * STAGE;     // float2 [2 streams][128]
+  static constexpr int OFF_ML = OFF_V + AP_RING * TILE;   // float2 [2 streams][128]
   static constexpr int OFF_NEAR = OFF_ML + 2 * AP_ROWS * 8;
   static constexpr int OFF_BAR = OFF_NEAR + (static_cast<int>(sizeof(ApNear)) + 15) / 16 * 16;
   static constexpr int BYTES = OFF_BAR + 512 + 1024;
 };
 static_assert(ApSmem<128>::BYTES <= 232448, "one CTA per SM");
+static_assert(sizeof(ApNear::Seqs) <= ApSmem<64>::TILE, "the plan's scratch lies on a query tile");
 
 DFM_DEV bool elect_one() {
   uint32_t r;
@@ -595,6 +593,18 @@ DFM_DEV uint32_t ap_zero_times(uint32_t x, uint32_t sum) {
   else
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(sum));
   return r;
+}
+
+DFM_DEV void st_global_v8(void* dst, const uint32_t (&v)[8]) {   // 32-byte aligned
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+DFM_DEV void ld_global_v8(const float* src, float4& a, float4& b) {   // 32-byte aligned
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w), "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w)
+               : "l"(src));
 }
 
 // Two fp32 operations in one instruction.
@@ -757,7 +767,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
   pdl_wait();
-  if (p.near_plan) near.make(p);
+  if (p.near_plan) near.make(p, *reinterpret_cast<ApNear::Seqs*>(sQ));
   ApWalk walk(p, near);
   ApSegment sg;
 
@@ -782,7 +792,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       if (lane == 0) {
         ok = nseg == 0 || ap_wait(q_empty, (nseg - 1) & 1, abort_flag, p.err);
         if (ok) {
-          const int nt = sg.f.narrow ? 1 : 2;
+          const int nt = sg.narrow ? 1 : 2;
           mbar_arrive_expect_tx(q_full, nt * S::BOXES * p.G * p.RT * 128);
           for (int x = 0; x < nt; ++x)
             for (int b = 0; b < S::BOXES; ++b)
@@ -894,7 +904,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (nt == 0) continue;
         ok = __all_sync(0xffffffffu, ap_wait(q_full, nseg & 1, abort_flag, p.err));
         ++nseg;
-        if (sg.f.narrow) {
+        if (sg.narrow) {
           for (int i = 0; i < 2 && i < nt; ++i) {
             k_wait(g + i);
             if (!ok) break;
@@ -961,14 +971,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (!ok) break;
         const int k0 = (sg.top - i) * AP_KT;
         if (k0 < sg.f.fmin || k0 + AP_KT > sg.f.fmax) {
-          // where all rows see the same keys, a special value is all rows' own
-          const bool split = max(k0, sg.f.lo) < sg.f.fmin || min(k0 + AP_KT, sg.f.hi) > sg.f.fmax;
           for (int x = 0; x < 2; ++x) {
             const int r = w * 64 + x * 32 + lane, key = k0 + r;
             uint8_t* row = sV + slot * S::TILE + r * 128;
             const bool seen = key >= sg.f.lo && key < sg.f.hi;
             bool special = false;
-            if (seen && split) {
+            // (where all rows see the key, a special value is all rows' own)
+            if (seen && (key < sg.f.fmin || key >= sg.f.fmax)) {
               // 0 x is NaN for an infinity or a NaN, and stays in the sum
               uint32_t sum = 0;
 #pragma unroll 4
@@ -982,7 +991,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             if (!seen || special) {
 #pragma unroll 4
               for (int c = 0; c < 8 * S::BOXES; ++c)
-                *reinterpret_cast<uint4*>(row + (c >> 3) * S::HALF + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(row + (c >> 3) * S::HALF + (((c & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(0, 0, 0, 0);
             }
             const uint32_t word = __ballot_sync(0xffffffffu, special);
             if (lane == 0) poison[slot * 4 + w * 2 + x] = word;
@@ -1000,38 +1010,43 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + s * AP_KT + lane_off, tO = tmem + 256 + lane_off;
     const int tok_of = p.by_g(r), head_of = r - tok_of * p.G;
-    uint8_t* stage = smem + S::OFF_OUT + warp * S::STAGE;
     int g = 0, ns = 0;                                 // V tiles of the CTA, score tiles of the stream
     int no[2] = {0, 0};                                // segments each stream had tiles in
     bool ok = true;
     ApCut cut;
     cut.last = -1;
-    while (walk.next(p, sg)) {
-      const int nt = sg.i1 - sg.i0;
-      const bool narrow = sg.f.narrow;
-      // this thread's row
-      const int j = sg.f.t0 + (narrow ? 0 : s * p.RT) + tok_of;
-      const bool valid = tok_of < p.RT && j < sg.f.t0 + sg.f.ntok;
-      const bool warp_valid = __any_sync(0xffffffffu, valid);
-      const int pos = sg.f.base + j;
-      int lo = 0, hi = 0;
-      unsigned long long bits = 0;
-      float slope = 0.f;
-      if (valid) {
-        if (p.tree) {
-          const int m = p.ctx[sg.f.seq] - sg.f.base;
-          bits = p.tree[sg.f.row0 + j] & (m >= 64 ? ~0ull : (1ull << m) - 1);
-          hi = sg.f.base;
-        } else {
-          ap_keys(p, sg.f.row0, j, sg.f.base, p.ctx[sg.f.seq], p.prefix ? p.prefix[sg.f.seq] : 0, lo, hi);
-        }
-        // in units of x
-        if (kMod && p.slopes) slope = p.slopes[sg.kv * p.G + head_of] * (1.4426950408889634f / p.scale_log2);
+    // this thread's row of the segment
+    int j, pos, lo, hi, base;
+    bool valid, warp_valid;
+    unsigned long long bits;
+    float slope;
+    auto row = [&]() {
+      j = sg.f.t0 + (sg.narrow ? 0 : s * p.RT) + tok_of;
+      valid = tok_of < p.RT && j < sg.f.t0 + sg.f.ntok;
+      warp_valid = __any_sync(0xffffffffu, valid);
+      base = sg.f.base;
+      pos = base + j;
+      lo = hi = 0;
+      bits = 0;
+      slope = 0.f;
+      if (!valid) return;
+      if (p.tree) {
+        bits = p.tree[sg.f.row0 + j] & (sg.f.m >= 64 ? ~0ull : (1ull << sg.f.m) - 1);
+        hi = base;
+      } else {
+        ap_keys(p, sg.f.row0, j, base, base + sg.f.m, sg.f.pre, lo, hi);
       }
+      if (kMod && p.slopes) slope = p.slopes[sg.kv * p.G + head_of] * (1.4426950408889634f / p.scale_log2);   // in units of x
+    };
+    bool more = walk.next(p, sg);
+    if (more) row();
+    while (more) {
+      const int nt = sg.i1 - sg.i0;
+      const bool narrow = sg.narrow;
       // which of the 32 keys from kc on the row sees
       auto sees = [&](int kc) {
         uint32_t see = low_bits(hi - kc) & ~low_bits(lo - kc);
-        const int o = sg.f.base - kc;   // drafted token 0's bit in this word
+        const int o = base - kc;   // drafted token 0's bit in this word
         if (bits) see |= o >= 32 || o <= -64 ? 0u
                          : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
         return see;
@@ -1172,6 +1187,20 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       }
       // ------------------------------------------------ the segment's rows
       const int n0 = narrow ? (nt + 1) / 2 : nt, n1 = narrow ? nt / 2 : nt;
+      const bool whole = sg.whole();
+      const int slot = blockIdx.x * 2 + (sg.i0 > 0 ? 0 : 1);
+      if (sg.i0 == 0 && !whole) {     // the end of the share cuts this unit
+        cut.row = sg.f.row0 + sg.f.t0;
+        cut.ntok = sg.f.ntok;
+        cut.narrow = sg.narrow;
+        cut.kv = sg.kv;
+        cut.last = (sg.kv * walk.line + sg.f.at + ((sg.tiles - 1) << !sg.narrow)) / walk.share;
+      }
+      const size_t row_off = (static_cast<size_t>(sg.f.row0 + j) * p.H + sg.kv * p.G + head_of) * D;
+      const bool put = valid, warp_put = warp_valid;
+      g += nt;
+      more = walk.next(p, sg);
+      if (more) row();     // its loads run under what follows
       float w0 = 1.f, w1 = 0.f;       // weights of O_0 and O_1 (narrow)
       if (narrow) {
         sML[s * AP_ROWS + r] = make_float2(m, l);
@@ -1190,72 +1219,46 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         ok = __all_sync(0xffffffffu, ap_wait(&o_full[1], no[1] & 1, abort_flag, p.err));
       no[0] += n0 > 0;
       no[1] += n1 > 0;
-      g += nt;
-      if (ok) {
+      if (ok && warp_put) {
         tc_fence_after();
         // columns of this warpgroup: all of its own tile's, or half of the shared one's
         const int c_lo = narrow ? s * (D / 2) : 0, c_hi = narrow ? c_lo + D / 2 : D;
-        const bool whole = sg.whole();
-        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        const int slot = blockIdx.x * 2 + (sg.i0 > 0 ? 0 : 1);
         const int tile = narrow ? 0 : s;
-        float* po = p.part_o + (static_cast<size_t>(slot) * 2 + tile) * AP_ROWS * D;
-        if (!whole && (!narrow || s == 0))
-          p.part_ml[(static_cast<size_t>(slot) * 2 + tile) * AP_ROWS + r] = make_float2(m, l);
-        const long long row_off =
-            valid ? (static_cast<long long>(sg.f.row0 + j) * p.H + sg.kv * p.G + head_of) * D : -1;
-        if (warp_valid) {
+        const size_t part = (static_cast<size_t>(slot) * 2 + tile) * AP_ROWS;
+        float* po = p.part_o + part * D + r * 8;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + row_off;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        w0 *= whole ? inv : 1.f;
+        w1 *= whole ? inv : 1.f;
+        if (!whole && put && (!narrow || s == 0)) p.part_ml[part + r] = make_float2(m, l);
 #pragma unroll 1
-          for (int c = c_lo; c < c_hi; c += 32) {
-            float v[32];
+        for (int c = c_lo; c < c_hi; c += 32) {
+          float v[32], o1[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0.f;
-            if (nt > 0) {
-              ap_load(tO + (narrow ? 0 : s * D) + c, v);
-              ap_landed(v);
+          for (int e = 0; e < 32; ++e) v[e] = o1[e] = 0.f;
+          if (n0 > 0) ap_load(tO + (narrow ? 0 : s * D) + c, v);
+          if (narrow && n1 > 0) ap_load(tO + D + c, o1);
+          ap_landed(v);
+          ap_landed(o1);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], w0, o1[e] * w1);
+          if (!put) continue;
+          // a thread's row, whole 32-byte sectors at a time
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 16) {
+              uint32_t pk[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) pk[x] = ap_pack<kFp16>(v[e + 2 * x], v[e + 2 * x + 1]);
+              st_global_v8(out + c + e, pk);
             }
-            if (narrow && n1 > 0) {
-              float o1[32];
-              ap_load(tO + D + c, o1);
-              ap_landed(o1);
+          } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], w0, o1[e] * w1);
-            }
-            if (!whole) {
-              if (!valid) continue;
-#pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(po + (static_cast<size_t>((c + e) >> 2) * AP_ROWS + r) * 4) =
-                    make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-              continue;
-            }
-            // through shared memory, so that the warp writes whole rows: 32 rows of 64 bytes
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(ap_pack<kFp16>(v[8 * e] * inv, v[8 * e + 1] * inv),
-                             ap_pack<kFp16>(v[8 * e + 2] * inv, v[8 * e + 3] * inv),
-                             ap_pack<kFp16>(v[8 * e + 4] * inv, v[8 * e + 5] * inv),
-                             ap_pack<kFp16>(v[8 * e + 6] * inv, v[8 * e + 7] * inv));
-            __syncwarp();
-#pragma unroll
-            for (int it = 0; it < 4; ++it) {
-              const int rr = it * 8 + (lane >> 2), e = lane & 3;
-              const long long off = __shfl_sync(0xffffffffu, row_off, rr);
-              const uint4 u = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((e ^ ((rr >> 1) & 3)) << 4));
-              if (off >= 0)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + off + c + e * 8) = u;
-            }
-            __syncwarp();
+            for (int e = 0; e < 32; e += 8)
+              st_global_v8(po + static_cast<size_t>((c + e) >> 3) * (AP_ROWS * 8),
+                           reinterpret_cast<const uint32_t(&)[8]>(v[e]));
           }
         }
-      }
-      if (sg.i0 == 0 && !sg.whole()) {     // the end of the share cuts this unit
-        cut.row = sg.f.row0 + sg.f.t0;
-        cut.ntok = sg.f.ntok;
-        cut.narrow = sg.f.narrow;
-        cut.kv = sg.kv;
-        cut.last = (sg.kv * walk.line + sg.f.at + (2 - sg.f.narrow) * (sg.tiles - 1)) / walk.share;
       }
       tc_fence_before();
       if (narrow) ok = ap_meet(1, 32 * AP_SOFT_WARPS, ok);   // both have read O_0 and O_1
@@ -1327,10 +1330,10 @@ __global__ void __launch_bounds__(AP_COMBINE_THREADS, AP_COMBINE_BLOCKS)
         const int c = c0 + x * team;
         const bool in = c <= f.last;
         const size_t at = (static_cast<size_t>(c) * 2 + (c > b ? 0 : 1)) * 2 + tile;
-        const float4* src = reinterpret_cast<const float4*>(p.part_o + at * AP_ROWS * D) + dg * 2 * AP_ROWS + r;
+        const float* src = p.part_o + at * AP_ROWS * D + (dg * AP_ROWS + r) * 8;
         ml[x] = in ? p.part_ml[at * AP_ROWS + r] : make_float2(-INFINITY, 0.f);
-        o[x][0] = in ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
-        o[x][1] = in ? src[AP_ROWS] : make_float4(0.f, 0.f, 0.f, 0.f);
+        o[x][0] = o[x][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in) ld_global_v8(src, o[x][0], o[x][1]);
       }
       float Mn = M;
 #pragma unroll

@@ -209,7 +209,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
     return DFM_ERR_INVALID_ARG;
   if (a->tree_masks && (a->prefix_lens || a->first_keys || a->slopes || a->window))
     return DFM_ERR_UNSUPPORTED;
-  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out) ||
+  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || reinterpret_cast<uintptr_t>(a->out) % 32 ||
       a->q_token_stride % 8 || a->q_head_stride % 8 || a->q_token_stride < 0 || a->q_head_stride < 0)
     return DFM_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return DFM_ERR_INVALID_ARG;
