@@ -12,6 +12,8 @@ import ctypes
 import os
 from ctypes import POINTER, c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
+import torch
+
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libdfm.so")
 
@@ -262,6 +264,19 @@ def check(rc: int, what: str) -> None:
     if rc != DFM_OK:
         msg = lib().dfm_error_string(rc).decode()
         raise RuntimeError(f"{what} failed: {msg} (code {rc})")
+
+
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of CUDA device ``index``."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def call_on(index: int, fn, *args) -> int:
+    """``fn(*args)`` with CUDA device ``index`` current, as it is on nearly every call."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
 
 
 def ptr(t) -> int | None:

@@ -12,8 +12,6 @@ trees of drafted tokens.  ``install_append_attention`` routes a reference
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -85,70 +83,79 @@ class B200AppendAttention:
             raise RuntimeError("unsupported append-attention shape")
         self.workspace = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
         self.workspace[:256].zero_()
-        self._last = torch.cuda.current_stream(self.device)   # of the zero-fill
+        self._index = self.device.index
+        self._dtype = _DTYPES[dtype]
+        self._call, self._workspace = self.L.dllm_append_attention, self.workspace.data_ptr()
+        self._stream = _lib.raw_stream(self._index)   # the last one used: that of the zero-fill
 
-    def _int(self, name, t, dtype, shape):
-        if t.dtype != dtype or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+    def _ints(self, name, t, dtype, shape):
+        if t.dtype is not dtype or t.get_device() != self._index or t.shape != shape or not t.is_contiguous():
             raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on "
                                f"{self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         return t.data_ptr()
 
     def _run(self, q, k_cache, v_cache, cu, ctx, table, prefix, first, tree, out, stream):
-        H, D, dev = self.num_heads, self.head_dim, self.device
-        if q.dim() != 3 or q.shape[1] != H or q.shape[2] != D or q.dtype != self.dtype or q.device != dev:
-            raise RuntimeError(f"q: expected a {self.dtype} tensor [tokens, {H}, {D}] on {dev}, "
+        H, D, index, dtype = self.num_heads, self.head_dim, self._index, self.dtype
+        if q.dim() != 3 or q.shape[1] != H or q.shape[2] != D or q.dtype is not dtype or q.get_device() != index:
+            raise RuntimeError(f"q: expected a {dtype} tensor [tokens, {H}, {D}] on {self.device}, "
                                f"got {q.dtype} {tuple(q.shape)} on {q.device}")
-        T, n = q.shape[0], ctx.shape[0]
+        T, n = q.shape[0], ctx.shape[0] if ctx.dim() else 0
         if T > self.max_tokens or not 1 <= n <= self.max_seqs:
             raise RuntimeError(f"append of {T} tokens of {n} sequences "
                                f"(at most {self.max_tokens} of {self.max_seqs})")
         st, sh, sd = q.stride()
         if sd != 1 or st % 8 or sh % 8 or q.data_ptr() % 16:
             raise RuntimeError("q: expected contiguous head dims and 16-byte aligned heads")
-        geometry = (self.block_size, self.num_kv_heads, D)
+        geometry = (k_cache.shape[0], self.block_size, self.num_kv_heads, D)
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if c.dtype != self.dtype or c.device != dev or c.shape[1:] != geometry or \
-                    c.shape[0] != k_cache.shape[0] or c.shape[0] < 1 or not c.is_contiguous():
-                raise RuntimeError(f"{name}: expected a contiguous {self.dtype} tensor [num_blocks, "
-                                   f"{', '.join(map(str, geometry))}] on {dev}")
+            if c.dtype is not dtype or c.get_device() != index or c.shape != geometry or \
+                    geometry[0] < 1 or not c.is_contiguous():
+                raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor [num_blocks, "
+                                   f"{', '.join(map(str, geometry[1:]))}] on {self.device}, both caches alike")
         if table.dim() != 2 or not 1 <= table.shape[1] <= self.max_blocks:
             raise RuntimeError(f"block_tables: expected [{n}, 1..{self.max_blocks}]")
-        s = stream if stream is not None else torch.cuda.current_stream(dev)
         if out is None:
             if stream is None:
-                out = torch.empty((T, H, D), dtype=self.dtype, device=dev)
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
             else:     # owned by the stream that writes it
-                with torch.cuda.stream(s):
-                    out = torch.empty((T, H, D), dtype=self.dtype, device=dev)
-        elif out.dtype != self.dtype or out.device != dev or tuple(out.shape) != (T, H, D) or \
+                with torch.cuda.stream(stream):
+                    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.dtype is not dtype or out.get_device() != index or out.shape != (T, H, D) or \
                 not out.is_contiguous():
-            raise RuntimeError(f"out: expected a contiguous {self.dtype} tensor {(T, H, D)} on {dev}")
-        i32 = torch.int32
+            raise RuntimeError(f"out: expected a contiguous {dtype} tensor {(T, H, D)} on {self.device}")
+        i32, width = torch.int32, table.shape[1]
+        plain = tree is None
         a = _lib.DllmAppend(
-            _DTYPES[self.dtype], T, n, H, self.num_kv_heads, D, k_cache.shape[0], self.block_size,
-            table.shape[1], self.causal, self.window if tree is None else 0, self.scale, self.softcap,
-            q.data_ptr(), st, sh, k_cache.data_ptr(), v_cache.data_ptr(),
-            self._int("cu_seqlens_q", cu, i32, (n + 1,)), self._int("context_lens", ctx, i32, (n,)),
-            self._int("block_tables", table, i32, (n, table.shape[1])),
-            None if prefix is None else self._int("prefix_lens", prefix, i32, (n,)),
-            None if first is None else self._int("first_keys", first, i32, (T,)),
-            None if tree is None else self._int("tree_masks", tree, torch.int64, (T,)),
-            None if tree is not None or self.slopes is None else self.slopes.data_ptr(),
-            out.data_ptr())
+            self._dtype, T, n, H, self.num_kv_heads, D, geometry[0], self.block_size, width, self.causal,
+            self.window if plain else 0, self.scale, self.softcap, q.data_ptr(), st, sh,
+            k_cache.data_ptr(), v_cache.data_ptr(), self._ints("cu_seqlens_q", cu, i32, (n + 1,)),
+            self._ints("context_lens", ctx, i32, (n,)), self._ints("block_tables", table, i32, (n, width)),
+            None if prefix is None else self._ints("prefix_lens", prefix, i32, (n,)),
+            None if first is None else self._ints("first_keys", first, i32, (T,)),
+            None if plain else self._ints("tree_masks", tree, torch.int64, (T,)),
+            self.slopes.data_ptr() if plain and self.slopes is not None else None, out.data_ptr())
         if T == 0:
             return out
-        if s != self._last and not torch.cuda.is_current_stream_capturing():
-            s.wait_stream(self._last)      # the workspace may still be in use there
-            self._last = s
-        if torch.cuda.current_device() == dev.index:
-            rc = self.L.dllm_append_attention(a, self.workspace.data_ptr(), self.ws_bytes,
-                                              ctypes.c_void_p(s.cuda_stream))
-        else:
-            with torch.cuda.device(dev):
-                rc = self.L.dllm_append_attention(a, self.workspace.data_ptr(), self.ws_bytes,
-                                                  ctypes.c_void_p(s.cuda_stream))
-        _lib.check(rc, "dllm_append_attention")
+        handle = _lib.raw_stream(index) if stream is None else stream.cuda_stream
+        if handle != self._stream:
+            self._follow(handle)
+        rc = _lib.call_on(index, self._call, a, self._workspace, self.ws_bytes, handle)
+        if rc:
+            _lib.check(rc, "dllm_append_attention")
         return out
+
+    def _follow(self, handle: int) -> None:
+        """The workspace may still be in use on the stream of the last call.  (A
+        capture cannot wait for one outside it.)"""
+        def stream(h):
+            return torch.cuda.ExternalStream(h, device=self.device) if h else \
+                torch.cuda.default_stream(self.device)
+
+        with torch.cuda.stream(stream(handle)):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        stream(handle).wait_stream(stream(self._stream))
+        self._stream = handle
 
     def append(self, q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, *,
                prefix_lens: torch.Tensor | None = None, first_keys: torch.Tensor | None = None,
@@ -178,7 +185,8 @@ class B200AppendAttention:
         """Synchronise and raise if a kernel reported a device-side error."""
         v = _lib.c_uint32(0)
         s = torch.cuda.current_stream(self.device)
-        s.wait_stream(self._last)
+        if s.cuda_stream != self._stream:
+            self._follow(s.cuda_stream)
         with torch.cuda.device(self.device):
             _lib.check(self.L.dllm_read_error(_lib.ptr(self.workspace), _lib.c_void_p(s.cuda_stream), v),
                        "dllm_read_error")

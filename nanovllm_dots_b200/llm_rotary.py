@@ -9,7 +9,6 @@ for contexts longer than the trained one.  There is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass
 
@@ -125,68 +124,88 @@ class B200Rotary:
         self.L = _lib.lib()
         self.turns = _turns(inv).to(self.device)
         self.err = torch.zeros(64, dtype=torch.int32, device=self.device)
+        self._index, self._inter, self._call = self.device.index, layout == "interleaved", self.L.dllm_rotary
+        self._turns, self._err = self.turns.data_ptr(), self.err.data_ptr()
 
-    def _check(self, name, t, dtype, shape):
-        if t.dtype != dtype or t.device != self.device or tuple(t.shape) != shape:
-            raise RuntimeError(f"{name}: expected a {dtype} tensor of shape {shape} on {self.device}, "
-                               f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-
-    def _heads(self, name, t, dtype=None, tokens=None):
-        if t.dim() != 3 or t.shape[2] != self.head_dim or t.device != self.device:
+    def _heads(self, name, t, dtype, tokens):
+        """[tokens, heads, head_dim] with contiguous head dims -> its heads and strides."""
+        if t.dim() != 3 or t.shape[2] != self.head_dim or t.get_device() != self._index:
             raise RuntimeError(f"{name}: expected [tokens, heads, {self.head_dim}] on {self.device}, "
                                f"got {tuple(t.shape)} on {t.device}")
-        if t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
-            raise RuntimeError(f"{name}: unsupported or mixed type {t.dtype}")
-        if tokens is not None and t.shape[0] != tokens:
-            raise RuntimeError(f"{name}: expected {tokens} tokens, got {t.shape[0]}")
-        if t.stride(2) != 1:
+        if t.dtype is not dtype:
+            raise RuntimeError(f"{name}: expected {dtype}, got {t.dtype}")
+        n, heads, _ = t.shape
+        if n != tokens:
+            raise RuntimeError(f"{name}: expected {tokens} tokens, got {n}")
+        ts, hs, one = t.stride()
+        if one != 1:
             raise RuntimeError(f"{name}: expected contiguous head dims")
+        return heads, ts, hs
 
-    def _args(self, q, positions, out):
-        self._heads("q", q)
-        if positions.dtype != torch.int32 or positions.device != self.device or \
-                positions.shape != (q.shape[0],) or not positions.is_contiguous():
-            raise RuntimeError(f"positions: expected a contiguous int32 [{q.shape[0]}] on {self.device}")
-        self._heads("out", out, q.dtype, q.shape[0])
-        if out.shape != q.shape:
-            raise RuntimeError(f"out: expected shape {tuple(q.shape)}")
-        qs, os = q.stride(), out.stride()
-        same = out.data_ptr() == q.data_ptr()
-        if same and qs[:2] != os[:2]:
-            raise RuntimeError("out: rotating in place needs q's own strides")
-        if not same and _overlap(q, out):
-            raise RuntimeError("out: overlaps q without being q")
-        if q.shape[0] > 1 and os[0] == 0 or q.shape[1] > 1 and os[1] == 0:
-            raise RuntimeError("out: rows share memory")
-        a = _lib.DllmRotary(dtype=_DTYPES[q.dtype], tokens=q.shape[0], q_heads=q.shape[1],
-                            head_dim=self.head_dim, rot_dim=self.rot_dim,
-                            interleaved=self.layout == "interleaved", factor=self.factor,
-                            turns=self.turns.data_ptr(), positions=positions.data_ptr(),
-                            q=q.data_ptr(), q_out=out.data_ptr(), q_token_stride=qs[0],
-                            q_head_stride=qs[1], out_token_stride=os[0], out_head_stride=os[1],
-                            err_word=self.err.data_ptr())
-        return a
+    def _ints(self, name, t, tokens):
+        if t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (tokens,) or \
+                not t.is_contiguous():
+            raise RuntimeError(f"{name}: expected a contiguous int32 [{tokens}] on {self.device}")
+        return t.data_ptr()
 
-    def _launch(self, a, stream):
-        s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(self.L.dllm_rotary(a, ctypes.c_void_p(s.cuda_stream)), "dllm_rotary")
-
-    def _out(self, q, out, stream):
-        if out is not None:
+    def _run(self, q, positions, out, stream, store):
+        dtype = _DTYPES.get(q.dtype)
+        if dtype is None:
+            raise RuntimeError(f"q: unsupported type {q.dtype}")
+        T = q.shape[0]
+        heads, qt, qh = self._heads("q", q, q.dtype, T)
+        pos = self._ints("positions", positions, T)
+        if out is None:
+            if stream is None:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            else:       # owned by the stream that writes it
+                with torch.cuda.stream(stream):
+                    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            ot, oh = heads * self.head_dim, self.head_dim
+        else:
+            oheads, ot, oh = self._heads("out", out, q.dtype, T)
+            if oheads != heads:
+                raise RuntimeError(f"out: expected shape {tuple(q.shape)}")
+            if out.data_ptr() == q.data_ptr():
+                if (qt, qh) != (ot, oh):
+                    raise RuntimeError("out: rotating in place needs q's own strides")
+            elif _overlap(q, out):
+                raise RuntimeError("out: overlaps q without being q")
+            if not _apart(out):
+                raise RuntimeError("out: rows share memory")
+        kvh, kt, kh, vt, vh, slots, places = 0, 0, 0, 0, 0, 0, None
+        kp = vp = kcp = vcp = None
+        if store is not None:
+            k, v, slot_mapping, k_cache, v_cache = store
+            kvh, kt, kh = self._heads("k", k, q.dtype, T)
+            vheads, vt, vh = self._heads("v", v, q.dtype, T)
+            if kvh != vheads or kvh < 1:
+                raise RuntimeError("k and v have different heads, or none")
+            places = self._ints("slot_mapping", slot_mapping, T)
+            shape = k_cache.shape
+            for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+                if c.dtype is not q.dtype or c.get_device() != self._index or c.dim() != 4 or \
+                        c.shape != shape or shape[2] != kvh or shape[3] != self.head_dim or \
+                        not c.is_contiguous() or not c.numel():
+                    raise RuntimeError(f"{name}: expected a contiguous {q.dtype} [num_blocks, block_size, "
+                                       f"{kvh}, {self.head_dim}] on {self.device}, and both caches alike")
+            slots = shape[0] * shape[1]
+            kp, vp, kcp, vcp = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+        if T == 0 or heads == 0 and store is None:
             return out
-        # owned by the stream that writes it
-        with torch.cuda.stream(stream):
-            return torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        a = _lib.DllmRotary(dtype, T, heads, kvh, self.head_dim, self.rot_dim, self._inter, self.factor,
+                            self._turns, pos, q.data_ptr(), out.data_ptr(), kp, vp, kcp, vcp, places,
+                            qt, qh, ot, oh, kt, kh, vt, vh, slots, self._err)
+        handle = _lib.raw_stream(self._index) if stream is None else stream.cuda_stream
+        rc = _lib.call_on(self._index, self._call, a, handle)
+        if rc:
+            _lib.check(rc, "dllm_rotary")
+        return out
 
     def rotate(self, q, positions, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """q [tokens, heads, head_dim] (any token and head strides) at int32
         positions [tokens] -> out (``out=q`` rotates in place)."""
-        out = self._out(q, out, stream)
-        if q.numel() == 0:
-            return out
-        self._launch(self._args(q, positions, out), stream)
-        return out
+        return self._run(q, positions, out, stream, None)
 
     def rotate_store(self, q, k, v, positions, slot_mapping, k_cache, v_cache,
                      out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
@@ -196,35 +215,7 @@ class B200Rotary:
         block_size + offset; -1 stores nothing).  Two tokens must not share a
         slot.  A slot past the cache is not stored and reported by
         ``check_errors``."""
-        T = q.shape[0]
-        self._heads("k", k, q.dtype, T)
-        self._heads("v", v, q.dtype, T)
-        kvh = k.shape[1]
-        if v.shape[1] != kvh or kvh < 1:
-            raise RuntimeError("k and v have different heads")
-        if slot_mapping.dtype != torch.int32 or slot_mapping.device != self.device or \
-                slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
-            raise RuntimeError(f"slot_mapping: expected a contiguous int32 [{T}] on {self.device}")
-        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if c.dtype != q.dtype or c.device != self.device or c.dim() != 4 or not c.is_contiguous() \
-                    or c.shape[2:] != (kvh, self.head_dim) or c.shape != k_cache.shape or not c.numel():
-                raise RuntimeError(f"{name}: expected a contiguous {q.dtype} [num_blocks, block_size, "
-                                   f"{kvh}, {self.head_dim}] on {self.device}")
-        out = self._out(q, out, stream)
-        if T == 0:
-            return out
-        if q.shape[1] < 1:
-            raise RuntimeError("q has no heads")
-        a = self._args(q, positions, out)
-        a.kv_heads = kvh
-        a.k, a.v = k.data_ptr(), v.data_ptr()
-        a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-        a.slot_mapping = slot_mapping.data_ptr()
-        (a.k_token_stride, a.k_head_stride), (a.v_token_stride, a.v_head_stride) = \
-            k.stride()[:2], v.stride()[:2]
-        a.num_slots = k_cache.shape[0] * k_cache.shape[1]
-        self._launch(a, stream)
-        return out
+        return self._run(q, positions, out, stream, (k, v, slot_mapping, k_cache, v_cache))
 
     def check_errors(self) -> None:
         """Synchronise and raise if a slot past the cache was met."""
@@ -245,5 +236,20 @@ def _span(t):
 
 
 def _overlap(a, b) -> bool:
+    if not a.numel() or not b.numel():
+        return False
     (a0, a1), (b0, b1) = _span(a), _span(b)
     return a0 < b1 and b0 < a1
+
+
+def _apart(t) -> bool:
+    """Whether no two elements of [tokens, heads, dims] share memory."""
+    if not t.numel():
+        return True
+    room = t.shape[2]
+    for n, stride in sorted(((t.shape[0], t.stride(0)), (t.shape[1], t.stride(1))), key=lambda x: x[1]):
+        if n > 1:
+            if stride < room:
+                return False
+            room = (n - 1) * stride + room
+    return True
