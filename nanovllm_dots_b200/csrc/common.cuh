@@ -435,6 +435,22 @@ DFM_DEV uint32_t pack_bf16(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// n / d for 0 <= n < 2^31: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d), m d
+// is above 2^(31 + s) by less than d <= 2^s, so n m / 2^(31 + s) has n / d's floor.
+struct FastDiv {
+  uint32_t m, s;
+  int d, pad;
+  void set(int by) {
+    d = by;
+    s = 0;
+    while ((1ll << s) < by) ++s;
+    m = static_cast<uint32_t>(((1ull << (31 + s)) + by - 1) / by);
+  }
+  DFM_DEV int operator()(int n) const {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<uint32_t>(n)) * m) >> (31 + s));
+  }
+};
+
 // Output-row map f(r) = (r / a) * b + c + (r % a): scatters a compact GEMM
 // result into the 34-row per-request slot layout (identity: a huge, b=0, c=0).
 struct RowMap {

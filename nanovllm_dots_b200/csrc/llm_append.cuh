@@ -77,22 +77,6 @@ struct ApCut {                      // the unit that the end of a share cuts
   int last, pad[3];                 // last share it reaches into; -1: no unit of this share is cut
 };
 
-// n / d for 0 <= n < 2^31: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d), m d
-// is above 2^(31 + s) by less than d <= 2^s, so n m / 2^(31 + s) has n / d's floor.
-struct ApDiv {
-  uint32_t m, s;
-  int d, pad;
-  void set(int by) {
-    d = by;
-    s = 0;
-    while ((1ll << s) < by) ++s;
-    m = static_cast<uint32_t>(((1ull << (31 + s)) + by - 1) / by);
-  }
-  DFM_DEV int operator()(int n) const {
-    return static_cast<int>((static_cast<unsigned long long>(static_cast<uint32_t>(n)) * m) >> (31 + s));
-  }
-};
-
 struct ApParams {
   const int* cu;                    // [n + 1]
   const int* ctx;                   // [n]
@@ -113,7 +97,7 @@ struct ApParams {
   int tokens, n, H, KVH, G, RT, max_units, ctas, near_plan;
   int num_blocks, block_size, max_blocks, box_rows;
   int causal, window;
-  ApDiv by_g, by_unit, by_ctas, by_block;   // G, 2 RT, ctas, block_size
+  FastDiv by_g, by_unit, by_ctas, by_block;   // G, 2 RT, ctas, block_size
   float scale_log2;                 // scale * log2(e)
   // With a cap (cap_a 0: none): cap_a = scale / cap, cap_b its inverse, cap_in =
   // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a.
@@ -1084,9 +1068,15 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             if (kMod && p.slopes && behind) shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
-              ld(xa, c);
               const uint32_t see = full ? ~0u : sees(k0 + c * 32);
               const bool masked = __any_sync(0xffffffffu, see != ~0u);
+              if (masked && !__any_sync(0xffffffffu, see != 0)) {   // nobody's
+#pragma unroll
+                for (int e = 0; e < 32; ++e) xa[e] = -INFINITY;
+                tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(xa));
+                continue;
+              }
+              ld(xa, c);
               ap_landed(xa);
               if constexpr (kMod) {
                 if (p.cap_a > 0.f) ap_cap(xa, p);

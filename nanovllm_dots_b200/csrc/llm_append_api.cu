@@ -10,7 +10,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 // ---------------------------------------------------------------- rotary
 template <typename T, bool INTER>
-cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t s) {
+cudaError_t launch_rotary(RotaryParams& p, cudaStream_t s) {
   constexpr int VP = 16 / sizeof(T);
   const long long heads = p.heads + (p.slots ? 2 * p.kv_heads : 0);
   auto strides_ok = [](std::initializer_list<long long> v) {
@@ -18,7 +18,7 @@ cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t s) {
       if (x % VP) return false;
     return true;
   };
-  bool vec = p.D % (2 * VP) == 0 && (p.rot / 2) % VP == 0 && aligned16(p.q) && aligned16(p.q_out) &&
+  bool vec = p.D % (2 * VP) == 0 && (p.rot / 2) % VP == 0 && p.rot / 2 <= RO_MAX_PAIRS && aligned16(p.q) && aligned16(p.q_out) &&
              strides_ok({p.q_ts, p.q_hs, p.o_ts, p.o_hs});
   if (p.slots)
     vec = vec && aligned16(p.k) && aligned16(p.v) && aligned16(p.k_cache) && aligned16(p.v_cache) &&
@@ -30,13 +30,15 @@ cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t s) {
     return launch_pdl(llm_rotary_scalar_kernel<T, INTER>, dim3(static_cast<unsigned>(nb)),
                       dim3(RO_THREADS), 0, s, p);
   }
-  // a thread's angles serve 4 heads once there are threads enough to fill the GPU without
-  const long long lanes = p.D / (2 * VP), one = p.tokens * heads * lanes;
-  const bool four = one > 4ll * sm_count() * 2048;
-  const long long nb = blocks(four ? p.tokens * ((heads + 3) / 4) * lanes : one);
-  if (nb > 0x7fffffffll) return cudaErrorInvalidValue;
-  return launch_pdl(four ? llm_rotary_kernel<T, INTER, 4> : llm_rotary_kernel<T, INTER, 1>,
-                    dim3(static_cast<unsigned>(nb)), dim3(RO_THREADS), 0, s, p);
+  // four tokens to a block where that still leaves every SM a few blocks
+  const long long lanes = p.D / (2 * VP);
+  const int tb = p.tokens >= 16 * sm_count() ? 4 : 1;
+  if (heads * lanes * tb > 0x7fffffffll) return cudaErrorInvalidValue;
+  p.by_token.set(static_cast<int>(heads * lanes));
+  p.by_lanes.set(static_cast<int>(lanes));
+  p.by_pairs.set(p.rot / 2);
+  return launch_pdl(tb == 4 ? llm_rotary_kernel<T, INTER, 4> : llm_rotary_kernel<T, INTER, 1>,
+                    dim3(static_cast<unsigned>((p.tokens + tb - 1) / tb)), dim3(RO_THREADS), 0, s, p);
 }
 
 // ---------------------------------------------------------------- append attention

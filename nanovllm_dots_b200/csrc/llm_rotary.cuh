@@ -36,6 +36,7 @@ struct RotaryParams {
   int tokens, heads, kv_heads, D, rot;
   float factor;
   bool copy_tail;                    // q_out is not q: its unrotated dims are written too
+  FastDiv by_token, by_lanes, by_pairs;   // items of a token, lanes of a head, pairs of a head
 };
 
 DFM_DEV void rotary_sincos(unsigned long long w, int pos, float f, float& c, float& s) {
@@ -131,66 +132,76 @@ __global__ void __launch_bounds__(RO_THREADS) llm_rotary_scalar_kernel(RotaryPar
   for (int d = 2 * e; d < 2 * e + 2 && d < p.D; ++d) r.dst[d] = r.src[d];
 }
 
-// Whole 16-byte vectors: VP pairs a thread, over HG heads of one token.  A
-// token takes D / (2 VP) lanes; lane l turns pairs [l VP, (l + 1) VP) or, past
-// the rotated dims, copies two vectors.  All HG heads' loads are issued before
-// the first result is written.
-template <typename T, bool INTER, int HG>
-__global__ void __launch_bounds__(RO_THREADS) llm_rotary_kernel(RotaryParams p) {
+// Whole 16-byte vectors.  A block takes TB tokens: its threads first compute the
+// tokens' cosines and sines, one pair each, into shared memory (threads that
+// compute those of their own vectors: 33 us instead of 27 at the size below), then
+// turn items of VP pairs of a head: lane l of D / (2 VP) has pairs [l VP, (l + 1) VP)
+// or, past the rotated dims, copies two vectors.  A thread's first item is loaded
+// before the angles are computed.  Bound by HBM and the latency of a block's
+// three dependent loads: 16384 tokens of 12 + 2 + 2 heads of 128 (134 MB) in 27.2 us,
+// 4.9 TB/s.  Two items a thread need 64 registers instead of 40: 30.4 us.
+constexpr int RO_MAX_PAIRS = 256;    // of a head in the table
+
+template <typename T, bool INTER, int TB>
+__global__ void __launch_bounds__(RO_THREADS, 6) llm_rotary_kernel(RotaryParams p) {
   constexpr int VP = 16 / sizeof(T);
+  __shared__ float2 table[TB][RO_MAX_PAIRS];
   pdl_trigger();
   pdl_wait();
-  const int lanes = p.D / (2 * VP), heads = p.heads + (p.slots ? 2 * p.kv_heads : 0);
-  const int groups = (heads + HG - 1) / HG;
-  const long long idx = static_cast<long long>(blockIdx.x) * RO_THREADS + threadIdx.x;
-  if (idx >= static_cast<long long>(p.tokens) * groups * lanes) return;
-  const int l = static_cast<int>(idx % lanes);
-  const long long tg = idx / lanes;
-  const int h0 = static_cast<int>(tg % groups) * HG, t = static_cast<int>(tg / groups);
-  const int half = p.rot / 2;
-  const bool turning = l * VP < half;
-  // the two vectors of this lane, in elements of the head: rotated pairs, and
-  // the copy of a head that is not rotated (or of dims past rot_dim)
-  const int ta = INTER ? 2 * l * VP : l * VP, tb = INTER ? ta + VP : ta + half;
-  const int ca = 2 * l * VP, cb = ca + VP;
-  const int slot = h0 + HG > p.heads ? rotary_slot(p, t, l == 0) : 0;
-  uint4 va[HG], vb[HG];
-#pragma unroll
-  for (int j = 0; j < HG; ++j) {
-    if (h0 + j >= heads) continue;
-    const RotaryHead<T> r = rotary_head<T>(p, t, h0 + j, slot);
-    const bool turn = r.turn && turning;
-    if (!r.dst || !(turn || r.tail)) continue;
-    va[j] = *reinterpret_cast<const uint4*>(r.src + (turn ? ta : ca));
-    vb[j] = *reinterpret_cast<const uint4*>(r.src + (turn ? tb : cb));
+  const int half = p.rot / 2, heads = p.heads + (p.slots ? 2 * p.kv_heads : 0);
+  const int lanes = p.D / (2 * VP), per_token = heads * lanes;
+  const int t0 = blockIdx.x * TB, tokens = min(TB, p.tokens - t0), items = tokens * per_token;
+  RotaryHead<T> r;
+  int t, a, b, l;        // token of the block, the two vectors' elements, the lane
+  bool on, turn;
+  uint4 va, vb;
+  auto load = [&](int item) {
+    on = item < items;
+    if (!on) return;
+    t = TB > 1 ? p.by_token(item) : 0;
+    const int rest = item - t * per_token, h = p.by_lanes(rest);
+    l = rest - h * lanes;
+    r = rotary_head<T>(p, t0 + t, h, h >= p.heads ? rotary_slot(p, t0 + t, l == 0) : 0);
+    turn = r.turn && l * VP < half;
+    on = r.dst && (turn || r.tail);
+    if (!on) return;
+    a = turn && !INTER ? l * VP : 2 * l * VP;
+    b = turn && !INTER ? a + half : a + VP;
+    va = *reinterpret_cast<const uint4*>(r.src + a);
+    vb = *reinterpret_cast<const uint4*>(r.src + b);
+  };
+  load(threadIdx.x);
+  for (int i = threadIdx.x; i < tokens * half; i += RO_THREADS) {
+    const int tok = TB > 1 ? p.by_pairs(i) : 0, e = i - tok * half;
+    float c, s;
+    rotary_sincos(p.turns[e], p.positions[t0 + tok], p.factor, c, s);
+    table[tok][e] = make_float2(c, s);
   }
-  float c[VP], s[VP];
-  if (turning && h0 < p.heads + p.kv_heads) {
-    const int pos = p.positions[t];
-#pragma unroll
-    for (int i = 0; i < VP; ++i) rotary_sincos(p.turns[l * VP + i], pos, p.factor, c[i], s[i]);
-  }
-#pragma unroll
-  for (int j = 0; j < HG; ++j) {
-    if (h0 + j >= heads) continue;
-    const RotaryHead<T> r = rotary_head<T>(p, t, h0 + j, slot);
-    const bool turn = r.turn && turning;
-    if (!r.dst || !(turn || r.tail)) continue;
+  __syncthreads();
+  for (int item = threadIdx.x; item < items; item += RO_THREADS) {
+    if (item >= RO_THREADS) load(item);
+    if (!on) continue;
     if (turn) {
-      T* a = reinterpret_cast<T*>(&va[j]);
-      T* b = reinterpret_cast<T*>(&vb[j]);
+      T* x = reinterpret_cast<T*>(&va);
+      T* y = reinterpret_cast<T*>(&vb);
+      const float4* cs = reinterpret_cast<const float4*>(&table[t][l * VP]);
 #pragma unroll
-      for (int i = 0; i < VP; ++i) {
-        // half layout: pair i is (a[i], b[i]); interleaved: elements 2i and 2i + 1 of a|b
-        T* xp = INTER ? (2 * i < VP ? a + 2 * i : b + 2 * i - VP) : a + i;
-        T* yp = INTER ? xp + 1 : b + i;
-        const float x = ro_load(*xp), y = ro_load(*yp);
-        *xp = ro_store<T>(x * c[i] - y * s[i]);
-        *yp = ro_store<T>(y * c[i] + x * s[i]);
+      for (int i = 0; i < VP; i += 2) {
+        const float4 c = cs[i / 2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          // half layout: pair n is (x[n], y[n]); interleaved: elements 2n and 2n + 1 of x|y
+          const int n = i + k;
+          T* xp = INTER ? (2 * n < VP ? x + 2 * n : y + 2 * n - VP) : x + n;
+          T* yp = INTER ? xp + 1 : y + n;
+          const float u = ro_load(*xp), w = ro_load(*yp), co = k ? c.z : c.x, si = k ? c.w : c.y;
+          *xp = ro_store<T>(u * co - w * si);
+          *yp = ro_store<T>(w * co + u * si);
+        }
       }
     }
-    *reinterpret_cast<uint4*>(r.dst + (turn ? ta : ca)) = va[j];
-    *reinterpret_cast<uint4*>(r.dst + (turn ? tb : cb)) = vb[j];
+    *reinterpret_cast<uint4*>(r.dst + a) = va;
+    *reinterpret_cast<uint4*>(r.dst + b) = vb;
   }
 }
 
