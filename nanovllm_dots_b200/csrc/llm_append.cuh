@@ -1102,6 +1102,15 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               top = ap_max32(xa, top);
               if (kMod || masked) tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(xa));
             }
+            if (!full) {
+              // special values of V that this row sees, noted until the product takes V
+              const int slot = (g + i) % AP_RING;
+              ok = __all_sync(0xffffffffu, ap_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
+              if (!ok) break;
+              uint32_t bad = 0;
+              for (int c = 0; c < 4; ++c) bad |= poison[slot * 4 + c] & sees(k0 + c * 32);
+              if (bad) l = __int_as_float(0x7fffffff);
+            }
             tmem_wait_st();
           }
           const float mt = fmaf(top, p.scale_log2, shift);
@@ -1162,14 +1171,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           float a, b;
           f2_split(f2_add(sum0, sum1), a, b);
           l += a + b;
-          if (!full) {   // special values of V that this row sees
-            const int slot = (g + i) % AP_RING;
-            ok = __all_sync(0xffffffffu, ap_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
-            if (!ok) break;
-            uint32_t bad = 0;
-            for (int c = 0; c < 4; ++c) bad |= poison[slot * 4 + c] & sees(k0 + c * 32);
-            if (bad) l = __int_as_float(0x7fffffff);
-          }
         } else if (lane == 0) {   // nobody reads this warp's rows
           mbar_arrive(&p_full[2 * s]);
           mbar_arrive(&p_full[2 * s + 1]);
