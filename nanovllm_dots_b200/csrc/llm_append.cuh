@@ -653,27 +653,56 @@ DFM_DEV void ap_exp2_pair(uint64_t x, float& a, float& b) {
 // of which an SM does 16 a clock, so that they and the softmax's exponential would
 // take three times the products' time.
 constexpr float AP_T0 = 0.999999464f, AP_T1 = -0.33326377f, AP_T2 = 0.131909163f, AP_T3 = -0.0444185946f;
-DFM_DEV void ap_cap(float (&x)[32], const ApParams& p) {
-  float big = 0.f;
+DFM_DEV void ap_cap(float (&xa)[32], float (&xb)[32], const ApParams& p) {
+  float big = 0.f, big1 = 0.f;
 #pragma unroll
-  for (int e = 0; e < 32; ++e) big = fmaxf(big, fabsf(x[e]));
+  for (int e = 0; e < 32; ++e) {
+    big = fmaxf(big, fabsf(xa[e]));
+    big1 = fmaxf(big1, fabsf(xb[e]));
+  }
   // (a NaN is not above the bound and stays one in the polynomial)
-  if (__any_sync(0xffffffffu, big * p.cap_a > 0.5f)) {
+  if (__any_sync(0xffffffffu, fmaxf(big, big1) * p.cap_a > 0.5f)) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
-      const float r = __fdividef(1.f, 1.f + fast_exp2(x[e] * p.cap_in));
-      x[e] = fmaf(-2.f * p.cap_b, r, p.cap_b);
+      const float ra = __fdividef(1.f, 1.f + fast_exp2(xa[e] * p.cap_in));
+      const float rb = __fdividef(1.f, 1.f + fast_exp2(xb[e] * p.cap_in));
+      xa[e] = fmaf(-2.f * p.cap_b, ra, p.cap_b);
+      xb[e] = fmaf(-2.f * p.cap_b, rb, p.cap_b);
     }
     return;
   }
+  const uint64_t q3 = f2(p.cap_q[2], p.cap_q[2]), q2 = f2(p.cap_q[1], p.cap_q[1]), q1 = f2(p.cap_q[0], p.cap_q[0]),
+                 q0 = f2(AP_T0, AP_T0);
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
-    const uint64_t y = f2(x[e], x[e + 1]), z = f2_mul(y, y);
-    uint64_t q = f2_fma(f2(p.cap_q[2], p.cap_q[2]), z, f2(p.cap_q[1], p.cap_q[1]));
-    q = f2_fma(q, z, f2(p.cap_q[0], p.cap_q[0]));
-    q = f2_fma(q, z, f2(AP_T0, AP_T0));
-    f2_split(f2_mul(y, q), x[e], x[e + 1]);
+    const uint64_t ya = f2(xa[e], xa[e + 1]), yb = f2(xb[e], xb[e + 1]);
+    const uint64_t za = f2_mul(ya, ya), zb = f2_mul(yb, yb);
+    const uint64_t ua = f2_fma(f2_fma(f2_fma(q3, za, q2), za, q1), za, q0);
+    const uint64_t ub = f2_fma(f2_fma(f2_fma(q3, zb, q2), zb, q1), zb, q0);
+    f2_split(f2_mul(ya, ua), xa[e], xa[e + 1]);
+    f2_split(f2_mul(yb, ub), xb[e], xb[e + 1]);
   }
+}
+
+// x += slope (c + e): with the row's shift, the distance bias of keys c + e.
+DFM_DEV void ap_slope(float (&x)[32], float slope, int c) {
+  const float at = slope * static_cast<float>(c);
+  const uint64_t sl = f2(slope, slope), base = f2(at, at);
+#pragma unroll
+  for (int e = 0; e < 32; e += 2)
+    f2_split(f2_fma(sl, f2(e, e + 1), f2_add(base, f2(x[e], x[e + 1]))), x[e], x[e + 1]);
+}
+// x -= slope |d - e|
+DFM_DEV void ap_slope_abs(float (&x)[32], float slope, int d) {
+  const float d0 = static_cast<float>(d);
+#pragma unroll
+  for (int e = 0; e < 32; ++e) x[e] = fmaf(-slope, fabsf(d0 - static_cast<float>(e)), x[e]);
+}
+// -inf where the row does not see the key
+DFM_DEV void ap_mask(float (&x)[32], uint32_t see) {
+  if (__all_sync(0xffffffffu, see == ~0u)) return;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) x[e] = (see >> e) & 1 ? x[e] : -INFINITY;
 }
 
 DFM_DEV float ap_max32(const float (&x)[32], float top) {
@@ -1067,40 +1096,41 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             const bool behind = k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix);
             if (kMod && p.slopes && behind) shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t see = full ? ~0u : sees(k0 + c * 32);
-              const bool masked = __any_sync(0xffffffffu, see != ~0u);
-              if (masked && !__any_sync(0xffffffffu, see != 0)) {   // nobody's
+            for (int c = 0; c < 128; c += 64) {
+              const uint32_t sa = full ? ~0u : sees(k0 + c), sb = full ? ~0u : sees(k0 + c + 32);
+              const bool masked = __any_sync(0xffffffffu, (sa & sb) != ~0u);
+              if (masked && !__any_sync(0xffffffffu, (sa | sb) != 0)) {   // nobody's
 #pragma unroll
                 for (int e = 0; e < 32; ++e) xa[e] = -INFINITY;
-                tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(xa));
+                tmem_st32(tS + c, reinterpret_cast<uint32_t(&)[32]>(xa));
+                tmem_st32(tS + c + 32, reinterpret_cast<uint32_t(&)[32]>(xa));
                 continue;
               }
-              ld(xa, c);
+              ap_load(tS + c, xa);
+              ap_load(tS + c + 32, xb);
               ap_landed(xa);
+              ap_landed(xb);
               if constexpr (kMod) {
-                if (p.cap_a > 0.f) ap_cap(xa, p);
+                if (p.cap_a > 0.f) ap_cap(xa, xb, p);
                 if (p.slopes) {
-                  const float c0 = static_cast<float>(c * 32);
                   if (behind) {   // every key the row sees is at or before it: |p - k| = (p - k0) - c
-                    const uint64_t sl = f2(slope, slope), base = f2(c0, c0);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                      f2_split(f2_fma(sl, f2_add(base, f2(e, e + 1)), f2(xa[e], xa[e + 1])), xa[e], xa[e + 1]);
+                    ap_slope(xa, slope, c);
+                    ap_slope(xb, slope, c + 32);
                   } else {
-                    const float d0 = static_cast<float>(pos - k0) - c0;
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                      xa[e] = fmaf(-slope, fabsf(d0 - static_cast<float>(e)), xa[e]);
+                    ap_slope_abs(xa, slope, pos - k0 - c);
+                    ap_slope_abs(xb, slope, pos - k0 - c - 32);
                   }
                 }
               }
               if (masked) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) xa[e] = (see >> e) & 1 ? xa[e] : -INFINITY;
+                ap_mask(xa, sa);
+                ap_mask(xb, sb);
               }
-              top = ap_max32(xa, top);
-              if (kMod || masked) tmem_st32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(xa));
+              top = ap_max32(xb, ap_max32(xa, top));
+              if (kMod || masked) {
+                tmem_st32(tS + c, reinterpret_cast<uint32_t(&)[32]>(xa));
+                tmem_st32(tS + c + 32, reinterpret_cast<uint32_t(&)[32]>(xb));
+              }
             }
             if (!full) {
               // special values of V that this row sees, noted until the product takes V
