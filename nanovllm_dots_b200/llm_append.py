@@ -193,3 +193,31 @@ class B200AppendAttention:
         if v.value:
             names = [nm for bit, nm in _lib.DEVERR_BITS.items() if v.value & bit]
             raise RuntimeError(f"append attention device error: {', '.join(names)} (0x{v.value:x})")
+
+
+def install_append_attention(module, get_context, att: B200AppendAttention, store_kvcache) -> None:
+    """Route a reference ``Attention`` module's prefill over the paged cache through ``att``.
+
+    ``get_context`` and ``store_kvcache`` are the reference's own
+    (``nanovllm_dots.utils.context.get_context``, ``layers/attention.py:33-47``),
+    passed in so that this package does not import the reference.  When the
+    context is a prefill with block tables (``attention.py:66-86``) the module's
+    forward stores this call's k and v at ``slot_mapping`` and becomes
+    ``att.append`` over ``cu_seqlens_q`` and the lengths in ``cu_seqlens_k``;
+    every other call keeps the forward that was there, so that
+    ``install_decode_attention`` may come before or after."""
+    original = module.forward
+
+    def forward(q, k, v):
+        ctx = get_context()
+        if not getattr(module, "is_causal", True) or not ctx.is_prefill or ctx.block_tables is None \
+                or not module.k_cache.numel():
+            return original(q, k, v)
+        store_kvcache(k.view(-1, module.num_kv_heads, module.head_dim),
+                      v.view(-1, module.num_kv_heads, module.head_dim), module.k_cache, module.v_cache,
+                      ctx.slot_mapping)
+        lens = ctx.cu_seqlens_k[1:] - ctx.cu_seqlens_k[:-1]
+        return att.append(q.view(-1, module.num_heads, module.head_dim), module.k_cache, module.v_cache,
+                          ctx.cu_seqlens_q, lens, ctx.block_tables)
+
+    module.forward = forward

@@ -190,3 +190,33 @@ def test_oracle_rotary_turns_pairs():
             torch.full((3, 1), 2.0, dtype=torch.float64), pos.double()[:, None] * 0.25)
         assert torch.allclose(y[..., a], z.real) and torch.allclose(y[..., b], z.imag)
         assert torch.equal(y[..., 4:], x[..., 4:].double())
+
+
+def test_install_routes_prefill_over_the_paged_cache():
+    """Prefill with block tables stores and appends; every other call keeps the module's forward."""
+    from types import SimpleNamespace as NS
+
+    from nanovllm_dots_b200.llm_append import install_append_attention
+    calls = []
+    module = NS(num_heads=4, num_kv_heads=2, head_dim=64, is_causal=True, k_cache=torch.zeros(2, 16, 2, 64),
+                v_cache=torch.zeros(2, 16, 2, 64), forward=lambda q, k, v: calls.append("own") or "own")
+    att = NS(append=lambda *a: calls.append(a) or "append")
+    ctx = NS(is_prefill=True, block_tables=torch.zeros(2, 1, dtype=torch.int32),
+             cu_seqlens_q=torch.tensor([0, 3, 5], dtype=torch.int32),
+             cu_seqlens_k=torch.tensor([0, 10, 12], dtype=torch.int32), slot_mapping=torch.arange(5))
+    stored = []
+    install_append_attention(module, lambda: ctx, att, lambda *a: stored.append(a))
+    q, k = torch.zeros(5, 4 * 64), torch.ones(5, 2 * 64)
+    assert module.forward(q, k, k) == "append"
+    a = calls.pop()
+    assert a[0].shape == (5, 4, 64) and a[1] is module.k_cache and a[2] is module.v_cache
+    assert a[3] is ctx.cu_seqlens_q and a[4].tolist() == [10, 2] and a[4].dtype == torch.int32
+    assert a[5] is ctx.block_tables
+    assert stored[0][0].shape == (5, 2, 64) and stored[0][4] is ctx.slot_mapping
+    for change in (dict(is_prefill=False), dict(block_tables=None)):
+        kept = dict(vars(ctx))
+        vars(ctx).update(change)
+        assert module.forward(q, k, k) == "own"
+        vars(ctx).update(kept)
+    module.is_causal = False
+    assert module.forward(q, k, k) == "own" and len(stored) == 1
