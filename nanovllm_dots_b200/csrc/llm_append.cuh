@@ -14,10 +14,10 @@
 // read once for all of them and single tokens, trees and prompts take the same
 // path.  A unit is up to two row tiles of a sequence; its keys are taken in
 // tiles of 128, newest first (the tiles with masks first, and with a distance
-// bias the largest scores first).  The units of every kv head form one line of
-// key tiles, cut into equal shares for the persistent CTAs: a unit whose keys
-// fall into several shares leaves unnormalised partials that
-// llm_append_combine_kernel adds up in the order of the shares.
+// bias the largest scores first).  The units of every kv head, each a fixed cost
+// and its key tiles, form one line that is cut into equal shares for the
+// persistent CTAs: a unit whose keys fall into several shares leaves unnormalised
+// partials that llm_append_combine_kernel adds up in the order of the shares.
 //
 // One CTA per SM, 12 warps: two softmax warpgroups (a thread is a row), a TMA
 // warp, an MMA warp and two warps that look after V.  Each softmax warpgroup
@@ -51,6 +51,12 @@ constexpr int AP_PLAN_THREADS = 1024;
 constexpr int AP_COMBINE_THREADS = 256, AP_COMBINE_BLOCKS = 2;   // blocks to an SM
 constexpr int AP_MAX_CTAS = 256;    // most SMs the shares go to
 constexpr int AP_NEAR_SEQS = 256, AP_NEAR_UNITS = 512;   // what a CTA plans by itself
+// What a unit costs besides its tiles (its first loads, the masked tiles, its rows'
+// way out: 4000 to 8000 clocks), in half tiles of a wide unit (1800 clocks).  With
+// shares of equal tiles alone, CTAs with many short units ended last: a chunked
+// prefill of 24 sequences took 62.0 us and now 49.1, 64 single tokens 30.4 and 28.7,
+// 64 small trees 30.1 and 28.3; 2 / 4 and 3 / 4 are equal, 1 / 3 and 3 / 6 slower.
+constexpr int AP_NARROW_COST = 3, AP_WIDE_COST = 4;
 constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's key tile counts 2)
 // The running maximum of a row is raised only when a score passes it by this
 // much (log2 units): probabilities then reach 2^8, exact in fp32 and within
@@ -64,7 +70,8 @@ struct __align__(16) ApUnit {
   int lo, hi, fmin, fmax;           // union of the rows' keys; tiles inside [fmin, fmax) have no mask
   int base, m, pre, at;             // position of token 0; the sequence's tokens and prefix; place in the line
   DFM_DEV int tiles() const { return hi > lo ? (hi + AP_KT - 1) / AP_KT - lo / AP_KT : 0; }
-  DFM_DEV int cost(int rt) const { return max(1, tiles() << (ntok > rt)); }   // a wide unit's tile counts 2
+  DFM_DEV int lead(int rt) const { return ntok > rt ? AP_WIDE_COST : AP_NARROW_COST; }
+  DFM_DEV int cost(int rt) const { return lead(rt) + (tiles() << (ntok > rt)); }   // a wide unit's tile counts 2
 };
 static_assert(sizeof(ApUnit) == 48, "unit record");
 
@@ -439,12 +446,12 @@ struct ApWalk {
       s.f = p.near_plan ? near.units[u] : p.units[u];
       s.kv = kv;
       s.narrow = s.f.ntok <= p.RT;
-      const int wide = !s.narrow, cost = s.f.cost(p.RT);
+      const int wide = !s.narrow, lead = s.f.lead(p.RT), cost = s.f.cost(p.RT);
       s.tiles = s.f.tiles();
       s.top = (s.f.hi + AP_KT - 1) / AP_KT - 1;
       const int end = min(off + left, cost);
-      s.i0 = (off + wide) >> wide;
-      s.i1 = min(s.tiles, (end + wide) >> wide);
+      s.i0 = (max(0, off - lead) + wide) >> wide;
+      s.i1 = min(s.tiles, (max(0, end - lead) + wide) >> wide);
       const bool zero = s.tiles == 0 && off == 0;
       left -= end - off;
       off = end;
@@ -1215,7 +1222,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         cut.ntok = sg.f.ntok;
         cut.narrow = sg.narrow;
         cut.kv = sg.kv;
-        cut.last = (sg.kv * walk.line + sg.f.at + ((sg.tiles - 1) << !sg.narrow)) / walk.share;
+        cut.last = (sg.kv * walk.line + sg.f.at + sg.f.lead(p.RT) + ((sg.tiles - 1) << !sg.narrow)) / walk.share;
       }
       const size_t row_off = (static_cast<size_t>(sg.f.row0 + j) * p.H + sg.kv * p.G + head_of) * D;
       const bool put = valid, warp_put = warp_valid;

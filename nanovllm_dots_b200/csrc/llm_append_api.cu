@@ -220,7 +220,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   if (workspace_bytes < w.total) return DFM_ERR_WORKSPACE;
   if (a->tokens == 0) return DFM_OK;
   // places in the line of key tiles are 32-bit
-  const long long tiles = static_cast<long long>(a->max_blocks) * a->block_size / AP_KT + 2;
+  const long long tiles = static_cast<long long>(a->max_blocks) * a->block_size / AP_KT + 2 + AP_WIDE_COST;
   if (2 * tiles * ap_max_units(a->tokens, a->n, RT) > 0x7fffffffll / a->num_kv_heads - 2 * ctas)
     return DFM_ERR_UNSUPPORTED;
   int rows = AP_KT;
