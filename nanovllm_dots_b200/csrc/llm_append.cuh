@@ -691,13 +691,11 @@ DFM_DEV void ap_cap(float (&xa)[32], float (&xb)[32], const ApParams& p) {
   }
 }
 
-// x += slope (c + e): with the row's shift, the distance bias of keys c + e.
-DFM_DEV void ap_slope(float (&x)[32], float slope, int c) {
-  const float at = slope * static_cast<float>(c);
-  const uint64_t sl = f2(slope, slope), base = f2(at, at);
+// x += slope e, one instruction a score (e is an immediate): with the row's and the
+// chunk's shifts, the distance bias.
+DFM_DEV void ap_slope(float (&x)[32], float slope) {
 #pragma unroll
-  for (int e = 0; e < 32; e += 2)
-    f2_split(f2_fma(sl, f2(e, e + 1), f2_add(base, f2(x[e], x[e + 1]))), x[e], x[e + 1]);
+  for (int e = 0; e < 32; ++e) x[e] = fmaf(slope, static_cast<float>(e), x[e]);
 }
 // x -= slope |d - e|
 DFM_DEV void ap_slope_abs(float (&x)[32], float slope, int d) {
@@ -723,12 +721,14 @@ DFM_DEV float ap_max32(const float (&x)[32], float top) {
 }
 
 // ---------------------------------------------------------------- the kernel
-// kMod: a cap or a distance bias on the scores.
-template <int D, bool kMod, bool kFp16>
+// A cap and a distance bias on the scores have kernels of their own: what only they
+// need costs the others registers.
+template <int D, bool kCap, bool kBias, bool kFp16>
 __global__ void __launch_bounds__(AP_THREADS, 1)
     llm_append_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ApParams p) {
   using S = ApSmem<D>;
+  constexpr bool kMod = kCap || kBias;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -1050,13 +1050,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       bits = 0;
       slope = 0.f;
       if (!valid) return;
-      if (p.tree) {
+      if (!kBias && p.tree) {   // (trees have no distance bias)
         bits = p.tree[sg.f.row0 + j] & (sg.f.m >= 64 ? ~0ull : (1ull << sg.f.m) - 1);
         hi = base;
       } else {
         ap_keys(p, sg.f.row0, j, base, base + sg.f.m, sg.f.pre, lo, hi);
       }
-      if (kMod && p.slopes) slope = p.slopes[sg.kv * p.G + head_of] * (1.4426950408889634f / p.scale_log2);   // in units of x
+      if (kBias) slope = p.slopes[sg.kv * p.G + head_of] * (1.4426950408889634f / p.scale_log2);   // in units of x
     };
     bool more = walk.next(p, sg);
     if (more) row();
@@ -1067,7 +1067,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       auto sees = [&](int kc) {
         uint32_t see = low_bits(hi - kc) & ~low_bits(lo - kc);
         const int o = base - kc;   // drafted token 0's bit in this word
-        if (bits) see |= o >= 32 || o <= -64 ? 0u
+        if (!kBias && bits) see |= o >= 32 || o <= -64 ? 0u
                          : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
         return see;
       };
@@ -1085,7 +1085,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           // code stays small: the maximum (with a cap, a bias or masks, the
           // changed scores x go back to TMEM), then the probabilities.
           // x scale + shift is the score in log2 units.
-          float shift = 0.f, top = -INFINITY;
+          // (and chunk c's 32 keys are c grow further on).
+          float shift = 0.f, grow = 0.f, top = -INFINITY;
           float xa[32], xb[32];
           auto ld = [&](float (&x)[32], int c) { ap_load(tS + c * 32, x); };
           if (!kMod && full) {
@@ -1101,7 +1102,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
           } else {
             const bool behind = k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix);
-            if (kMod && p.slopes && behind) shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
+            if (kBias && behind) {
+              shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
+              grow = 32.f * slope;
+            }
 #pragma unroll 1
             for (int c = 0; c < 128; c += 64) {
               const uint32_t sa = full ? ~0u : sees(k0 + c), sb = full ? ~0u : sees(k0 + c + 32);
@@ -1117,23 +1121,27 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               ap_load(tS + c + 32, xb);
               ap_landed(xa);
               ap_landed(xb);
-              if constexpr (kMod) {
-                if (p.cap_a > 0.f) ap_cap(xa, xb, p);
-                if (p.slopes) {
-                  if (behind) {   // every key the row sees is at or before it: |p - k| = (p - k0) - c
-                    ap_slope(xa, slope, c);
-                    ap_slope(xb, slope, c + 32);
-                  } else {
-                    ap_slope_abs(xa, slope, pos - k0 - c);
-                    ap_slope_abs(xb, slope, pos - k0 - c - 32);
-                  }
+              if constexpr (kCap) ap_cap(xa, xb, p);
+              if constexpr (kBias) {
+                if (behind) {   // every key the row sees is at or before it: |p - k| = (p - k0) - c
+                  ap_slope(xa, slope);
+                  ap_slope(xb, slope);
+                } else {
+                  ap_slope_abs(xa, slope, pos - k0 - c);
+                  ap_slope_abs(xb, slope, pos - k0 - c - 32);
                 }
               }
               if (masked) {
                 ap_mask(xa, sa);
                 ap_mask(xb, sb);
               }
-              top = ap_max32(xb, ap_max32(xa, top));
+              if constexpr (kBias) {
+                const float c32 = static_cast<float>(c >> 5);
+                top = fmaxf(top, fmaf(grow, c32, ap_max32(xa, -INFINITY)));
+                top = fmaxf(top, fmaf(grow, c32 + 1.f, ap_max32(xb, -INFINITY)));
+              } else {
+                top = ap_max32(xb, ap_max32(xa, top));
+              }
               if (kMod || masked) {
                 tmem_st32(tS + c, reinterpret_cast<uint32_t(&)[32]>(xa));
                 tmem_st32(tS + c + 32, reinterpret_cast<uint32_t(&)[32]>(xb));
@@ -1169,10 +1177,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
           }
           const float ms = shift - (m == -INFINITY ? 0.f : m);
-          const uint64_t sc = f2(p.scale_log2, p.scale_log2), sh = f2(ms, ms);
+          const uint64_t sc = f2(p.scale_log2, p.scale_log2);
+          grow *= p.scale_log2;
           uint64_t sum0 = f2(0.f, 0.f), sum1 = f2(0.f, 0.f);
           uint32_t pk[32];
-          auto probabilities = [&](const float (&x)[32], int at) {
+          auto probabilities = [&](const float (&x)[32], int at, int c) {
+            const float mc = kBias ? fmaf(grow, static_cast<float>(c), ms) : ms;
+            const uint64_t sh = f2(mc, mc);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               float a, b;
@@ -1195,10 +1206,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           for (int h = 0; h < 2; ++h) {
             ap_landed(xa);
             ld(xb, 2 * h + 1);
-            probabilities(xa, 0);
+            probabilities(xa, 0, 2 * h);
             ap_landed(xb);
             if (h == 0) ld(xa, 2);
-            probabilities(xb, 16);
+            probabilities(xb, 16, 2 * h + 1);
             tmem_st32(tS + h * 32, pk);
             tmem_wait_st();
             tc_fence_before();

@@ -105,12 +105,12 @@ bool map_ap_q(CUtensorMap* m, const DllmAppend& a, int G, int RT) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool kMod, bool kFp16>
+template <int D, bool kCap, bool kBias, bool kFp16>
 cudaError_t launch_append(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                           const ApParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   constexpr int smem = ApSmem<D>::BYTES;
-  auto fn = llm_append_kernel<D, kMod, kFp16>;
+  auto fn = llm_append_kernel<D, kCap, kBias, kFp16>;
   cudaError_t r = smem_attr_once(done, fn, smem);
   if (r != cudaSuccess) return r;
   if (!p.near_plan) {
@@ -123,12 +123,14 @@ cudaError_t launch_append(const CUtensorMap& q, const CUtensorMap& k, const CUte
                     dim3(AP_COMBINE_THREADS), 0, s, p);
 }
 
-template <int D>
-cudaError_t launch_append(bool mod, bool fp16, const CUtensorMap& q, const CUtensorMap& k,
+template <int D, bool kFp16>
+cudaError_t launch_append(bool cap, bool bias, const CUtensorMap& q, const CUtensorMap& k,
                           const CUtensorMap& v, const ApParams& p, cudaStream_t s) {
-  if (mod)
-    return fp16 ? launch_append<D, true, true>(q, k, v, p, s) : launch_append<D, true, false>(q, k, v, p, s);
-  return fp16 ? launch_append<D, false, true>(q, k, v, p, s) : launch_append<D, false, false>(q, k, v, p, s);
+  if (cap)
+    return bias ? launch_append<D, true, true, kFp16>(q, k, v, p, s)
+                : launch_append<D, true, false, kFp16>(q, k, v, p, s);
+  return bias ? launch_append<D, false, true, kFp16>(q, k, v, p, s)
+              : launch_append<D, false, false, kFp16>(q, k, v, p, s);
 }
 
 }  // namespace
@@ -279,9 +281,13 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
     p.cap_q[2] = AP_T3 * z * z * z;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool mod = a->softcap > 0.f || a->slopes, fp16 = a->dtype == DLLM_FP16;
-  const cudaError_t r = a->head_dim == 128 ? launch_append<128>(mod, fp16, mq, mk, mv, p, s)
-                                           : launch_append<64>(mod, fp16, mq, mk, mv, p, s);
+  const bool cap = a->softcap > 0.f, bias = a->slopes != nullptr, fp16 = a->dtype == DLLM_FP16;
+  const cudaError_t r =
+      a->head_dim == 128
+          ? (fp16 ? launch_append<128, true>(cap, bias, mq, mk, mv, p, s)
+                  : launch_append<128, false>(cap, bias, mq, mk, mv, p, s))
+          : (fp16 ? launch_append<64, true>(cap, bias, mq, mk, mv, p, s)
+                  : launch_append<64, false>(cap, bias, mq, mk, mv, p, s));
   return r == cudaSuccess ? DFM_OK : DFM_ERR_CUDA;
 }
 
