@@ -51,6 +51,7 @@ constexpr int AP_PLAN_THREADS = 1024;
 constexpr int AP_COMBINE_THREADS = 256, AP_COMBINE_BLOCKS = 2;   // blocks to an SM
 constexpr int AP_MAX_CTAS = 256;    // most SMs the shares go to
 constexpr int AP_NEAR_SEQS = 256, AP_NEAR_UNITS = 512;   // what a CTA plans by itself
+constexpr int AP_NEAR_FIRST = 64;   // units, where every token has bounds of its own
 // What a unit costs besides its tiles (its first loads, the masked tiles, its rows'
 // way out: 4000 to 8000 clocks), in half tiles of a wide unit (1800 clocks).  With
 // shares of equal tiles alone, CTAs with many short units ended last: a chunked
@@ -69,6 +70,7 @@ struct __align__(16) ApUnit {
   int seq, t0, ntok, row0;          // tokens [t0, t0 + ntok) of the sequence; row0: its first in q
   int lo, hi, fmin, fmax;           // union of the rows' keys; tiles inside [fmin, fmax) have no mask
   int base, m, pre, at;             // position of token 0; the sequence's tokens and prefix; place in the line
+  DFM_DEV void keys(const ApUnit& o) { lo = o.lo, hi = o.hi, fmin = o.fmin, fmax = o.fmax; }
   DFM_DEV int tiles() const { return hi > lo ? (hi + AP_KT - 1) / AP_KT - lo / AP_KT : 0; }
   DFM_DEV int lead(int rt) const { return ntok > rt ? AP_WIDE_COST : AP_NARROW_COST; }
   DFM_DEV int cost(int rt) const { return lead(rt) + (tiles() << (ntok > rt)); }   // a wide unit's tile counts 2
@@ -185,6 +187,27 @@ DFM_DEV ApUnit ap_unit(const ApParams& p, int seq, int s0, int m, int ctx, int p
   return f;
 }
 
+// With bounds of every token's own: lo .. fmax of the unit at token t0, by a warp.
+DFM_DEV int4 ap_bounds(const ApParams& p, int s0, int m, int ctx, int pre, int t0) {
+  const int last = min(m, t0 + 2 * p.RT) - 1;
+  int lo = 0x7fffffff, hi = 0, fmin = 0, fmax = 0x7fffffff;
+  for (int j0 = t0 + (threadIdx.x & 31); j0 - 31 <= last; j0 += 32 * 4) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {   // past the end, the last token again
+      int l, h;
+      ap_keys(p, s0, min(j0 + 32 * x, last), ctx - m, ctx, pre, l, h);
+      if (l < h) {
+        lo = min(lo, l);
+        hi = max(hi, h);
+      }
+      fmin = max(fmin, l);
+      fmax = min(fmax, h);
+    }
+  }
+  return make_int4(__reduce_min_sync(0xffffffffu, lo), __reduce_max_sync(0xffffffffu, hi),
+                   __reduce_max_sync(0xffffffffu, fmin), __reduce_min_sync(0xffffffffu, fmax));
+}
+
 DFM_DEV int ap_share(const ApParams& p, int line) {
   return max(AP_MIN_SHARE, p.by_ctas(line * p.KVH + p.ctas - 1));
 }
@@ -226,7 +249,7 @@ struct ApNear {
     int2 all;
     const int2 before = block_scan<AP_THREADS / 32>(make_int2(c | (c > 0) << 20, cost), sums, all);
     int u = before.x & 0xfffff, place = before.y, total = all.x & 0xfffff;
-    const bool several = total != all.x >> 20;
+    const bool several = p.first || total != all.x >> 20;
     if (t < p.n) q.ubase[t] = u;
     if (total > p.max_units) {   // rows of overlapping sequences
       if (blockIdx.x == 0 && t == 0) atomicOr(p.err, DFM_DEV_ERR_LEN);
@@ -255,18 +278,32 @@ struct ApNear {
       start(mine);
     } else {
       __syncthreads();
+      auto seq_of = [&](int v) {   // the last sequence with ubase <= v (one without units shares the next one's)
+        int a = 0, b = p.n - 1;
+        while (a < b) {
+          const int mid = (a + b + 1) >> 1;
+          if (q.ubase[mid] <= v) a = mid; else b = mid - 1;
+        }
+        return a;
+      };
+      if (p.first) {
+        for (u = t >> 5; u < total; u += AP_THREADS / 32) {
+          const int a = seq_of(u);
+          if (!ap_length(p, q.m[a], q.ctx[a])) continue;
+          const int4 k = ap_bounds(p, q.s0[a], q.m[a], q.ctx[a], q.pre[a], (u - q.ubase[a]) * 2 * p.RT);
+          if ((t & 31) == 0) *reinterpret_cast<int4*>(&units[u].lo) = k;
+        }
+        __syncthreads();
+      }
       all.y = 0;
 #pragma unroll 1
       for (int u0 = 0; u0 < total; u0 += AP_THREADS) {
         u = u0 + t;
         cost = 0;
         if (u < total) {
-          int a = 0, b = p.n - 1;   // the last sequence with ubase <= u (one without units shares the next one's)
-          while (a < b) {
-            const int mid = (a + b + 1) >> 1;
-            if (q.ubase[mid] <= u) a = mid; else b = mid - 1;
-          }
+          const int a = seq_of(u);
           f = ap_unit(p, a, q.s0[a], q.m[a], q.ctx[a], q.pre[a], (u - q.ubase[a]) * 2 * p.RT);
+          if (p.first && ap_length(p, f.m, q.ctx[a])) f.keys(units[u]);
           cost = f.cost(p.RT);
         }
         int2 sum;
@@ -291,7 +328,7 @@ struct ApNear {
 };
 static_assert(AP_NEAR_SEQS <= AP_THREADS, "a thread to a sequence");
 
-// The plan of larger batches, and of per-token bounds: units, their keys and
+// The plan of larger batches: units, their keys and
 // their places in the line, from the device's lengths.  A sequence whose lengths
 // make no sense is reported: its rows are written as zeros, or not at all when
 // not even they are known.
@@ -339,23 +376,9 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
       int s0, m;
       ap_rows(p, a, s0, m);
       const int ctx = p.ctx[a], pre = p.prefix ? p.prefix[a] : 0;
-      const int t0 = (u - ubase(a)) * 2 * p.RT, end = min(m, t0 + 2 * p.RT);
-      int lo = 0x7fffffff, hi = 0, fmin = 0, fmax = 0x7fffffff;
-      for (int j = t0 + (t & 31); j < end; j += 32) {
-        int l, h;
-        ap_keys(p, s0, j, ctx - m, ctx, pre, l, h);
-        if (l < h) {
-          lo = min(lo, l);
-          hi = max(hi, h);
-        }
-        fmin = max(fmin, l);
-        fmax = min(fmax, h);
-      }
-      lo = __reduce_min_sync(0xffffffffu, lo);
-      hi = __reduce_max_sync(0xffffffffu, hi);
-      fmin = __reduce_max_sync(0xffffffffu, fmin);
-      fmax = __reduce_min_sync(0xffffffffu, fmax);
-      if ((t & 31) == 0) *reinterpret_cast<int4*>(&p.units[u].lo) = make_int4(lo, hi, fmin, fmax);
+      if (!ap_length(p, m, ctx)) continue;
+      const int4 k = ap_bounds(p, s0, m, ctx, pre, (u - ubase(a)) * 2 * p.RT);
+      if ((t & 31) == 0) *reinterpret_cast<int4*>(&p.units[u].lo) = k;
     }
     __syncthreads();
   }
@@ -370,13 +393,7 @@ __global__ void __launch_bounds__(AP_PLAN_THREADS) llm_append_plan_kernel(ApPara
       ap_rows(p, a, s0, m);
       const int ctx = p.ctx[a];
       f = ap_unit(p, a, s0, m, ctx, p.prefix ? p.prefix[a] : 0, (u - ubase(a)) * 2 * p.RT);
-      if (p.first && ap_length(p, m, ctx)) {
-        const int4 b = *reinterpret_cast<const int4*>(&p.units[u].lo);
-        f.lo = b.x;
-        f.hi = b.y;
-        f.fmin = b.z;
-        f.fmax = b.w;
-      }
+      if (p.first && ap_length(p, m, ctx)) f.keys(p.units[u]);
       cost = f.cost(p.RT);
     }
     int2 total;

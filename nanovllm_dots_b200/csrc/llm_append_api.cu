@@ -258,7 +258,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.max_units = ap_max_units(a->tokens, a->n, RT);
   p.ctas = ctas;
   // each CTA plans by itself where that fits its shared memory
-  p.near_plan = !a->first_keys && a->n <= AP_NEAR_SEQS && p.max_units <= AP_NEAR_UNITS;
+  p.near_plan = a->n <= AP_NEAR_SEQS && p.max_units <= (a->first_keys ? AP_NEAR_FIRST : AP_NEAR_UNITS);
   p.num_blocks = a->num_blocks;
   p.block_size = a->block_size;
   p.max_blocks = a->max_blocks;

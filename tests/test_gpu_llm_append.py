@@ -163,6 +163,15 @@ def test_documents(opts):
     run(Case(RAGGED, 16, 16, 64, 16, first=documents(RAGGED, 3), **opts))
 
 
+@pytest.mark.parametrize("n", [40, 200, 300])
+def test_documents_of_many_sequences(n):
+    """Units planned by the CTAs themselves, and by the kernel in front of them: more
+    units, and more sequences (some of them empty)."""
+    r = random.Random(n)
+    lens = [(r.choice((0, 1, 9, 33, 65)), r.randrange(1, 300)) for _ in range(n)]
+    run(Case(lens, 8, 1, 64, 64, first=documents(lens, n), slopes=slopes_of(8)))
+
+
 def test_rows_that_see_nothing_are_zero():
     """Every third token's document begins behind it; one sequence is all such tokens."""
     lens = [(70, 100), (3, 40), (64, 0)]
