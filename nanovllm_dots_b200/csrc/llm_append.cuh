@@ -44,7 +44,6 @@ namespace dfm {
 
 constexpr int AP_KT = 128;          // keys per tile
 constexpr int AP_ROWS = 128;        // rows per tile (TMEM lanes)
-constexpr int AP_RING = 2;          // K tiles and V tiles in shared memory
 constexpr int AP_SOFT_WARPS = 8;
 constexpr int AP_THREADS = 32 * (AP_SOFT_WARPS + 4);
 constexpr int AP_PLAN_THREADS = 1024;
@@ -490,12 +489,15 @@ struct ApWalk {
 template <int D>
 struct ApSmem {
   static constexpr int BOXES = D / 64;
+  // K tiles and V tiles: as many as there is room for (64 single tokens with heads of
+  // 64 over 6000 positions: 112 us with 2, 87 with 4).
+  static constexpr int RING = D == 64 ? 4 : 2;
   static constexpr int TILE = AP_KT * D * 2;              // one K, V or Q tile
   static constexpr int HALF = AP_KT * 128;                // its 64-dim boxes
   static constexpr int OFF_Q = 0;                         // [2]
-  static constexpr int OFF_K = OFF_Q + 2 * TILE;          // [AP_RING]
-  static constexpr int OFF_V = OFF_K + AP_RING * TILE;    // [AP_RING]
-  static constexpr int OFF_ML = OFF_V + AP_RING * TILE;   // float2 [2 streams][128]
+  static constexpr int OFF_K = OFF_Q + 2 * TILE;          // [RING]
+  static constexpr int OFF_V = OFF_K + RING * TILE;    // [RING]
+  static constexpr int OFF_ML = OFF_V + RING * TILE;   // float2 [2 streams][128]
   static constexpr int OFF_NEAR = OFF_ML + 2 * AP_ROWS * 8;
   static constexpr int OFF_BAR = OFF_NEAR + (static_cast<int>(sizeof(ApNear)) + 15) / 16 * 16;
   static constexpr int BYTES = OFF_BAR + 512 + 1024;
@@ -677,35 +679,33 @@ DFM_DEV void ap_exp2_pair(uint64_t x, float& a, float& b) {
 // of which an SM does 16 a clock, so that they and the softmax's exponential would
 // take three times the products' time.
 constexpr float AP_T0 = 0.999999464f, AP_T1 = -0.33326377f, AP_T2 = 0.131909163f, AP_T3 = -0.0444185946f;
-DFM_DEV void ap_cap(float (&xa)[32], float (&xb)[32], const ApParams& p) {
-  float big = 0.f, big1 = 0.f;
+DFM_DEV bool ap_hot(float big, const ApParams& p) {   // (a NaN is not above the bound and stays one)
+  return __any_sync(0xffffffffu, big * p.cap_a > 0.5f);
+}
+DFM_DEV void ap_cap(float (&x)[32], bool hot, const ApParams& p) {
+  if (hot) {
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
-    big = fmaxf(big, fabsf(xa[e]));
-    big1 = fmaxf(big1, fabsf(xb[e]));
-  }
-  // (a NaN is not above the bound and stays one in the polynomial)
-  if (__any_sync(0xffffffffu, fmaxf(big, big1) * p.cap_a > 0.5f)) {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      const float ra = __fdividef(1.f, 1.f + fast_exp2(xa[e] * p.cap_in));
-      const float rb = __fdividef(1.f, 1.f + fast_exp2(xb[e] * p.cap_in));
-      xa[e] = fmaf(-2.f * p.cap_b, ra, p.cap_b);
-      xb[e] = fmaf(-2.f * p.cap_b, rb, p.cap_b);
-    }
+    for (int e = 0; e < 32; ++e)
+      x[e] = fmaf(-2.f * p.cap_b, __fdividef(1.f, 1.f + fast_exp2(x[e] * p.cap_in)), p.cap_b);
     return;
   }
   const uint64_t q3 = f2(p.cap_q[2], p.cap_q[2]), q2 = f2(p.cap_q[1], p.cap_q[1]), q1 = f2(p.cap_q[0], p.cap_q[0]),
                  q0 = f2(AP_T0, AP_T0);
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
-    const uint64_t ya = f2(xa[e], xa[e + 1]), yb = f2(xb[e], xb[e + 1]);
-    const uint64_t za = f2_mul(ya, ya), zb = f2_mul(yb, yb);
-    const uint64_t ua = f2_fma(f2_fma(f2_fma(q3, za, q2), za, q1), za, q0);
-    const uint64_t ub = f2_fma(f2_fma(f2_fma(q3, zb, q2), zb, q1), zb, q0);
-    f2_split(f2_mul(ya, ua), xa[e], xa[e + 1]);
-    f2_split(f2_mul(yb, ub), xb[e], xb[e + 1]);
+    const uint64_t y = f2(x[e], x[e + 1]), z = f2_mul(y, y);
+    f2_split(f2_mul(y, f2_fma(f2_fma(f2_fma(q3, z, q2), z, q1), z, q0)), x[e], x[e + 1]);
   }
+}
+DFM_DEV float ap_cap_one(float x, bool hot, const ApParams& p) {
+  if (hot) return fmaf(-2.f * p.cap_b, __fdividef(1.f, 1.f + fast_exp2(x * p.cap_in)), p.cap_b);
+  const float z = x * x;
+  return x * fmaf(fmaf(fmaf(p.cap_q[2], z, p.cap_q[1]), z, p.cap_q[0]), z, AP_T0);
+}
+DFM_DEV float ap_abs32(const float (&x)[32], float big) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) big = fmaxf(big, fabsf(x[e]));
+  return big;
 }
 
 // x += slope e, one instruction a score (e is an immediate): with the row's and the
@@ -755,24 +755,24 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   float2* sML = reinterpret_cast<float2*>(smem + S::OFF_ML);
   ApNear& near = *reinterpret_cast<ApNear*>(smem + S::OFF_NEAR);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
-  uint64_t* k_empty = k_full + AP_RING;
-  uint64_t* v_full = k_empty + AP_RING;
-  uint64_t* v_ready = v_full + AP_RING;   // V without special values: arrivals of its two warps
-  uint64_t* v_empty = v_ready + AP_RING;
-  uint64_t* s_full = v_empty + AP_RING;   // [2] per stream
+  uint64_t* k_empty = k_full + S::RING;
+  uint64_t* v_full = k_empty + S::RING;
+  uint64_t* v_ready = v_full + S::RING;   // V without special values: arrivals of its two warps
+  uint64_t* v_empty = v_ready + S::RING;
+  uint64_t* s_full = v_empty + S::RING;   // [2] per stream
   uint64_t* p_full = s_full + 2;          // [2][2] its two halves of P: arrivals of its four warps
   uint64_t* o_full = p_full + 4;          // [2]
   uint64_t* q_full = o_full + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* drain = q_empty + 1;
-  uint32_t* poison = reinterpret_cast<uint32_t*>(drain + 1);   // [AP_RING][4]
-  uint32_t* tmem_slot = poison + AP_RING * 4;
+  uint32_t* poison = reinterpret_cast<uint32_t*>(drain + 1);   // [S::RING][4]
+  uint32_t* tmem_slot = poison + S::RING * 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((5 * AP_RING + 11) * 8 + AP_RING * 16 + 8 <= 512, "barrier area");
+  static_assert((5 * S::RING + 11) * 8 + S::RING * 16 + 8 <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < AP_RING; ++i) {
+    for (int i = 0; i < S::RING; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
@@ -819,13 +819,18 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       const int* bt = p.bt + static_cast<size_t>(sg.f.seq) * p.max_blocks;
       // lane = (box along the keys, 64-dim half); lanes past the tile's boxes are idle
       const int box = lane / S::BOXES, half = lane % S::BOXES;
-      auto block_of = [&](int i) {   // the lane's cache block in tile i, -2 if nobody sees the box
-        const int key = (sg.top - i) * AP_KT + box * p.box_rows;
-        if (box >= per_tile || i >= sg.i1 || key + p.box_rows <= sg.f.lo || key >= sg.f.hi) return -2;
+      // The cache blocks of 32 boxes, those of the tiles from i on, a lane's each: -2 if
+      // nobody sees the box.  With 16-row boxes that is 4 tiles' worth; looked up a tile
+      // at a time, 64 single tokens over 16-row pages took 126 us instead of 112.
+      auto blocks_from = [&](int i) {
+        i += lane / per_tile;
+        const int key = (sg.top - i) * AP_KT + lane % per_tile * p.box_rows;
+        if (i >= sg.i1 || key + p.box_rows <= sg.f.lo || key >= sg.f.hi) return -2;
         const int b = bt[p.by_block(key)];
         return b < 0 ? -1 : b;
       };
-      int blk = block_of(sg.i0);
+      const int ahead = 32 / per_tile;
+      int now = blocks_from(sg.i0), next = blocks_from(sg.i0 + ahead), used = 0;
       if (lane == 0) {
         ok = nseg == 0 || ap_wait(q_empty, (nseg - 1) & 1, abort_flag, p.err);
         if (ok) {
@@ -840,27 +845,31 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       ok = __shfl_sync(0xffffffffu, ok, 0);
       ++nseg;
       for (int i = sg.i0; ok && i < sg.i1; ++i, ++g) {
-        const int slot = g % AP_RING;
+        const int slot = g % S::RING;
         const int key = (sg.top - i) * AP_KT + box * p.box_rows;
         const int row = key - p.by_block(key) * p.block_size;
-        const bool mine = blk != -2;
-        int cb = blk;
+        int cb = __shfl_sync(0xffffffffu, now, used * per_tile + box);
+        const bool mine = box < per_tile && cb != -2;
+        if (++used == ahead) {
+          used = 0;
+          now = next;
+          next = blocks_from(i + 1 + ahead);
+        }
         if (mine && (cb < 0 || cb >= p.num_blocks)) {
           if (half == 0) atomicOr(p.err, DFM_DEV_ERR_PAGE);
           cb = p.num_blocks;   // out of range: zeros
         }
-        blk = block_of(i + 1);
         const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box_bytes;
         const int dst = slot * S::TILE + half * S::HALF + box * box_bytes;
         if (lane == 0) {
-          ok = g < AP_RING || ap_wait(&k_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
+          ok = g < S::RING || ap_wait(&k_empty[slot], ((g / S::RING) & 1) ^ 1, abort_flag, p.err);
           if (ok) mbar_arrive_expect_tx(&k_full[slot], bytes);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         if (mine) tma_load_4d(sK + dst, &tm_k, &k_full[slot], half * 64, sg.kv, row, cb);
         if (lane == 0) {
-          ok = g < AP_RING || ap_wait(&v_empty[slot], ((g / AP_RING) & 1) ^ 1, abort_flag, p.err);
+          ok = g < S::RING || ap_wait(&v_empty[slot], ((g / S::RING) & 1) ^ 1, abort_flag, p.err);
           if (ok) mbar_arrive_expect_tx(&v_full[slot], bytes);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -874,9 +883,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     if (!ok && lane == 0) {
       // copies that nobody waited for must land before the CTA's memory is gone
       if (nseg > 0) mbar_drain(q_full, (nseg - 1) & 1);
-      for (int x = g > AP_RING ? g - AP_RING : 0; x < g; ++x) {
-        mbar_drain(&k_full[x % AP_RING], (x / AP_RING) & 1);
-        mbar_drain(&v_full[x % AP_RING], (x / AP_RING) & 1);
+      for (int x = g > S::RING ? g - S::RING : 0; x < g; ++x) {
+        mbar_drain(&k_full[x % S::RING], (x / S::RING) & 1);
+        mbar_drain(&v_full[x % S::RING], (x / S::RING) & 1);
       }
     }
   } else if (warp == AP_SOFT_WARPS + 1) {
@@ -899,7 +908,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       };
       // S_s = Q_x K^T for the K tile of ring position `at`
       auto scores = [&](int s, int x, int at) {
-        const uint64_t q = dq + x * (S::TILE >> 4), k = dk + (at % AP_RING) * (S::TILE >> 4);
+        const uint64_t q = dq + x * (S::TILE >> 4), k = dk + (at % S::RING) * (S::TILE >> 4);
         const uint32_t d = tmem + s * AP_KT;
         if (leader) {
 #pragma unroll
@@ -912,18 +921,18 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         }
       };
       auto k_wait = [&](int at) {
-        ok = ok && ap_wait(&k_full[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err);
+        ok = ok && ap_wait(&k_full[at % S::RING], (at / S::RING) & 1, abort_flag, p.err);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       };
       // O_s += P_s V, half a key tile at a time
       auto values = [&](int s, int at, bool first) {
-        const uint64_t v = dv + (at % AP_RING) * (S::TILE >> 4);
+        const uint64_t v = dv + (at % S::RING) * (S::TILE >> 4);
         const uint32_t d = tmem + 256 + s * D, a = tmem + s * AP_KT;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           ok = ok && ap_wait(&p_full[2 * s + h], np[s] & 1, abort_flag, p.err) &&
-               (h > 0 || ap_wait(&v_ready[at % AP_RING], (at / AP_RING) & 1, abort_flag, p.err));
+               (h > 0 || ap_wait(&v_ready[at % S::RING], (at / S::RING) & 1, abort_flag, p.err));
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           tc_fence_after();
@@ -946,20 +955,20 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             k_wait(g + i);
             if (!ok) break;
             scores(i, 0, g + i);
-            commit(&k_empty[(g + i) % AP_RING]);
+            commit(&k_empty[(g + i) % S::RING]);
             if (i == nt - 1) commit(q_empty);
           }
           for (int i = 0; ok && i < nt; ++i) {
             const int s = i & 1;
             values(s, g + i, i < 2);
             if (!ok) break;
-            commit(&v_empty[(g + i) % AP_RING]);
+            commit(&v_empty[(g + i) % S::RING]);
             if (i + 2 >= nt) commit(&o_full[s]);
             if (i + 2 < nt) {
               k_wait(g + i + 2);
               if (!ok) break;
               scores(s, 0, g + i + 2);
-              commit(&k_empty[(g + i + 2) % AP_RING]);
+              commit(&k_empty[(g + i + 2) % S::RING]);
               if (i + 2 == nt - 1) commit(q_empty);
             }
           }
@@ -968,13 +977,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if (!ok) break;
           scores(0, 0, g);
           scores(1, 1, g);
-          commit(&k_empty[g % AP_RING]);
+          commit(&k_empty[g % S::RING]);
           if (nt == 1) commit(q_empty);
           for (int i = 0; ok && i < nt; ++i) {
             for (int s = 0; s < 2; ++s) {
               values(s, g + i, i == 0);
               if (!ok) break;
-              if (s == 1) commit(&v_empty[(g + i) % AP_RING]);
+              if (s == 1) commit(&v_empty[(g + i) % S::RING]);
               if (i == nt - 1) {
                 commit(&o_full[s]);
                 continue;
@@ -983,7 +992,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if (!ok) break;
               scores(s, s, g + i + 1);
               if (s == 1) {
-                commit(&k_empty[(g + i + 1) % AP_RING]);
+                commit(&k_empty[(g + i + 1) % S::RING]);
                 if (i + 1 == nt - 1) commit(q_empty);
               }
             }
@@ -1003,8 +1012,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     bool ok = true;
     while (ok && walk.next(p, sg)) {
       for (int i = sg.i0; i < sg.i1; ++i, ++g) {
-        const int slot = g % AP_RING;
-        ok = __all_sync(0xffffffffu, ap_wait(&v_full[slot], (g / AP_RING) & 1, abort_flag, p.err));
+        const int slot = g % S::RING;
+        ok = __all_sync(0xffffffffu, ap_wait(&v_full[slot], (g / S::RING) & 1, abort_flag, p.err));
         if (!ok) break;
         const int k0 = (sg.top - i) * AP_KT;
         if (k0 < sg.f.fmin || k0 + AP_KT > sg.f.fmax) {
@@ -1106,16 +1115,25 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           float shift = 0.f, grow = 0.f, top = -INFINITY;
           float xa[32], xb[32];
           auto ld = [&](float (&x)[32], int c) { ap_load(tS + c * 32, x); };
-          if (!kMod && full) {
+          bool raw = false, hot = false;   // the cap is left to the second pass
+          if (!kBias && full) {
+            float big = 0.f;
             ld(xa, 0);
 #pragma unroll 1
             for (int c = 0; c < 4; c += 2) {
               ap_landed(xa);
               ld(xb, c + 1);
               top = ap_max32(xa, top);
+              if (kCap) big = ap_abs32(xa, big);
               ap_landed(xb);
               if (c == 0) ld(xa, 2);
               top = ap_max32(xb, top);
+              if (kCap) big = ap_abs32(xb, big);
+            }
+            if constexpr (kCap) {   // the cap rises with the score: the maximum's is the maximum
+              raw = true;
+              hot = ap_hot(big, p);
+              top = ap_cap_one(top, hot, p);
             }
           } else {
             const bool behind = k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix);
@@ -1138,7 +1156,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               ap_load(tS + c + 32, xb);
               ap_landed(xa);
               ap_landed(xb);
-              if constexpr (kCap) ap_cap(xa, xb, p);
+              if constexpr (kCap) {
+                const bool h = ap_hot(ap_abs32(xa, ap_abs32(xb, 0.f)), p);
+                ap_cap(xa, h, p);
+                ap_cap(xb, h, p);
+              }
               if constexpr (kBias) {
                 if (behind) {   // every key the row sees is at or before it: |p - k| = (p - k0) - c
                   ap_slope(xa, slope);
@@ -1166,8 +1188,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
             if (!full) {
               // special values of V that this row sees, noted until the product takes V
-              const int slot = (g + i) % AP_RING;
-              ok = __all_sync(0xffffffffu, ap_wait(&v_ready[slot], ((g + i) / AP_RING) & 1, abort_flag, p.err));
+              const int slot = (g + i) % S::RING;
+              ok = __all_sync(0xffffffffu, ap_wait(&v_ready[slot], ((g + i) / S::RING) & 1, abort_flag, p.err));
               if (!ok) break;
               uint32_t bad = 0;
               for (int c = 0; c < 4; ++c) bad |= poison[slot * 4 + c] & sees(k0 + c * 32);
@@ -1223,9 +1245,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           for (int h = 0; h < 2; ++h) {
             ap_landed(xa);
             ld(xb, 2 * h + 1);
+            if (kCap && raw) ap_cap(xa, hot, p);
             probabilities(xa, 0, 2 * h);
             ap_landed(xb);
             if (h == 0) ld(xa, 2);
+            if (kCap && raw) ap_cap(xb, hot, p);
             probabilities(xb, 16, 2 * h + 1);
             tmem_st32(tS + h * 32, pk);
             tmem_wait_st();
