@@ -175,7 +175,7 @@ typedef struct DllmAppend {
   int32_t causal, window;
   float scale, softcap;
   const void* q;                /* [tokens, num_heads, head_dim], 16-byte aligned rows */
-  int64_t q_token_stride, q_head_stride;       /* elements, multiples of 8 */
+  int64_t q_token_stride, q_head_stride;       /* elements, multiples of 8, head_dim or more */
   const void* k_cache;          /* [num_blocks, block_size, num_kv_heads, head_dim] */
   const void* v_cache;
   const int32_t* cu_seqlens_q;  /* [n + 1] */
@@ -185,7 +185,8 @@ typedef struct DllmAppend {
   const int32_t* first_keys;    /* [tokens] or NULL */
   const uint64_t* tree_masks;   /* [tokens] or NULL */
   const float* slopes;          /* [num_heads] or NULL */
-  void* out;                    /* [tokens, num_heads, head_dim] */
+  void* out;                    /* [tokens, num_heads, head_dim], 32-byte aligned; may be a
+                                 * q of the same strides, else no overlap */
 } DllmAppend;
 
 /* Workspace bytes for up to these bounds, 0 if the shape is not supported.
@@ -196,10 +197,12 @@ size_t dllm_append_workspace_size(int32_t tokens, int32_t n, int32_t num_heads,
                                   int32_t num_kv_heads, int32_t head_dim);
 
 /* Stream ordered, no allocation, no host synchronisation; the launches depend
- * on the arguments but not on the lengths in device memory.  Lengths that make
- * no sense, a block id out of range or a tree of more than 64 tokens set a
- * device error bit (dllm_read_error); such a sequence's rows are zeros, or
- * untouched where cu_seqlens_q itself is wrong, and such a block reads as zeros. */
+ * on the arguments but not on the lengths in device memory.  Block tables of
+ * nearly 2^31 positions, or of more key tiles in all than 32 bits count, are
+ * refused (DFM_ERR_UNSUPPORTED).  Lengths that make no sense, a block id out of
+ * range or a tree of more than 64 tokens set a device error bit
+ * (dllm_read_error); such a sequence's rows are zeros, or untouched where
+ * cu_seqlens_q itself is wrong, and such a block reads as zeros. */
 int dllm_append_attention(const DllmAppend* args, void* workspace, size_t workspace_bytes,
                           void* stream);
 

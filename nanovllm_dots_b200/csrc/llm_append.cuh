@@ -880,8 +880,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (mine) tma_load_4d(sV + dst, &tm_v, &v_full[slot], half * 64, sg.kv, row, cb);
       }
     }
-    if (!ok && lane == 0) {
-      // copies that nobody waited for must land before the CTA's memory is gone
+    if (lane == 0) {
+      // Copies must have landed before the CTA's memory is gone, also those that a
+      // warp which gave up did not wait for.
       if (nseg > 0) mbar_drain(q_full, (nseg - 1) & 1);
       for (int x = g > S::RING ? g - S::RING : 0; x < g; ++x) {
         mbar_drain(&k_full[x % S::RING], (x / S::RING) & 1);
@@ -1000,10 +1001,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         }
         g += nt;
       }
-      if (!ok) {   // products in flight read shared memory and TMEM
-        commit(drain);
-        if (leader) mbar_drain(drain, 0);
-      }
+      commit(drain);   // products in flight read shared memory and TMEM
+      if (leader) mbar_drain(drain, 0);
     }
   } else if (warp > AP_SOFT_WARPS) {
     // ------------------------------------------------------------ special rows of V

@@ -95,8 +95,9 @@ bool map_ap_q(CUtensorMap* m, const DllmAppend& a, int G, int RT) {
   if (!fn) return false;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.num_heads),
                         static_cast<cuuint64_t>(a.tokens)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.q_head_stride) * 2,
-                           static_cast<cuuint64_t>(a.q_token_stride) * 2};
+  // (a dimension of one element has any stride: it is not stepped over)
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.num_heads > 1 ? a.q_head_stride : a.head_dim) * 2,
+                           static_cast<cuuint64_t>(a.tokens > 1 ? a.q_token_stride : a.head_dim) * 2};
   cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(RT)};
   cuuint32_t es[3] = {1, 1, 1};
   return fn(m, a.dtype == DLLM_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
@@ -214,7 +215,8 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   if (a->tree_masks && (a->prefix_lens || a->first_keys || a->slopes || a->window))
     return DFM_ERR_UNSUPPORTED;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || reinterpret_cast<uintptr_t>(a->out) % 32 ||
-      a->q_token_stride % 8 || a->q_head_stride % 8 || a->q_token_stride < 0 || a->q_head_stride < 0)
+      (a->tokens > 1 && (a->q_token_stride % 8 || a->q_token_stride < a->head_dim)) ||
+      (a->num_heads > 1 && (a->q_head_stride % 8 || a->q_head_stride < a->head_dim)))
     return DFM_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return DFM_ERR_INVALID_ARG;
   const int G = a->num_heads / a->num_kv_heads, RT = AP_ROWS / G, ctas = ap_ctas();

@@ -15,6 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .llm_rotary import overlap
 
 _DTYPES = {torch.bfloat16: _lib.DLLM_BF16, torch.float16: _lib.DLLM_FP16}
 TREE_MAX = 64     # drafted tokens of one sequence
@@ -104,8 +105,8 @@ class B200AppendAttention:
             raise RuntimeError(f"append of {T} tokens of {n} sequences "
                                f"(at most {self.max_tokens} of {self.max_seqs})")
         st, sh, sd = q.stride()
-        if sd != 1 or st % 8 or sh % 8 or q.data_ptr() % 16:
-            raise RuntimeError("q: expected contiguous head dims and 16-byte aligned heads")
+        if sd != 1 or T > 1 and (st % 8 or st < D) or H > 1 and (sh % 8 or sh < D) or q.data_ptr() % 16:
+            raise RuntimeError("q: expected contiguous head dims and 16-byte aligned heads that share no memory")
         geometry = (k_cache.shape[0], self.block_size, self.num_kv_heads, D)
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
             if c.dtype is not dtype or c.get_device() != index or c.shape != geometry or \
@@ -123,6 +124,10 @@ class B200AppendAttention:
         elif out.dtype is not dtype or out.get_device() != index or out.shape != (T, H, D) or \
                 not out.is_contiguous():
             raise RuntimeError(f"out: expected a contiguous {dtype} tensor {(T, H, D)} on {self.device}")
+        elif out.data_ptr() % 32:
+            raise RuntimeError("out: expected 32-byte alignment")
+        elif overlap(q, out) and not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):
+            raise RuntimeError("out: overlaps q without being q")
         i32, width = torch.int32, table.shape[1]
         plain = tree is None
         a = _lib.DllmAppend(
@@ -165,8 +170,9 @@ class B200AppendAttention:
         cached positions, the new tokens included; int32 block_tables [n, width].
         prefix_lens [n]: leading positions every token of the sequence sees,
         whatever its own; first_keys [tokens]: the first position a token sees
-        (its document's).  -> [tokens, H, D]; zeros where a token sees nothing,
-        rows past cu_seqlens_q[n] as they were."""
+        (its document's).  -> [tokens, H, D] (``out=q`` overwrites a contiguous
+        q); zeros where a token sees nothing, rows past cu_seqlens_q[n] as they
+        were (in an ``out`` of its own: undefined)."""
         return self._run(q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, prefix_lens,
                          first_keys, None, out, stream)
 

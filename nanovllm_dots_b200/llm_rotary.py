@@ -169,7 +169,7 @@ class B200Rotary:
             if out.data_ptr() == q.data_ptr():
                 if (qt, qh) != (ot, oh):
                     raise RuntimeError("out: rotating in place needs q's own strides")
-            elif _overlap(q, out):
+            elif overlap(q, out):
                 raise RuntimeError("out: overlaps q without being q")
             if not _apart(out):
                 raise RuntimeError("out: rows share memory")
@@ -235,7 +235,7 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _overlap(a, b) -> bool:
+def overlap(a, b) -> bool:
     if not a.numel() or not b.numel():
         return False
     (a0, a1), (b0, b1) = _span(a), _span(b)

@@ -315,6 +315,46 @@ def test_strided_queries():
     assert torch.equal(c.call(att), want)
 
 
+def test_one_token_or_head_has_any_stride():
+    c = Case([(1, 300)]).device()
+    att = c.attention()
+    want = c.call(att)
+    c.qd = c.qd.as_strided((1, 12, 128), (7, 128, 1))
+    assert torch.equal(c.call(att), want)
+    c = Case([(9, 300)], 1, 1).device()
+    att = c.attention()
+    want = c.call(att)
+    c.qd = c.qd.as_strided((9, 1, 128), (128, 5, 1))
+    assert torch.equal(c.call(att), want)
+
+
+def test_out_may_be_q_and_nothing_near_it():
+    """Units of one and of several shares, narrow and wide, written over their queries."""
+    c = Case([(200, 3000), (1, 5000), (64, 100), (7, 0)], 8, 2).device()
+    att = c.attention()
+    want, q = c.call(att), c.qd
+    for _ in range(3):
+        c.qd = q.clone()
+        assert c.call(att, out=c.qd) is c.qd and torch.equal(c.qd, want)
+    T = q.shape[0]
+    room = torch.zeros(T + 1, 8, 128, dtype=BF, device=DEV)
+    c.qd = room[:T]
+    with pytest.raises(RuntimeError, match="overlaps"):
+        c.call(att, out=room[1:])
+    with pytest.raises(RuntimeError, match="32-byte"):
+        c.call(att, out=room.flatten()[8:8 + T * 1024].view(T, 8, 128))
+    c.qd = room[:1].expand(T, 8, 128)
+    with pytest.raises(RuntimeError, match="share no memory"):
+        c.call(att)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [2.0, 12.0, 60.0])
+def test_cap_of_unmasked_tiles(cap, D):
+    """Scores mostly past the cap, around half of it, and far below."""
+    run(Case([(30, 900), (1, 1100), (70, 600)], D=D, softcap=cap, spread=2.0))
+
+
 def test_bad_block_id_is_reported_and_read_as_zeros():
     c = Case([(5, 600), (3, 20)])
     c.device()
