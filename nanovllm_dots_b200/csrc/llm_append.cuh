@@ -47,7 +47,7 @@ constexpr int AP_ROWS = 128;        // rows per tile (TMEM lanes)
 constexpr int AP_SOFT_WARPS = 8;
 constexpr int AP_THREADS = 32 * (AP_SOFT_WARPS + 4);
 constexpr int AP_PLAN_THREADS = 1024;
-constexpr int AP_COMBINE_THREADS = 256, AP_COMBINE_BLOCKS = 2;   // blocks to an SM
+constexpr int AP_COMBINE_THREADS = 256, AP_COMBINE_BLOCKS = 3;   // blocks to an SM
 constexpr int AP_MAX_CTAS = 256;    // most SMs the shares go to
 constexpr int AP_NEAR_SEQS = 256, AP_NEAR_UNITS = 512;   // what a CTA plans by itself
 constexpr int AP_NEAR_FIRST = 64;   // units, where every token has bounds of its own
@@ -81,8 +81,8 @@ struct ApHead {                     // the plan's header
 };
 
 struct ApCut {                      // the unit that the end of a share cuts
-  int row, ntok, narrow, kv;        // its first token's row in q
-  int last, pad[3];                 // last share it reaches into; -1: no unit of this share is cut
+  int row, ntok, kv;                // its first token's row in q
+  int last;                         // last share it reaches into; -1: no unit of this share is cut
 };
 
 struct ApParams {
@@ -1271,7 +1271,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       if (sg.i0 == 0 && !whole) {     // the end of the share cuts this unit
         cut.row = sg.f.row0 + sg.f.t0;
         cut.ntok = sg.f.ntok;
-        cut.narrow = sg.narrow;
         cut.kv = sg.kv;
         cut.last = (sg.kv * walk.line + sg.f.at + sg.f.lead(p.RT) + ((sg.tiles - 1) << !sg.narrow)) / walk.share;
       }
@@ -1357,15 +1356,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 //   out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j over the shares j.
 // An item is 8 dims of 32 rows, which lie next to each other in the partials.  A
 // load of another SM's partial takes over a microsecond, so the items of all cuts
-// are spread evenly over one wave of blocks, and where there are few, 2 or 4
+// are spread evenly over one wave of blocks (three to an SM with three shares in
+// flight a thread: 0.5 to 1 us faster than two with four), and where there are few, 2 or 4
 // warps take an item's shares in turn (their sums are added in the warps' order).
 template <int D, bool kFp16>
 __global__ void __launch_bounds__(AP_COMBINE_THREADS, AP_COMBINE_BLOCKS)
     llm_append_combine_kernel(const ApParams p) {
-  constexpr int CB = 4, DG = D / 8, WARPS = AP_COMBINE_THREADS / 32;
+  constexpr int CB = 3, DG = D / 8, WARPS = AP_COMBINE_THREADS / 32;
   __shared__ float part[WARPS][10][32];
   __shared__ int2 sums[WARPS];
-  __shared__ ApCut cuts[AP_MAX_CTAS];
+  __shared__ int4 cuts[AP_MAX_CTAS];    // ApCut: row, ntok, kv, last
   __shared__ int starts[AP_MAX_CTAS];
   pdl_trigger();
   pdl_wait();
@@ -1373,8 +1373,8 @@ __global__ void __launch_bounds__(AP_COMBINE_THREADS, AP_COMBINE_BLOCKS)
   auto row_groups = [&](int tokens) { return (tokens * p.G + 31) >> 5; };
   int n = 0;
   if (t < p.ctas) {
-    const ApCut c = p.cuts[t];
-    if (c.last > t) n = (row_groups(min(c.ntok, p.RT)) + row_groups(c.ntok - min(c.ntok, p.RT))) * DG;
+    const int4 c = *reinterpret_cast<const int4*>(&p.cuts[t]);
+    if (c.w > t) n = (row_groups(min(c.y, p.RT)) + row_groups(c.y - min(c.y, p.RT))) * DG;
     cuts[t] = c;
   }
   int2 all;
@@ -1393,21 +1393,22 @@ __global__ void __launch_bounds__(AP_COMBINE_THREADS, AP_COMBINE_BLOCKS)
       const int mid = (b + hi + 1) >> 1;
       if (starts[mid] <= it) b = mid; else hi = mid - 1;
     }
-    const ApCut f = cuts[b];
+    const int4 cut = cuts[b];
+    const int row = cut.x, ntok = cut.y, kv = cut.z, last = cut.w;
     const int item = it - starts[b], dg = item % DG, rg = item / DG;
-    const int first = min(f.ntok, p.RT), groups1 = row_groups(first), tile = rg >= groups1;
+    const int first = min(ntok, p.RT), groups1 = row_groups(first), tile = rg >= groups1;
     const int r = (tile ? rg - groups1 : rg) * 32 + lane;
-    const bool mine = i0 + warp / team < items && r < (tile ? f.ntok - first : first) * p.G;
+    const bool mine = i0 + warp / team < items && r < (tile ? ntok - first : first) * p.G;
     float M = -INFINITY, L = 0.f, acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    for (int c0 = b + k; mine && c0 <= f.last; c0 += CB * team) {
+    for (int c0 = b + k; mine && c0 <= last; c0 += CB * team) {
       float2 ml[CB];
       float4 o[CB][2];
 #pragma unroll
       for (int x = 0; x < CB; ++x) {
         const int c = c0 + x * team;
-        const bool in = c <= f.last;
+        const bool in = c <= last;
         const size_t at = (static_cast<size_t>(c) * 2 + (c > b ? 0 : 1)) * 2 + tile;
         const float* src = p.part_o + at * AP_ROWS * D + (dg * AP_ROWS + r) * 8;
         ml[x] = in ? p.part_ml[at * AP_ROWS + r] : make_float2(-INFINITY, 0.f);
@@ -1464,7 +1465,7 @@ __global__ void __launch_bounds__(AP_COMBINE_THREADS, AP_COMBINE_BLOCKS)
     const int tok = p.by_g(r), j = tile * p.RT + tok;
     *reinterpret_cast<uint4*>(
         static_cast<uint16_t*>(p.out) +
-        (static_cast<size_t>(f.row + j) * p.H + f.kv * p.G + r - tok * p.G) * D + dg * 8) =
+        (static_cast<size_t>(row + j) * p.H + kv * p.G + r - tok * p.G) * D + dg * 8) =
         make_uint4(ap_pack<kFp16>(acc[0] * inv, acc[1] * inv), ap_pack<kFp16>(acc[2] * inv, acc[3] * inv),
                    ap_pack<kFp16>(acc[4] * inv, acc[5] * inv), ap_pack<kFp16>(acc[6] * inv, acc[7] * inv));
   }
