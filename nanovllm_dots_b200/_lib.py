@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 import torch
@@ -277,6 +278,18 @@ def call_on(index: int, fn, *args) -> int:
         return fn(*args)
     with torch.cuda.device(index):
         return fn(*args)
+
+
+def packer(args):
+    """What packs the fields of the ctypes structure ``args`` into its bytes (null
+    pointers as 0): a quarter of the time of building the structure."""
+    codes = {c_int32: "i", c_float: "f", c_int64: "q", c_void_p: "P"}
+    return struct.Struct("@" + "".join(codes[t] for _, t in args._fields_)).pack
+
+
+def packed(name: str, *argtypes):
+    """The library's function ``name``, its structure taken as packed bytes."""
+    return ctypes.CFUNCTYPE(c_int32, ctypes.c_char_p, *argtypes)((name, lib()))
 
 
 def ptr(t) -> int | None:

@@ -18,6 +18,7 @@ from . import _lib
 from .llm_rotary import overlap
 
 _DTYPES = {torch.bfloat16: _lib.DLLM_BF16, torch.float16: _lib.DLLM_FP16}
+_pack = _lib.packer(_lib.DllmAppend)
 TREE_MAX = 64     # drafted tokens of one sequence
 
 
@@ -86,7 +87,9 @@ class B200AppendAttention:
         self.workspace[:256].zero_()
         self._index = self.device.index
         self._dtype = _DTYPES[dtype]
-        self._call, self._workspace = self.L.dllm_append_attention, self.workspace.data_ptr()
+        self._call = _lib.packed("dllm_append_attention", _lib.c_void_p, _lib.c_size_t, _lib.c_void_p)
+        self._workspace = self.workspace.data_ptr()
+        self._slopes = 0 if slopes is None else slopes.data_ptr()
         self._stream = _lib.raw_stream(self._index)   # the last one used: that of the zero-fill
 
     def _ints(self, name, t, dtype, shape):
@@ -130,15 +133,15 @@ class B200AppendAttention:
             raise RuntimeError("out: overlaps q without being q")
         i32, width = torch.int32, table.shape[1]
         plain = tree is None
-        a = _lib.DllmAppend(
+        a = _pack(
             self._dtype, T, n, H, self.num_kv_heads, D, geometry[0], self.block_size, width, self.causal,
             self.window if plain else 0, self.scale, self.softcap, q.data_ptr(), st, sh,
             k_cache.data_ptr(), v_cache.data_ptr(), self._ints("cu_seqlens_q", cu, i32, (n + 1,)),
             self._ints("context_lens", ctx, i32, (n,)), self._ints("block_tables", table, i32, (n, width)),
-            None if prefix is None else self._ints("prefix_lens", prefix, i32, (n,)),
-            None if first is None else self._ints("first_keys", first, i32, (T,)),
-            None if plain else self._ints("tree_masks", tree, torch.int64, (T,)),
-            self.slopes.data_ptr() if plain and self.slopes is not None else None, out.data_ptr())
+            0 if prefix is None else self._ints("prefix_lens", prefix, i32, (n,)),
+            0 if first is None else self._ints("first_keys", first, i32, (T,)),
+            0 if plain else self._ints("tree_masks", tree, torch.int64, (T,)),
+            self._slopes if plain else 0, out.data_ptr())
         if T == 0:
             return out
         handle = _lib.raw_stream(index) if stream is None else stream.cuda_stream

@@ -18,6 +18,7 @@ from . import _lib
 
 _DTYPES = {torch.bfloat16: _lib.DLLM_BF16, torch.float16: _lib.DLLM_FP16,
            torch.float32: _lib.DLLM_FP32}
+_pack = _lib.packer(_lib.DllmRotary)
 KINDS = ("linear", "ntk", "bands", "yarn")
 LAYOUTS = ("half", "interleaved")
 
@@ -124,7 +125,8 @@ class B200Rotary:
         self.L = _lib.lib()
         self.turns = _turns(inv).to(self.device)
         self.err = torch.zeros(64, dtype=torch.int32, device=self.device)
-        self._index, self._inter, self._call = self.device.index, layout == "interleaved", self.L.dllm_rotary
+        self._index, self._inter = self.device.index, layout == "interleaved"
+        self._call = _lib.packed("dllm_rotary", _lib.c_void_p)
         self._turns, self._err = self.turns.data_ptr(), self.err.data_ptr()
 
     def _heads(self, name, t, dtype, tokens):
@@ -173,8 +175,7 @@ class B200Rotary:
                 raise RuntimeError("out: overlaps q without being q")
             if not _apart(out):
                 raise RuntimeError("out: rows share memory")
-        kvh, kt, kh, vt, vh, slots, places = 0, 0, 0, 0, 0, 0, None
-        kp = vp = kcp = vcp = None
+        kvh = kt = kh = vt = vh = slots = places = kp = vp = kcp = vcp = 0
         if store is not None:
             k, v, slot_mapping, k_cache, v_cache = store
             kvh, kt, kh = self._heads("k", k, q.dtype, T)
@@ -193,9 +194,9 @@ class B200Rotary:
             kp, vp, kcp, vcp = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
         if T == 0 or heads == 0 and store is None:
             return out
-        a = _lib.DllmRotary(dtype, T, heads, kvh, self.head_dim, self.rot_dim, self._inter, self.factor,
-                            self._turns, pos, q.data_ptr(), out.data_ptr(), kp, vp, kcp, vcp, places,
-                            qt, qh, ot, oh, kt, kh, vt, vh, slots, self._err)
+        a = _pack(dtype, T, heads, kvh, self.head_dim, self.rot_dim, self._inter, self.factor,
+                  self._turns, pos, q.data_ptr(), out.data_ptr(), kp, vp, kcp, vcp, places,
+                  qt, qh, ot, oh, kt, kh, vt, vh, slots, self._err)
         handle = _lib.raw_stream(self._index) if stream is None else stream.cuda_stream
         rc = _lib.call_on(self._index, self._call, a, handle)
         if rc:

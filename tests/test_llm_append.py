@@ -39,6 +39,13 @@ def test_struct_matches_header(name, tmp_path):
     assert said == [ctypes.sizeof(cls)] + [getattr(cls, f).offset for f, _ in cls._fields_]
 
 
+@pytest.mark.parametrize("args", [_lib.DllmRotary, _lib.DllmAppend])
+def test_packed_arguments_are_the_structure(args):
+    values = [i + 0.5 if t is ctypes.c_float else (1 << 40) + i if ctypes.sizeof(t) == 8 else -i
+              for i, (_, t) in enumerate(args._fields_)]
+    assert _lib.packer(args)(*values) == bytes(args(*values))
+
+
 # pointers of refused calls are never followed: the checks come first
 A = 1 << 12
 
