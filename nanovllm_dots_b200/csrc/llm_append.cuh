@@ -29,6 +29,18 @@
 //   S[128 x 128] = Q K^T      (Q and K from shared memory)
 //   O[128 x D]  += P V        (P from TMEM, V from shared memory)
 //
+// What bounds it.  Single tokens and small trees: HBM, at its rate while the tiles
+// stream (64 single tokens over 4000 positions of 4 x 128 dims: 99 us, 5.5 TB/s), plus
+// the fixed way in (3.5 us from the start to the first scores) and out (join 4.5 us).
+// Two full row tiles: a stream's chain of maximum (750 clocks), probabilities (1500)
+// and the products of P and of the next scores (1250 of latency and of the other
+// stream's): 3500 clocks a key tile, of which the tensor cores are busy 2048 with
+// D = 128.  8192 tokens behind 8192: 516 us, 1.2 PFLOP/s (595 us and 1.04 under the
+// power cap; the same loads and products without a softmax 440).  All 512 TMEM columns are
+// taken (S, S, O, O), so scores cannot be computed ahead of P; key tiles of 64 in two
+// buffers, which could, take the tensor cores twice as long a score (676 us);
+// two threads a row instead of one: 568.
+//
 // Keys nobody in the unit may see are not loaded (their pages may be gone) and
 // their rows of V are set to zero.  In a tile with masks, a visible row of V
 // that holds an infinity or a NaN is set to zero as well and noted: the rows
@@ -50,7 +62,8 @@ constexpr int AP_PLAN_THREADS = 1024;
 constexpr int AP_COMBINE_THREADS = 256, AP_COMBINE_BLOCKS = 3;   // blocks to an SM
 constexpr int AP_MAX_CTAS = 256;    // most SMs the shares go to
 constexpr int AP_NEAR_SEQS = 256, AP_NEAR_UNITS = 512;   // what a CTA plans by itself
-constexpr int AP_NEAR_FIRST = 64;   // units, where every token has bounds of its own
+constexpr int AP_NEAR_FIRST = 64;   // units, where every token has bounds of its own (6000 packed
+                                    // tokens: 72 us instead of 75 with a kernel of its own)
 // What a unit costs besides its tiles (its first loads, the masked tiles, its rows'
 // way out: 4000 to 8000 clocks), in half tiles of a wide unit (1800 clocks).  With
 // shares of equal tiles alone, CTAs with many short units ended last: a chunked
@@ -62,7 +75,9 @@ constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's
 // much (log2 units): probabilities then reach 2^8, exact in fp32 and within
 // fp16's range, and O is seldom rescaled.
 constexpr float AP_TAU = 8.0f;
-// Of AP_EXP_OF pairs of exponentials, AP_EXP_POLY go to the fp32 pipe.
+// Of AP_EXP_OF pairs of exponentials, AP_EXP_POLY go to the fp32 pipe: the special
+// function unit takes 8 clocks a warp's exponential.  A quarter is the fastest of
+// none, a quarter, a third and a half.
 constexpr int AP_EXP_POLY = 1, AP_EXP_OF = 4;
 
 struct __align__(16) ApUnit {
@@ -708,7 +723,8 @@ DFM_DEV float ap_abs32(const float (&x)[32], float big) {
   return big;
 }
 
-// x += slope e, one instruction a score (e is an immediate): with the row's and the
+// x += slope e, one instruction a score (e is an immediate; in pairs, with e from
+// registers, 6000 packed tokens took 84.6 us instead of 79.8): with the row's and the
 // chunk's shifts, the distance bias.
 DFM_DEV void ap_slope(float (&x)[32], float slope) {
 #pragma unroll
@@ -1114,7 +1130,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           float shift = 0.f, grow = 0.f, top = -INFINITY;
           float xa[32], xb[32];
           auto ld = [&](float (&x)[32], int c) { ap_load(tS + c * 32, x); };
-          bool raw = false, hot = false;   // the cap is left to the second pass
+          bool raw = false, hot = false;   // the cap is left to the second pass; some score passes half of it
           if (!kBias && full) {
             float big = 0.f;
             ld(xa, 0);
@@ -1130,6 +1146,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if (kCap) big = ap_abs32(xb, big);
             }
             if constexpr (kCap) {   // the cap rises with the score: the maximum's is the maximum
+              // (16 trees of 33 to 63 tokens with a cap: 69.5 us instead of 75.4, with the
+              // capped scores stored back and read again)
               raw = true;
               hot = ap_hot(big, p);
               top = ap_cap_one(top, hot, p);

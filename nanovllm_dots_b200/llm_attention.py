@@ -5,7 +5,7 @@ stores each step's K/V with a Triton kernel and attends with flash-attn's
 ``flash_attn_with_kvcache`` (sm_80 FA2).  ``B200DecodeAttention.decode`` is that
 decode branch as one ``dllm_decode_attention`` call on the caller's stream;
 ``install_decode_attention`` routes a reference ``Attention`` module's decode
-steps through it (prefill keeps the module's own path).  There is no CPU path.
+steps through it (prefill keeps the module's own path, or ``llm_append``'s).  There is no CPU path.
 """
 from __future__ import annotations
 
