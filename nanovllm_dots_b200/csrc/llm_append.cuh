@@ -123,8 +123,8 @@ struct ApParams {
   FastDiv by_g, by_unit, by_ctas, by_block;   // G, 2 RT, ctas, block_size
   float scale_log2;                 // scale * log2(e)
   // With a cap (cap_a 0: none): cap_a = scale / cap, cap_b its inverse, cap_in =
-  // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a.
-  float cap_a, cap_b, cap_in, cap_q[3];
+  // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a, taken up to cap_hot.
+  float cap_a, cap_b, cap_in, cap_hot, cap_q[3];
 };
 
 // ---------------------------------------------------------------- plan
@@ -695,7 +695,7 @@ DFM_DEV void ap_exp2_pair(uint64_t x, float& a, float& b) {
 // take three times the products' time.
 constexpr float AP_T0 = 0.999999464f, AP_T1 = -0.33326377f, AP_T2 = 0.131909163f, AP_T3 = -0.0444185946f;
 DFM_DEV bool ap_hot(float big, const ApParams& p) {   // (a NaN is not above the bound and stays one)
-  return __any_sync(0xffffffffu, big * p.cap_a > 0.5f);
+  return __any_sync(0xffffffffu, big * p.cap_a > p.cap_hot);
 }
 DFM_DEV void ap_cap(float (&x)[32], bool hot, const ApParams& p) {
   if (hot) {

@@ -212,6 +212,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   if (!(a->scale > 0.f) || !(a->softcap >= 0.f) || !(a->scale < INFINITY) || !(a->softcap < INFINITY) ||
       a->window < 0)
     return DFM_ERR_INVALID_ARG;
+  if (a->softcap > 0.f && !(a->scale / a->softcap < 1e37f)) return DFM_ERR_UNSUPPORTED;
   if (a->tree_masks && (a->prefix_lens || a->first_keys || a->slopes || a->window))
     return DFM_ERR_UNSUPPORTED;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || reinterpret_cast<uintptr_t>(a->out) % 32 ||
@@ -225,7 +226,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   if (a->tokens == 0) return DFM_OK;
   // places in the line of key tiles are 32-bit
   const long long tiles = static_cast<long long>(a->max_blocks) * a->block_size / AP_KT + 2 + AP_WIDE_COST;
-  if (2 * tiles * ap_max_units(a->tokens, a->n, RT) > 0x7fffffffll / a->num_kv_heads - 2 * ctas)
+  if (2 * tiles * ap_max_units(a->tokens, a->n, RT) > 0x3fffffffll / a->num_kv_heads)
     return DFM_ERR_UNSUPPORTED;
   int rows = AP_KT;
   while (a->block_size % rows) rows /= 2;
@@ -277,6 +278,8 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
     p.cap_a = a->scale / a->softcap;
     p.cap_b = a->softcap / a->scale;
     p.cap_in = 2.f * log2e * p.cap_a;
+    // (the powers of a cap_a above 10^6 would overflow: no polynomial)
+    p.cap_hot = p.cap_a > 1e6f ? -1.f : 0.5f;
     const float z = p.cap_a * p.cap_a;
     p.cap_q[0] = AP_T1 * z;
     p.cap_q[1] = AP_T2 * z * z;

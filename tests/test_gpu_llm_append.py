@@ -355,6 +355,23 @@ def test_cap_of_unmasked_tiles(cap, D):
     run(Case([(30, 900), (1, 1100), (70, 600)], D=D, softcap=cap, spread=2.0))
 
 
+@pytest.mark.parametrize("spread", [0.0, 1.0])
+def test_cap_far_below_the_scores(spread):
+    """Every score is capped to nothing: the mean of V, also where the scores are zero."""
+    run(Case([(30, 900), (1, 100)], softcap=1e-8, spread=spread))
+
+
+@pytest.mark.parametrize("n", [3, 300])
+def test_no_sequence_has_tokens(n):
+    c = Case([(2, 30)] + [(0, 20)] * (n - 1)).device()
+    att = c.attention()
+    c.cud.zero_()
+    out = torch.full_like(c.qd, 3.0)
+    c.call(att, out=out)
+    att.check_errors()
+    assert (out == 3.0).all()
+
+
 def test_bad_block_id_is_reported_and_read_as_zeros():
     c = Case([(5, 600), (3, 20)])
     c.device()

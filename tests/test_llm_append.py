@@ -93,7 +93,8 @@ def append(ws=1 << 12, size=1 << 30, **over):
     (dict(block_size=1 << 16, max_blocks=1 << 15), UNSUPPORTED),
     (dict(num_blocks=0), INVALID), (dict(max_blocks=0), INVALID), (dict(scale=0.0), INVALID),
     (dict(scale=math.nan), INVALID), (dict(scale=math.inf), INVALID), (dict(softcap=-1.0), INVALID),
-    (dict(softcap=math.nan), INVALID), (dict(window=-1), INVALID), (dict(q_token_stride=1540), INVALID),
+    (dict(softcap=math.nan), INVALID), (dict(softcap=1e-39), UNSUPPORTED), (dict(window=-1), INVALID),
+    (dict(max_blocks=1 << 22, tokens=100000, size=1 << 40), UNSUPPORTED), (dict(q_token_stride=1540), INVALID),
     (dict(q_head_stride=4), INVALID), (dict(q_head_stride=64), INVALID), (dict(q_token_stride=0), INVALID),
     (dict(q_head_stride=-128), INVALID), (dict(q=A + 2), INVALID), (dict(k_cache=A + 8), INVALID),
     (dict(out=A + 8), INVALID), (dict(tree_masks=A, slopes=A), UNSUPPORTED),
