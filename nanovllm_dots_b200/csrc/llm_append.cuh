@@ -50,6 +50,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace dfm {
@@ -125,6 +127,7 @@ struct ApParams {
   // With a cap (cap_a 0: none): cap_a = scale / cap, cap_b its inverse, cap_in =
   // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a, taken up to cap_hot.
   float cap_a, cap_b, cap_in, cap_hot, cap_q[3];
+  float cap_y[4];                   // the polynomial times scale_log2
 };
 
 // ---------------------------------------------------------------- plan
@@ -712,8 +715,7 @@ DFM_DEV void ap_cap(float (&x)[32], bool hot, const ApParams& p) {
     f2_split(f2_mul(y, f2_fma(f2_fma(f2_fma(q3, z, q2), z, q1), z, q0)), x[e], x[e + 1]);
   }
 }
-DFM_DEV float ap_cap_one(float x, bool hot, const ApParams& p) {
-  if (hot) return fmaf(-2.f * p.cap_b, __fdividef(1.f, 1.f + fast_exp2(x * p.cap_in)), p.cap_b);
+DFM_DEV float ap_cap_one(float x, const ApParams& p) {   // below half the cap
   const float z = x * x;
   return x * fmaf(fmaf(fmaf(p.cap_q[2], z, p.cap_q[1]), z, p.cap_q[0]), z, AP_T0);
 }
@@ -1123,15 +1125,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         const bool full = k0 >= sg.f.fmin && k0 + AP_KT <= sg.f.fmax;
         if (warp_valid) {
           // Two passes over the row's 128 scores in TMEM, 32 at a time so that the
-          // code stays small: the maximum (with a cap, a bias or masks, the
-          // changed scores x go back to TMEM), then the probabilities.
-          // x scale + shift is the score in log2 units.
-          // (and chunk c's 32 keys are c grow further on).
+          // code stays small: the maximum, then the probabilities.  With masks, a bias or
+          // scores near the cap, the changed scores x go back to TMEM in between; a cap
+          // far above a whole tile's scores is a polynomial in the second pass.
+          // x scale + shift is the score in log2 units (with a bias, chunk c's 32 keys are
+          // c grow further on).
           float shift = 0.f, grow = 0.f, top = -INFINITY;
           float xa[32], xb[32];
           auto ld = [&](float (&x)[32], int c) { ap_load(tS + c * 32, x); };
-          bool raw = false, hot = false;   // the cap is left to the second pass; some score passes half of it
-          if (!kBias && full) {
+          bool stored = kBias || !full, raw = false;   // raw: the cap is left to the second pass
+          if (!stored) {
             float big = 0.f;
             ld(xa, 0);
 #pragma unroll 1
@@ -1146,13 +1149,14 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if (kCap) big = ap_abs32(xb, big);
             }
             if constexpr (kCap) {   // the cap rises with the score: the maximum's is the maximum
-              // (16 trees of 33 to 63 tokens with a cap: 69.5 us instead of 75.4, with the
-              // capped scores stored back and read again)
-              raw = true;
-              hot = ap_hot(big, p);
-              top = ap_cap_one(top, hot, p);
+              // (16 trees of 33 to 63 tokens with a cap: 62.4 us; 75.4 with the capped scores
+              // stored back and read again)
+              raw = !ap_hot(big, p);
+              stored = !raw;
+              top = raw ? ap_cap_one(top, p) : -INFINITY;
             }
-          } else {
+          }
+          if (stored) {
             const bool behind = k0 + AP_KT - 1 <= pos || (p.causal && !p.prefix);
             if (kBias && behind) {
               shift = -slope * p.scale_log2 * static_cast<float>(pos - k0);
@@ -1237,43 +1241,58 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           grow *= p.scale_log2;
           uint64_t sum0 = f2(0.f, 0.f), sum1 = f2(0.f, 0.f);
           uint32_t pk[32];
-          auto probabilities = [&](const float (&x)[32], int at, int c) {
-            const float mc = kBias ? fmaf(grow, static_cast<float>(c), ms) : ms;
-            const uint64_t sh = f2(mc, mc);
+          auto second_pass = [&](auto capped) {
+            constexpr bool kRaw = decltype(capped)::value;
+            uint64_t y0, y1, y2, y3;
+            if constexpr (kRaw) {
+              y0 = f2(p.cap_y[0], p.cap_y[0]), y1 = f2(p.cap_y[1], p.cap_y[1]);
+              y2 = f2(p.cap_y[2], p.cap_y[2]), y3 = f2(p.cap_y[3], p.cap_y[3]);
+            }
+            auto probabilities = [&](const float (&x)[32], int at, int c) {
+              const float mc = kBias ? fmaf(grow, static_cast<float>(c), ms) : ms;
+              const uint64_t sh = f2(mc, mc);
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float a, b;
-              const uint64_t y = f2_fma(f2(x[e], x[e + 1]), sc, sh);
-              if ((e >> 1) % AP_EXP_OF < AP_EXP_POLY) {
-                ap_exp2_pair(y, a, b);
-              } else {
-                f2_split(y, a, b);
-                a = fast_exp2(a);
-                b = fast_exp2(b);
+              for (int e = 0; e < 32; e += 2) {
+                float a, b;
+                const uint64_t v = f2(x[e], x[e + 1]);
+                uint64_t y;
+                if constexpr (kRaw) {
+                  const uint64_t z = f2_mul(v, v);
+                  y = f2_fma(v, f2_fma(f2_fma(f2_fma(y3, z, y2), z, y1), z, y0), sh);
+                } else {
+                  y = f2_fma(v, sc, sh);
+                }
+                if ((e >> 1) % AP_EXP_OF < AP_EXP_POLY) {
+                  ap_exp2_pair(y, a, b);
+                } else {
+                  f2_split(y, a, b);
+                  a = fast_exp2(a);
+                  b = fast_exp2(b);
+                }
+                if (e & 2) sum1 = f2_add(sum1, f2(a, b));
+                else sum0 = f2_add(sum0, f2(a, b));
+                pk[at + (e >> 1)] = ap_pack<kFp16>(a, b);
               }
-              if (e & 2) sum1 = f2_add(sum1, f2(a, b));
-              else sum0 = f2_add(sum0, f2(a, b));
-              pk[at + (e >> 1)] = ap_pack<kFp16>(a, b);
+            };
+            ld(xa, 0);
+            // (P's chunks lie on scores that have been read)
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              ap_landed(xa);
+              ld(xb, 2 * h + 1);
+              probabilities(xa, 0, 2 * h);
+              ap_landed(xb);
+              if (h == 0) ld(xa, 2);
+              probabilities(xb, 16, 2 * h + 1);
+              tmem_st32(tS + h * 32, pk);
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
             }
           };
-          ld(xa, 0);
-          // (P's chunks lie on scores that have been read)
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            ap_landed(xa);
-            ld(xb, 2 * h + 1);
-            if (kCap && raw) ap_cap(xa, hot, p);
-            probabilities(xa, 0, 2 * h);
-            ap_landed(xb);
-            if (h == 0) ld(xa, 2);
-            if (kCap && raw) ap_cap(xb, hot, p);
-            probabilities(xb, 16, 2 * h + 1);
-            tmem_st32(tS + h * 32, pk);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
-          }
+          if (kCap && raw) second_pass(std::integral_constant<bool, kCap>{});
+          else second_pass(std::false_type{});
           float a, b;
           f2_split(f2_add(sum0, sum1), a, b);
           l += a + b;

@@ -284,6 +284,8 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
     p.cap_q[0] = AP_T1 * z;
     p.cap_q[1] = AP_T2 * z * z;
     p.cap_q[2] = AP_T3 * z * z * z;
+    p.cap_y[0] = AP_T0 * p.scale_log2;
+    for (int i = 0; i < 3; ++i) p.cap_y[i + 1] = p.cap_q[i] * p.scale_log2;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool cap = a->softcap > 0.f, bias = a->slopes != nullptr, fp16 = a->dtype == DLLM_FP16;
