@@ -69,8 +69,9 @@ constexpr int AP_NEAR_FIRST = 64;   // units, where every token has bounds of it
 // What a unit costs besides its tiles (its first loads, the masked tiles, its rows'
 // way out: 4000 to 8000 clocks), in half tiles of a wide unit (1800 clocks).  With
 // shares of equal tiles alone, CTAs with many short units ended last: a chunked
-// prefill of 24 sequences took 62.0 us and now 49.1, 64 single tokens 30.4 and 28.7,
-// 64 small trees 30.1 and 28.3; 2 / 4 and 3 / 4 are equal, 1 / 3 and 3 / 6 slower.
+// prefill of 24 sequences took 62.0 us instead of 49.2, 64 single tokens 30.4 instead
+// of 28.7, 64 small trees 30.1 instead of 28.3; 2 / 4 and 3 / 4 are equal, 1 / 3 and
+// 3 / 6 slower.
 constexpr int AP_NARROW_COST = 3, AP_WIDE_COST = 4;
 constexpr int AP_MIN_SHARE = 2;     // smallest share of the line (a wide unit's key tile counts 2)
 // The running maximum of a row is raised only when a score passes it by this
