@@ -1,5 +1,5 @@
 """CPU oracle for the LLM's rotary, append attention and tree verification --
-TEST INFRASTRUCTURE ONLY: tests use it as the checker, the product path never
+TEST INFRASTRUCTURE ONLY: tests compare the kernels with it, the product path never
 imports it.
 
 Everything is in float64 from the definitions in ``include/dllm.h``.  Beside the
