@@ -100,10 +100,11 @@ class B200AppendAttention:
 
     def _run(self, q, k_cache, v_cache, cu, ctx, table, prefix, first, tree, out, stream):
         H, D, index, dtype = self.num_heads, self.head_dim, self._index, self.dtype
-        if q.dim() != 3 or q.shape[1] != H or q.shape[2] != D or q.dtype is not dtype or q.get_device() != index:
+        shape, rows, seqs = q.shape, table.shape, ctx.shape
+        if len(shape) != 3 or shape[1] != H or shape[2] != D or q.dtype is not dtype or q.get_device() != index:
             raise RuntimeError(f"q: expected a {dtype} tensor [tokens, {H}, {D}] on {self.device}, "
-                               f"got {q.dtype} {tuple(q.shape)} on {q.device}")
-        T, n = q.shape[0], ctx.shape[0] if ctx.dim() else 0
+                               f"got {q.dtype} {tuple(shape)} on {q.device}")
+        T, n = shape[0], seqs[0] if seqs else 0
         if T > self.max_tokens or not 1 <= n <= self.max_seqs:
             raise RuntimeError(f"append of {T} tokens of {n} sequences "
                                f"(at most {self.max_tokens} of {self.max_seqs})")
@@ -116,7 +117,7 @@ class B200AppendAttention:
                     geometry[0] < 1 or not c.is_contiguous():
                 raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor [num_blocks, "
                                    f"{', '.join(map(str, geometry[1:]))}] on {self.device}, both caches alike")
-        if table.dim() != 2 or not 1 <= table.shape[1] <= self.max_blocks:
+        if len(rows) != 2 or not 1 <= rows[1] <= self.max_blocks:
             raise RuntimeError(f"block_tables: expected [{n}, 1..{self.max_blocks}]")
         if out is None:
             if stream is None:
@@ -131,7 +132,7 @@ class B200AppendAttention:
             raise RuntimeError("out: expected 32-byte alignment")
         elif overlap(q, out) and not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):
             raise RuntimeError("out: overlaps q without being q")
-        i32, width = torch.int32, table.shape[1]
+        i32, width = torch.int32, rows[1]
         plain = tree is None
         a = _pack(
             self._dtype, T, n, H, self.num_kv_heads, D, geometry[0], self.block_size, width, self.causal,

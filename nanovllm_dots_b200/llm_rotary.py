@@ -131,18 +131,18 @@ class B200Rotary:
 
     def _heads(self, name, t, dtype, tokens):
         """[tokens, heads, head_dim] with contiguous head dims -> its heads and strides."""
-        if t.dim() != 3 or t.shape[2] != self.head_dim or t.get_device() != self._index:
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or t.get_device() != self._index:
             raise RuntimeError(f"{name}: expected [tokens, heads, {self.head_dim}] on {self.device}, "
-                               f"got {tuple(t.shape)} on {t.device}")
+                               f"got {tuple(shape)} on {t.device}")
         if t.dtype is not dtype:
             raise RuntimeError(f"{name}: expected {dtype}, got {t.dtype}")
-        n, heads, _ = t.shape
-        if n != tokens:
-            raise RuntimeError(f"{name}: expected {tokens} tokens, got {n}")
+        if shape[0] != tokens:
+            raise RuntimeError(f"{name}: expected {tokens} tokens, got {shape[0]}")
         ts, hs, one = t.stride()
         if one != 1:
             raise RuntimeError(f"{name}: expected contiguous head dims")
-        return heads, ts, hs
+        return shape[1], ts, hs
 
     def _ints(self, name, t, tokens):
         if t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (tokens,) or \
@@ -183,11 +183,11 @@ class B200Rotary:
             if kvh != vheads or kvh < 1:
                 raise RuntimeError("k and v have different heads, or none")
             places = self._ints("slot_mapping", slot_mapping, T)
-            shape = k_cache.shape
+            shape, cache_type = k_cache.shape, q.dtype
+            good = len(shape) == 4 and shape[0] and shape[1] and shape[2] == kvh and shape[3] == self.head_dim
             for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-                if c.dtype is not q.dtype or c.get_device() != self._index or c.dim() != 4 or \
-                        c.shape != shape or shape[2] != kvh or shape[3] != self.head_dim or \
-                        not c.is_contiguous() or not c.numel():
+                if not good or c.dtype is not cache_type or c.get_device() != self._index or \
+                        c.shape != shape or not c.is_contiguous():
                     raise RuntimeError(f"{name}: expected a contiguous {q.dtype} [num_blocks, block_size, "
                                        f"{kvh}, {self.head_dim}] on {self.device}, and both caches alike")
             slots = shape[0] * shape[1]
