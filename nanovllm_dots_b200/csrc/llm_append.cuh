@@ -1220,14 +1220,17 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             tmem_wait_st();
           }
           const float mt = fmaf(top, p.scale_log2, shift);
+          // Each row raises its maximum by its own scores alone, so that its result does
+          // not depend on the rows beside it: of other tokens, and past the unit's last
+          // token on the next sequence's queries or, past RT G, on what the shared memory held.
+          const bool raise = valid && mt > m + AP_TAU;
           if (i == i_first) {
             m = mt;
-          } else if (__any_sync(0xffffffffu, mt > m + AP_TAU)) {
+          } else if (__any_sync(0xffffffffu, raise)) {
             // the stream's last product is done: this tile's scores came after it
-            const float mn = fmaxf(m, mt);
-            const float a = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+            const float a = raise ? fast_exp2(m - mt) : 1.f;
             l *= a;
-            m = mn;
+            m = raise ? mt : m;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               ap_load(tO + s * D + c, xb);

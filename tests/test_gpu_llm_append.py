@@ -474,3 +474,42 @@ def test_offsets_past_32_bits():
     att = c.attention()
     assert torch.equal(c.call(att), want)
     att.check_errors()
+
+
+# Bit-for-bit tests: enough sequences that a share has several key tiles of a unit, over
+# which a row's maximum rises, by less and by more than what is put off.
+MANY = [(9, 1900), (3, 2000), (1, 1800), (60, 1500)] * 12
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("opts", [dict(), dict(slopes=True), dict(tree=True)])
+def test_a_row_depends_on_its_own_query_alone(opts, D):
+    """Queries of other tokens of the sequence, and of the sequence packed behind it,
+    whose rows fill up the row tile, have no say."""
+    kw = dict(slopes=slopes_of(12)) if "slopes" in opts else \
+        dict(tree=trees(MANY, 4)) if "tree" in opts else {}
+    c = Case(MANY, D=D, **kw)
+    att = c.attention()
+    want, q = c.device().call(att), c.q
+    r = random.Random(D)
+    for by in (8.0, 0.0, 30.0, 0.01):
+        rows = [t for t in range(q.shape[0]) if r.random() < 0.3]
+        c.q = q.clone()
+        c.q[rows] *= by
+        others = torch.ones(q.shape[0], dtype=torch.bool)
+        others[rows] = False
+        assert torch.equal(c.device().call(att).cpu()[others], want.cpu()[others])
+
+
+def test_what_the_shared_memory_held_has_no_say():
+    """Six heads to a kv head are 126 rows of 128: the last two hold what was there, here
+    queries of another call's, large and small."""
+    c = Case([(21, 1900), (42, 1700), (20, 2100)] * 12).device()
+    att = c.attention()
+    want = c.call(att)
+    fill = Case([(64, 1200)] * 8, 2, 2).device()
+    other, q = fill.attention(), fill.qd
+    for by in (60.0, 1e-3, 0.0, 8.0):
+        fill.qd = q * by
+        fill.call(other)
+        assert torch.equal(c.call(att), want)
