@@ -199,9 +199,9 @@ size_t dllm_append_workspace_size(int32_t tokens, int32_t n, int32_t num_heads,
 /* Stream ordered, no allocation, no host synchronisation; the launches depend
  * on the arguments but not on the lengths in device memory.  Block tables of
  * nearly 2^31 positions, or of more key tiles in all than 30 bits count, and a
- * softcap below 1e-37 scale are refused (DFM_ERR_UNSUPPORTED).  Lengths that make no sense, a block id out of
- * range or a tree of more than 64 tokens set a device error bit
- * (dllm_read_error); such a sequence's rows are zeros, or untouched where
+ * softcap below 1e-37 scale or above 1e18 scale are refused
+ * (DFM_ERR_UNSUPPORTED).  Lengths that make no sense, a block id out of range
+ * or a tree of more than 64 tokens set a device error bit (dllm_read_error); such a sequence's rows are zeros, or untouched where
  * cu_seqlens_q itself is wrong, and such a block reads as zeros. */
 int dllm_append_attention(const DllmAppend* args, void* workspace, size_t workspace_bytes,
                           void* stream);

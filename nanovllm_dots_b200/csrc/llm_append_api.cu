@@ -212,7 +212,9 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   if (!(a->scale > 0.f) || !(a->softcap >= 0.f) || !(a->scale < INFINITY) || !(a->softcap < INFINITY) ||
       a->window < 0)
     return DFM_ERR_INVALID_ARG;
-  if (a->softcap > 0.f && !(a->scale / a->softcap < 1e37f)) return DFM_ERR_UNSUPPORTED;
+  // (beyond these bounds the cap's constants, or the square of a score below it, leave fp32)
+  if (a->softcap > 0.f && !(a->scale / a->softcap < 1e37f && a->scale / a->softcap > 1e-18f))
+    return DFM_ERR_UNSUPPORTED;
   if (a->tree_masks && (a->prefix_lens || a->first_keys || a->slopes || a->window))
     return DFM_ERR_UNSUPPORTED;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || reinterpret_cast<uintptr_t>(a->out) % 32 ||
@@ -278,8 +280,11 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
     p.cap_a = a->scale / a->softcap;
     p.cap_b = a->softcap / a->scale;
     p.cap_in = 2.f * log2e * p.cap_a;
-    // (the powers of a cap_a above 10^6 would overflow: no polynomial)
-    p.cap_hot = p.cap_a > 1e6f ? -1.f : 0.5f;
+    // The powers of a cap_a above 10^6 would overflow: no polynomial.  Those of one below
+    // 10^-6 vanish, up to 0.0075 of a score near half the cap: the polynomial only where
+    // they do not count (0.02^4 of the score), and above it 1 - 2 / (1 + e^2y), whose
+    // error of 10^-7 caps is then 5e-6 of the score.
+    p.cap_hot = p.cap_a > 1e6f ? -1.f : p.cap_a < 1e-6f ? 0.02f : 0.5f;
     const float z = p.cap_a * p.cap_a;
     p.cap_q[0] = AP_T1 * z;
     p.cap_q[1] = AP_T2 * z * z;

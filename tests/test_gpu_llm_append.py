@@ -513,3 +513,24 @@ def test_what_the_shared_memory_held_has_no_say():
         fill.qd = q * by
         fill.call(other)
         assert torch.equal(c.call(att), want)
+
+
+@pytest.mark.parametrize("ctx", [40, 1500])
+@pytest.mark.parametrize("cap", [1e-3, 1.0, 1e5])
+def test_caps_far_above_the_scale(ctx, cap):
+    """Queries and keys of 60000 under a small scale: scores near 0.46 caps, where tanh's
+    higher terms count (the cap in units of the raw product is 10^12).  Half of the keys
+    have positive scores and values of 1, half negative ones and zeros."""
+    scale = cap * 1e-12
+    q = torch.full((3, 2, 128), 6e4, dtype=FP)
+    sign = torch.where(torch.arange(ctx) % 2 == 0, 1.0, -1.0)
+    K = (sign * 6e4)[:, None, None].expand(ctx, 2, 128).to(FP).contiguous()
+    V = (sign > 0).to(FP)[:, None, None].expand(ctx, 2, 128).contiguous()
+    att = B200AppendAttention(2, 128, scale, 2, max_tokens=3, max_seqs=1, max_blocks=1, block_size=1536,
+                              dtype=FP, softcap=cap, device=DEV)
+    pages = torch.zeros(2, 1, 1536, 2, 128, dtype=FP, device=DEV)
+    pages[0, 0, :ctx], pages[1, 0, :ctx] = K.to(DEV), V.to(DEV)
+    d = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    got = att.append(q.to(DEV), pages[0], pages[1], d(0, 3), d(ctx), d(0)[None])
+    att.check_errors()
+    check(got, *O.attend(q, K, V, O.visible(3, ctx), scale, cap))

@@ -106,6 +106,14 @@ def test_append_refusals(over, code):
     assert append(**over) == code
 
 
+@pytest.mark.parametrize("scale,softcap,code", [
+    (0.1, 1e16, OK), (0.1, 1e18, UNSUPPORTED), (0.1, 3e38, UNSUPPORTED), (1e-30, 1e15, UNSUPPORTED),
+    (1e-20, 3e38, UNSUPPORTED), (1e-12, 1.0, OK)])
+def test_append_refuses_caps_beyond_its_arithmetic(scale, softcap, code):
+    """The square of a score below the cap, and the cap's constants, have to fit fp32."""
+    assert append(scale=scale, softcap=softcap, tokens=0) == code
+
+
 def test_append_workspace_size():
     size = _lib.lib().dllm_append_workspace_size
     assert size(8, 2, 12, 2, 128) > size(8, 2, 12, 2, 64) > 0
