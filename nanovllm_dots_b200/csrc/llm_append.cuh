@@ -126,7 +126,7 @@ struct ApParams {
   FastDiv by_g, by_unit, by_ctas, by_block;   // G, 2 RT, ctas, block_size
   float scale_log2;                 // scale * log2(e)
   // With a cap (cap_a 0: none): cap_a = scale / cap, cap_b its inverse, cap_in =
-  // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a, taken up to cap_hot.
+  // 2 log2(e) cap_a and tanh's polynomial in powers of cap_a, taken up to |q.k| = cap_hot.
   float cap_a, cap_b, cap_in, cap_hot, cap_q[3];
   float cap_y[4];                   // the polynomial times scale_log2
 };
@@ -690,31 +690,74 @@ DFM_DEV void ap_exp2_pair(uint64_t x, float& a, float& b) {
   f2_split(q, a, b);
 }
 
-// x = (cap / scale) tanh(S scale / cap) of 32 scores of a row (x scale is the
-// capped score).  Where every score of the warp's chunk is below half the cap,
-// tanh y = y q(y^2) with q the cubic fitted at Chebyshev nodes of [0, 1/4] (6e-7
-// relative), its coefficients scaled so that x = S q(S^2): 2.5 instructions a score
-// on the fp32 pipe.  Else 1 - 2 / (1 + e^{2y}): two special-function operations,
-// of which an SM does 16 a clock, so that they and the softmax's exponential would
-// take three times the products' time.
-constexpr float AP_T0 = 0.999999464f, AP_T1 = -0.33326377f, AP_T2 = 0.131909163f, AP_T3 = -0.0444185946f;
-DFM_DEV bool ap_hot(float big, const ApParams& p) {   // (a NaN is not above the bound and stays one)
-  return __any_sync(0xffffffffu, big * p.cap_a > p.cap_hot);
+DFM_DEV float ap_max32(const float (&x)[32], float top) {
+  float t0 = top, t1 = x[0];
+#pragma unroll
+  for (int e = 1; e < 31; e += 2) {
+    t0 = fmaxf(t0, x[e]);
+    t1 = fmaxf(t1, x[e + 1]);
+  }
+  return fmaxf(fmaxf(t0, t1), x[31]);
 }
-DFM_DEV void ap_cap(float (&x)[32], bool hot, const ApParams& p) {
-  if (hot) {
+
+// The cap: x = (cap / scale) tanh(S scale / cap) of a raw score S (x scale is the
+// capped score).  Below half the cap, tanh y = y q(y^2) with q the cubic fitted at
+// Chebyshev nodes of [0, 1/4] (6e-7 relative), its coefficients scaled so that x = S
+// q(S^2): 2.5 instructions a score on the fp32 pipe.  From there on 1 - 2 / (1 + e^{2y}),
+// 10^-7 caps off: two special-function operations, of which an SM does 16 a clock,
+// so that they and the softmax's exponential would take three times the products' time.
+// Which of the two counts is a score's own matter in tiles with masks or a bias and
+// a row's own in the others, so that no other row, and no key that the row does not
+// see, has a say in its result.
+constexpr float AP_T0 = 0.999999464f, AP_T1 = -0.33326377f, AP_T2 = 0.131909163f, AP_T3 = -0.0444185946f;
+DFM_DEV bool ap_far(float big, const ApParams& p) {   // (a NaN is not above the bound and stays one)
+  return big > p.cap_hot;
+}
+DFM_DEV uint64_t ap_cap_near(uint64_t y, const ApParams& p) {
+  const uint64_t z = f2_mul(y, y);
+  return f2_mul(y, f2_fma(f2_fma(f2_fma(f2(p.cap_q[2], p.cap_q[2]), z, f2(p.cap_q[1], p.cap_q[1])), z,
+                                 f2(p.cap_q[0], p.cap_q[0])), z, f2(AP_T0, AP_T0)));
+}
+DFM_DEV float ap_cap_far(float x, const ApParams& p) {
+  float t;   // (volatile: computed for every row, a branch around it costs more)
+  asm volatile("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(1.f + fast_exp2(x * p.cap_in)));
+  return fmaf(-2.f * p.cap_b, t, p.cap_b);
+}
+DFM_DEV void ap_cap(float (&x)[32], const ApParams& p) {   // none of the warp's is past the bound
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      x[e] = fmaf(-2.f * p.cap_b, __fdividef(1.f, 1.f + fast_exp2(x[e] * p.cap_in)), p.cap_b);
-    return;
-  }
-  const uint64_t q3 = f2(p.cap_q[2], p.cap_q[2]), q2 = f2(p.cap_q[1], p.cap_q[1]), q1 = f2(p.cap_q[0], p.cap_q[0]),
-                 q0 = f2(AP_T0, AP_T0);
+  for (int e = 0; e < 32; e += 2) f2_split(ap_cap_near(f2(x[e], x[e + 1]), p), x[e], x[e + 1]);
+}
+// Where some of the warp's scores are past the bound: 64 scores in TMEM, capped each
+// its way (kRows false), or those of the rows that are `far` alone, with the row's largest
+// as the result.  (Calls, so that the kernel's other paths have its registers: inlined
+// they spilled, and 16 trees of 33 to 63 tokens with a cap far above their scores
+// took 70.9 us instead of 63.5.)
+template <bool kRows>
+__device__ __noinline__ float ap_cap_some(uint32_t taddr, bool far, const ApParams& p) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 64; c += 32) {
+    float x[32];
+    ap_load(taddr + c, x);
+    ap_landed(x);
 #pragma unroll
-  for (int e = 0; e < 32; e += 2) {
-    const uint64_t y = f2(x[e], x[e + 1]), z = f2_mul(y, y);
-    f2_split(f2_mul(y, f2_fma(f2_fma(f2_fma(q3, z, q2), z, q1), z, q0)), x[e], x[e + 1]);
+    for (int e = 0; e < 32; e += 2) {
+      const float fa = ap_cap_far(x[e], p), fb = ap_cap_far(x[e + 1], p);
+      if (kRows) {
+        x[e] = far ? fa : x[e];
+        x[e + 1] = far ? fb : x[e + 1];
+      } else {
+        float a, b;
+        f2_split(ap_cap_near(f2(x[e], x[e + 1]), p), a, b);
+        x[e] = ap_far(fabsf(x[e]), p) ? fa : a;
+        x[e + 1] = ap_far(fabsf(x[e + 1]), p) ? fb : b;
+      }
+    }
+    if (kRows) top = ap_max32(x, top);
+    tmem_st32(taddr + c, reinterpret_cast<uint32_t(&)[32]>(x));
   }
+  tmem_wait_st();
+  return top;
 }
 DFM_DEV float ap_cap_one(float x, const ApParams& p) {   // below half the cap
   const float z = x * x;
@@ -746,16 +789,6 @@ DFM_DEV void ap_mask(float (&x)[32], uint32_t see) {
   for (int e = 0; e < 32; ++e) x[e] = (see >> e) & 1 ? x[e] : -INFINITY;
 }
 
-DFM_DEV float ap_max32(const float (&x)[32], float top) {
-  float t0 = top, t1 = x[0];
-#pragma unroll
-  for (int e = 1; e < 31; e += 2) {
-    t0 = fmaxf(t0, x[e]);
-    t1 = fmaxf(t1, x[e + 1]);
-  }
-  return fmaxf(fmaxf(t0, t1), x[31]);
-}
-
 // ---------------------------------------------------------------- the kernel
 // A cap and a distance bias on the scores have kernels of their own: what only they
 // need costs the others registers.
@@ -764,7 +797,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     llm_append_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ApParams p) {
   using S = ApSmem<D>;
-  constexpr bool kMod = kCap || kBias;
+  constexpr bool kMod = kCap || kBias, kLateCap = kCap && !kBias;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -1127,14 +1160,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (warp_valid) {
           // Two passes over the row's 128 scores in TMEM, 32 at a time so that the
           // code stays small: the maximum, then the probabilities.  With masks, a bias or
-          // scores near the cap, the changed scores x go back to TMEM in between; a cap
-          // far above a whole tile's scores is a polynomial in the second pass.
+          // scores near the cap, the changed scores x go back to TMEM in between; in a tile
+          // without masks a row far below the cap leaves it to the second pass, as a polynomial.
           // x scale + shift is the score in log2 units (with a bias, chunk c's 32 keys are
           // c grow further on).
           float shift = 0.f, grow = 0.f, top = -INFINITY;
           float xa[32], xb[32];
           auto ld = [&](float (&x)[32], int c) { ap_load(tS + c * 32, x); };
-          bool stored = kBias || !full, raw = false;   // raw: the cap is left to the second pass
+          bool stored = kBias || !full;
+          bool raw = false, some_raw = false;   // this row, some row leaves its cap to the second pass
+          float near_top = 0.f;
           if (!stored) {
             float big = 0.f;
             ld(xa, 0);
@@ -1150,11 +1185,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if (kCap) big = ap_abs32(xb, big);
             }
             if constexpr (kCap) {   // the cap rises with the score: the maximum's is the maximum
-              // (16 trees of 33 to 63 tokens with a cap: 62.4 us; 75.4 with the capped scores
+              // (16 trees of 33 to 63 tokens with a cap: 63.5 us; 75.4 with the capped scores
               // stored back and read again)
-              raw = !ap_hot(big, p);
-              stored = !raw;
-              top = raw ? ap_cap_one(top, p) : -INFINITY;
+              raw = !ap_far(big, p);
+              stored = __any_sync(0xffffffffu, valid && !raw);
+              some_raw = __any_sync(0xffffffffu, valid && raw);
+              near_top = ap_cap_one(top, p);
+              top = -INFINITY;
             }
           }
           if (stored) {
@@ -1174,14 +1211,25 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 tmem_st32(tS + c + 32, reinterpret_cast<uint32_t(&)[32]>(xa));
                 continue;
               }
+              if (kLateCap && full) {
+                top = fmaxf(top, ap_cap_some<true>(tS + c, !raw, p));
+                continue;
+              }
               ap_load(tS + c, xa);
               ap_load(tS + c + 32, xb);
               ap_landed(xa);
               ap_landed(xb);
               if constexpr (kCap) {
-                const bool h = ap_hot(ap_abs32(xa, ap_abs32(xb, 0.f)), p);
-                ap_cap(xa, h, p);
-                ap_cap(xb, h, p);
+                if (__any_sync(0xffffffffu, ap_far(ap_abs32(xa, ap_abs32(xb, 0.f)), p))) {
+                  ap_cap_some<false>(tS + c, false, p);
+                  ap_load(tS + c, xa);
+                  ap_load(tS + c + 32, xb);
+                  ap_landed(xa);
+                  ap_landed(xb);
+                } else {
+                  ap_cap(xa, p);
+                  ap_cap(xb, p);
+                }
               }
               if constexpr (kBias) {
                 if (behind) {   // every key the row sees is at or before it: |p - k| = (p - k0) - c
@@ -1219,6 +1267,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
             tmem_wait_st();
           }
+          if (raw) top = near_top;
           const float mt = fmaf(top, p.scale_log2, shift);
           // Each row raises its maximum by its own scores alone, so that its result does
           // not depend on the rows beside it: of other tokens, and past the unit's last
@@ -1245,12 +1294,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           grow *= p.scale_log2;
           uint64_t sum0 = f2(0.f, 0.f), sum1 = f2(0.f, 0.f);
           uint32_t pk[32];
-          auto second_pass = [&](auto capped) {
-            constexpr bool kRaw = decltype(capped)::value;
+          // kind 1: every score takes the cap's polynomial; 2: those of rows that are raw;
+          // 0: none
+          auto second_pass = [&](auto kind) {
+            constexpr int kLate = decltype(kind)::value;
             uint64_t y0, y1, y2, y3;
-            if constexpr (kRaw) {
-              y0 = f2(p.cap_y[0], p.cap_y[0]), y1 = f2(p.cap_y[1], p.cap_y[1]);
-              y2 = f2(p.cap_y[2], p.cap_y[2]), y3 = f2(p.cap_y[3], p.cap_y[3]);
+            if constexpr (kLate > 0) {
+              const bool q = kLate == 1 || raw;
+              const float c0 = q ? p.cap_y[0] : p.scale_log2, c1 = q ? p.cap_y[1] : 0.f,
+                          c2 = q ? p.cap_y[2] : 0.f, c3 = q ? p.cap_y[3] : 0.f;
+              y0 = f2(c0, c0), y1 = f2(c1, c1), y2 = f2(c2, c2), y3 = f2(c3, c3);
             }
             auto probabilities = [&](const float (&x)[32], int at, int c) {
               const float mc = kBias ? fmaf(grow, static_cast<float>(c), ms) : ms;
@@ -1260,7 +1313,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 float a, b;
                 const uint64_t v = f2(x[e], x[e + 1]);
                 uint64_t y;
-                if constexpr (kRaw) {
+                if constexpr (kLate > 0) {
                   const uint64_t z = f2_mul(v, v);
                   y = f2_fma(v, f2_fma(f2_fma(f2_fma(y3, z, y2), z, y1), z, y0), sh);
                 } else {
@@ -1295,8 +1348,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
             }
           };
-          if (kCap && raw) second_pass(std::integral_constant<bool, kCap>{});
-          else second_pass(std::false_type{});
+          if (!kLateCap || !full) second_pass(std::integral_constant<int, 0>{});
+          else if (!stored) second_pass(std::integral_constant<int, kLateCap ? 1 : 0>{});
+          else second_pass(std::integral_constant<int, kLateCap ? 2 : 0>{});
           float a, b;
           f2_split(f2_add(sum0, sum1), a, b);
           l += a + b;

@@ -284,7 +284,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
     // 10^-6 vanish, up to 0.0075 of a score near half the cap: the polynomial only where
     // they do not count (0.02^4 of the score), and above it 1 - 2 / (1 + e^2y), whose
     // error of 10^-7 caps is then 5e-6 of the score.
-    p.cap_hot = p.cap_a > 1e6f ? -1.f : p.cap_a < 1e-6f ? 0.02f : 0.5f;
+    p.cap_hot = (p.cap_a > 1e6f ? -1.f : p.cap_a < 1e-6f ? 0.02f : 0.5f) / p.cap_a;
     const float z = p.cap_a * p.cap_a;
     p.cap_q[0] = AP_T1 * z;
     p.cap_q[1] = AP_T2 * z * z;

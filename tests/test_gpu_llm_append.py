@@ -534,3 +534,37 @@ def test_caps_far_above_the_scale(ctx, cap):
     got = att.append(q.to(DEV), pages[0], pages[1], d(0, 3), d(ctx), d(0)[None])
     att.check_errors()
     check(got, *O.attend(q, K, V, O.visible(3, ctx), scale, cap))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("opts", [dict(softcap=30.0), dict(softcap=6.0), dict(softcap=1e4),
+                                  dict(softcap=30.0, slopes=slopes_of(12))])
+def test_a_capped_row_depends_on_its_query_and_the_keys_it_sees(opts, D):
+    """Bit for bit, for caps whose scores lie below and around half of them: other tokens'
+    queries, what stands in cache rows that no token sees, and the key of a drafted
+    token that only it sees, choose no other token's way to compute tanh."""
+    c = Case(MANY, D=D, **opts)
+    att = c.attention()
+    want, q, K = c.device().call(att).cpu(), c.q, c.K
+    r = random.Random(D)
+    for by in (8.0, 0.0, 30.0):
+        rows = [t for t in range(q.shape[0]) if r.random() < 0.3]
+        c.q = q.clone()
+        c.q[rows] *= by
+        others = torch.ones(q.shape[0], dtype=torch.bool)
+        others[rows] = False
+        assert torch.equal(c.device().call(att).cpu()[others], want[others])
+    c.q = q
+    for fill in (0.0, 1.0, 1e4, 1e38, float("inf")):
+        c.K = torch.where(K.isnan(), fill, K)
+        assert torch.equal(c.device().call(att).cpu(), want)
+    if "slopes" in opts:
+        return
+    c = Case(TREES * 6, D=D, tree=trees(TREES * 6, 5), **opts)
+    att = c.attention()
+    want = c.device().call(att).cpu()
+    others = torch.ones(c.q.shape[0], dtype=torch.bool)
+    for i, (m, p) in enumerate(c.lens):      # the last drafted token is nobody's parent
+        others[int(c.cu[i]) + m - 1] = False
+        c.K[c.table[i, (p + m - 1) // c.bs].long(), (p + m - 1) % c.bs] *= 64
+    assert torch.equal(c.device().call(att).cpu()[others], want[others])
