@@ -161,9 +161,9 @@ int dllm_rotary(const DllmRotary* args, void* stream);
  * mask, whatever their order; the other masks and slopes are not used then.
  * Scores are s = scale q.k, softcap tanh(s / softcap) if softcap > 0, minus
  * slopes[h] |p - k| if slopes; the output is softmax(s) v, and zeros for a
- * token that sees no key.  An infinity or NaN in a K or V row reaches the
- * tokens that see it (V in a tile with masked keys: their rows become NaN) and
- * no other; keys that no token sees are not read beyond the pages of those
+ * token that sees no key.  An infinity or NaN in a K row reaches the tokens
+ * that see it, one in a V row its own dims of theirs (as an infinity or NaN),
+ * and no other; keys that no token sees are not read beyond the pages of those
  * that are.  Rows of q and out past cu_seqlens_q[n] are not touched.
  * ------------------------------------------------------------------------- */
 typedef struct DllmAppend {

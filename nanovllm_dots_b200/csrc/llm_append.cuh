@@ -42,10 +42,10 @@
 // two threads a row instead of one: 568.
 //
 // Keys nobody in the unit may see are not loaded (their pages may be gone) and
-// their rows of V are set to zero.  In a tile with masks, a visible row of V
-// that holds an infinity or a NaN is set to zero as well and noted: the rows
-// that see it become NaN, and no other row is touched (0 * inf in the product
-// would reach them all).
+// their rows of V are set to zero.  In a tile with masks, an infinity or a NaN in a
+// visible row of V is set to zero as well (0 * inf in the product would reach
+// every row) and the key noted: the rows that see it add it to their output at
+// the end, at its own dim.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -111,6 +111,7 @@ struct ApParams {
   const int* first;                 // [tokens] or null
   const unsigned long long* tree;   // [tokens] or null
   const float* slopes;              // [H] or null
+  const void* v;                    // the V cache, for its special values
   void* out;                        // [tokens][H][D]
   uint32_t* err;
   ApHead* head;                     // head .. start: of the plan kernel, unused with near_plan
@@ -120,6 +121,7 @@ struct ApParams {
   ApCut* cuts;                      // [ctas]
   float* part_o;                    // [ctas][2][2][D / 8][128][8]
   float2* part_ml;                  // [ctas][2][2][128]
+  void* special;                    // ApSpecial<D> [ctas][2 streams][128]
   int tokens, n, H, KVH, G, RT, max_units, ctas, near_plan;
   int num_blocks, block_size, max_blocks, box_rows;
   int causal, window;
@@ -624,6 +626,78 @@ DFM_DEV uint32_t ap_zero_times(uint32_t x, uint32_t sum) {
   return r;
 }
 
+// Two 16-bit values, an infinity or a NaN replaced by zero.
+template <bool kFp16>
+DFM_DEV uint32_t ap_finite(uint32_t x) {
+  constexpr uint32_t E = kFp16 ? 0x7c007c00u : 0x7f807f80u;
+  return x & ~__vcmpeq2(x & E, E);
+}
+
+// The lowest n bits, n clamped to [0, 32].
+DFM_DEV uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Which of the 32 keys from kc on a row sees: [lo, hi), and drafted tokens of a tree.
+DFM_DEV uint32_t ap_sees(int kc, int lo, int hi, int base, unsigned long long bits) {
+  uint32_t see = low_bits(hi - kc) & ~low_bits(lo - kc);
+  const int o = base - kc;   // drafted token 0's bit in this word
+  if (bits) see |= o >= 32 || o <= -64 ? 0u
+                 : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
+  return see;
+}
+
+template <bool kFp16>
+DFM_DEV float ap_value(uint16_t x) {
+  return kFp16 ? __half2float(__ushort_as_half(x)) : __uint_as_float(static_cast<uint32_t>(x) << 16);
+}
+
+// A row's special values of V: two bits a dim, an infinity seen (x) or a negative one
+// (y), both where their sum is a NaN.
+template <int D>
+struct ApSpecial {
+  uint2 dims[D / 32];
+};
+
+// Notes those of the key tile at k0 that the row sees; poison: the tile's keys that have
+// any; fresh: the segment's first.
+template <int D, bool kFp16>
+__device__ __noinline__ void ap_special_note(const ApParams& p, int seq, int kv, int k0, const uint32_t* poison,
+                                             int lo, int hi, int base, unsigned long long bits,
+                                             ApSpecial<D>* sp, bool fresh) {
+  if (fresh) *sp = ApSpecial<D>{};
+  for (int c = 0; c < 128; c += 32) {
+    for (uint32_t w = poison[c >> 5] & ap_sees(k0 + c, lo, hi, base, bits); w; w &= w - 1) {
+      const int key = k0 + c + __ffs(w) - 1, block = p.by_block(key);
+      const int cb = p.bt[static_cast<size_t>(seq) * p.max_blocks + block];
+      if (cb < 0 || cb >= p.num_blocks) continue;   // (read as zeros)
+      const size_t row = static_cast<size_t>(cb) * p.block_size + (key - block * p.block_size);
+      const uint16_t* v = static_cast<const uint16_t*>(p.v) + (row * p.KVH + kv) * D;
+      for (int d = 0; d < D; ++d) {
+        constexpr uint32_t E = kFp16 ? 0x7c00u : 0x7f80u;
+        if ((v[d] & E) != E) continue;
+        const bool nan = v[d] & (E ^ 0x7fffu), neg = v[d] >> 15;
+        if (nan || !neg) sp->dims[d >> 5].x |= 1u << (d & 31);
+        if (nan || neg) sp->dims[d >> 5].y |= 1u << (d & 31);
+      }
+    }
+  }
+}
+
+// Adds them to dims [lo, hi) of what this thread wrote: the row's output, or its
+// partial (out null).
+template <int D, bool kFp16>
+__device__ __noinline__ void ap_special_put(const ApSpecial<D>* a, const ApSpecial<D>* b, int lo, int hi,
+                                            uint16_t* out, float* po) {
+  for (int d = lo; d < hi; ++d) {
+    const uint32_t bit = 1u << (d & 31);
+    const bool inf = ((a ? a->dims[d >> 5].x : 0) | (b ? b->dims[d >> 5].x : 0)) & bit;
+    const bool neg = ((a ? a->dims[d >> 5].y : 0) | (b ? b->dims[d >> 5].y : 0)) & bit;
+    if (!inf && !neg) continue;
+    const float x = inf && neg ? __int_as_float(0x7fffffff) : inf ? INFINITY : -INFINITY;
+    if (out) out[d] = static_cast<uint16_t>(ap_pack<kFp16>(ap_value<kFp16>(out[d]) + x, 0.f));
+    else po[static_cast<size_t>(d >> 3) * (AP_ROWS * 8) + (d & 7)] += x;
+  }
+}
+
 DFM_DEV void st_global_v8(void* dst, const uint32_t (&v)[8]) {   // 32-byte aligned
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
                "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -660,9 +734,6 @@ DFM_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-
-// The lowest n bits, n clamped to [0, 32].
-DFM_DEV uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // 2^x of two scores on the fp32 pipe: x = n + f with n the nearest integer, 2^f by
 // the polynomial of degree 5 fitted at Chebyshev nodes of [-1/2, 1/2] (1e-7
@@ -1085,11 +1156,18 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               }
               special = (sum & 0x7fff7fffu) != 0;
             }
-            if (!seen || special) {
+            if (!seen) {
 #pragma unroll 4
               for (int c = 0; c < 8 * S::BOXES; ++c)
                 *reinterpret_cast<uint4*>(row + (c >> 3) * S::HALF + (((c & 7) ^ (r & 7)) << 4)) =
                     make_uint4(0, 0, 0, 0);
+            } else if (special) {
+#pragma unroll 1
+              for (int c = 0; c < 8 * S::BOXES; ++c) {
+                uint4& u = *reinterpret_cast<uint4*>(row + (c >> 3) * S::HALF + (((c & 7) ^ (r & 7)) << 4));
+                u = make_uint4(ap_finite<kFp16>(u.x), ap_finite<kFp16>(u.y), ap_finite<kFp16>(u.z),
+                               ap_finite<kFp16>(u.w));
+              }
             }
             const uint32_t word = __ballot_sync(0xffffffffu, special);
             if (lane == 0) poison[slot * 4 + w * 2 + x] = word;
@@ -1140,15 +1218,12 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     while (more) {
       const int nt = sg.i1 - sg.i0;
       const bool narrow = sg.narrow;
-      // which of the 32 keys from kc on the row sees
-      auto sees = [&](int kc) {
-        uint32_t see = low_bits(hi - kc) & ~low_bits(lo - kc);
-        const int o = base - kc;   // drafted token 0's bit in this word
-        if (!kBias && bits) see |= o >= 32 || o <= -64 ? 0u
-                         : o >= 0 ? static_cast<uint32_t>(bits << o) : static_cast<uint32_t>(bits >> -o);
-        return see;
-      };
+      auto sees = [&](int kc) { return ap_sees(kc, lo, hi, base, kBias ? 0 : bits); };
       float m = -INFINITY, l = 0.f;
+      bool special = false, special_too = false;   // of V: this stream's, the other's (narrow)
+      auto special_of = [&](int stream) {
+        return reinterpret_cast<ApSpecial<D>*>(p.special) + (blockIdx.x * 2 + stream) * AP_ROWS + r;
+      };
       const int step = narrow ? 2 : 1, i_first = narrow ? s : 0;
 #pragma unroll 1
       for (int i = i_first; ok && i < nt; i += step, ++ns) {
@@ -1263,7 +1338,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if (!ok) break;
               uint32_t bad = 0;
               for (int c = 0; c < 4; ++c) bad |= poison[slot * 4 + c] & sees(k0 + c * 32);
-              if (bad) l = __int_as_float(0x7fffffff);
+              if (bad) {
+                ap_special_note<D, kFp16>(p, sg.f.seq, sg.kv, k0, poison + slot * 4, lo, hi, base,
+                                          kBias ? 0 : bits, special_of(s), !special);
+                special = true;
+              }
             }
             tmem_wait_st();
           }
@@ -1376,9 +1455,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       if (more) row();     // its loads run under what follows
       float w0 = 1.f, w1 = 0.f;       // weights of O_0 and O_1 (narrow)
       if (narrow) {
-        sML[s * AP_ROWS + r] = make_float2(m, l);
+        sML[s * AP_ROWS + r] = make_float2(m, copysignf(l, special ? -1.f : 1.f));
         ok = ap_meet(1, 32 * AP_SOFT_WARPS, ok);
-        const float2 o = sML[(1 - s) * AP_ROWS + r];
+        float2 o = sML[(1 - s) * AP_ROWS + r];
+        special_too = signbit(o.y);
+        o.y = fabsf(o.y);
         const float mm = fmaxf(m, o.x);
         const float wm = m == -INFINITY ? 0.f : fast_exp2(m - mm), wo = o.x == -INFINITY ? 0.f : fast_exp2(o.x - mm);
         w0 = s ? wo : wm;
@@ -1432,6 +1513,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                            reinterpret_cast<const uint32_t(&)[8]>(v[e]));
           }
         }
+        if (special || special_too)
+          ap_special_put<D, kFp16>(special ? special_of(s) : nullptr, special_too ? special_of(1 - s) : nullptr,
+                                   c_lo, c_hi, whole ? out : nullptr, po);
       }
       tc_fence_before();
       if (narrow) ok = ap_meet(1, 32 * AP_SOFT_WARPS, ok);   // both have read O_0 and O_1

@@ -43,7 +43,7 @@ cudaError_t launch_rotary(RotaryParams& p, cudaStream_t s) {
 
 // ---------------------------------------------------------------- append attention
 struct ApWs {
-  size_t head, units, ubase, start, cuts, part_ml, part_o, total;
+  size_t head, units, ubase, start, cuts, special, part_ml, part_o, total;
 };
 
 int ap_max_units(int tokens, int n, int RT) {
@@ -59,7 +59,8 @@ ApWs ap_ws(int tokens, int n, int G, int D, int ctas) {
   w.ubase = w.units + up(sizeof(ApUnit) * static_cast<size_t>(ap_max_units(tokens, n, AP_ROWS / G)));
   w.start = w.ubase + up(4 * (static_cast<size_t>(n) + 1));
   w.cuts = w.start + up(4 * (static_cast<size_t>(ctas) + 1));
-  w.part_ml = w.cuts + up(sizeof(ApCut) * static_cast<size_t>(ctas));
+  w.special = w.cuts + up(sizeof(ApCut) * static_cast<size_t>(ctas));
+  w.part_ml = w.special + up(static_cast<size_t>(ctas) * 2 * AP_ROWS * D / 4);   // two bits a dim
   w.part_o = w.part_ml + up(static_cast<size_t>(ctas) * 4 * AP_ROWS * sizeof(float2));
   w.total = w.part_o + static_cast<size_t>(ctas) * 4 * AP_ROWS * D * 4;
   return w;
@@ -245,6 +246,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.first = a->first_keys;
   p.tree = reinterpret_cast<const unsigned long long*>(a->tree_masks);
   p.slopes = a->slopes;
+  p.v = a->v_cache;
   p.out = a->out;
   p.err = reinterpret_cast<uint32_t*>(ws);
   p.head = reinterpret_cast<ApHead*>(ws + w.head);
@@ -252,6 +254,7 @@ int dllm_append_attention(const DllmAppend* a, void* workspace, size_t workspace
   p.ubase = reinterpret_cast<int*>(ws + w.ubase);
   p.start = reinterpret_cast<int*>(ws + w.start);
   p.cuts = reinterpret_cast<ApCut*>(ws + w.cuts);
+  p.special = ws + w.special;
   p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + w.part_o);
   p.tokens = a->tokens;

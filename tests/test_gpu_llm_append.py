@@ -568,3 +568,49 @@ def test_a_capped_row_depends_on_its_query_and_the_keys_it_sees(opts, D):
         others[int(c.cu[i]) + m - 1] = False
         c.K[c.table[i, (p + m - 1) // c.bs].long(), (p + m - 1) % c.bs] *= 64
     assert torch.equal(c.device().call(att).cpu()[others], want[others])
+
+
+SPECIALS = [  # sequences (new, before), their options, special rows of V (sequence, position, value)
+    ("tree", [(6, 150), (64, 300)], dict(tree=[[-1, 0, -1, 2, 3, 1], list(range(-1, 31)) + list(range(-1, 31))]),
+     [(0, 151, 1), (0, 154, -1), (1, 320, 0), (1, 350, 1), (1, 351, -1)]),
+    ("causal", [(9, 200), (70, 90)], dict(),
+     [(0, 203, 1), (0, 205, 0), (0, 206, -1), (1, 100, 1), (1, 101, -1), (1, 140, 0), (1, 3, 1)]),
+    ("split", [(30, 40000), (3, 30000)], dict(), [(0, 40010, 1), (0, 40020, -1), (1, 30001, 0), (1, 20000, 1)]),
+    ("window", [(40, 1000), (1, 777)], dict(window=100), [(0, 905, 1), (0, 930, -1), (0, 1010, 1), (1, 700, 0)]),
+    ("prefix", [(150, 300), (20, 0)], dict(prefix=[400, 9]), [(0, 390, 1), (0, 420, -1), (0, 449, 0), (1, 7, 1), (1, 15, -1)]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("name,lens,opts,rows", SPECIALS, ids=[x[0] for x in SPECIALS])
+def test_special_values_of_v_reach_their_own_dims(name, lens, opts, rows, D, dtype):
+    """An infinity or a NaN at one dim of a V row, in tiles with masks and without, in
+    units of one share and of several: the tokens that see it have the sum of what they see
+    at that dim, and every other value is, bit for bit, as it is with zeros there."""
+    opts = dict(opts)
+    if "tree" in opts:
+        opts["tree"] = tree_masks(opts["tree"])
+    c = Case(lens, D=D, dtype=dtype, spread=0.3, **opts)
+    value = {1: float("inf"), -1: float("-inf"), 0: float("nan")}
+    T = c.q.shape[0]
+    expect = torch.zeros(T, D, dtype=torch.float64)
+    for x, (i, at, kind) in enumerate(rows):
+        dims = [(7 * x) % D, 11]         # one of its own, one that the special rows share
+        a = int(c.cu[i])
+        see = c.see[i][:, at]
+        assert see.any()
+        for d in dims:
+            expect[a:a + lens[i][0], d] += torch.where(see, value[kind], 0.0).double()
+            c.V[int(c.table[i, at // c.bs]), at % c.bs, :, d] = 0
+    att = c.attention()
+    want = c.device().call(att).cpu()
+    for x, (i, at, kind) in enumerate(rows):
+        for d in ((7 * x) % D, 11):
+            c.V[int(c.table[i, at // c.bs]), at % c.bs, :, d] = value[kind]
+    got = c.device().call(att).cpu()
+    att.check_errors()
+    expect = expect[:, None].expand(T, 12, D)
+    plain = expect == 0
+    assert torch.equal(got[plain], want[plain])
+    assert torch.equal(got[~plain].double().nan_to_num(7.0), expect[~plain].nan_to_num(7.0))
