@@ -129,7 +129,10 @@ int dllm_read_error(void* workspace, void* stream, uint32_t* err_word) {
   uint32_t v = 0;
   CK(cudaMemcpyAsync(&v, workspace, sizeof(v), cudaMemcpyDeviceToHost, s));
   CK(cudaStreamSynchronize(s));
-  CK(cudaMemsetAsync(workspace, 0, sizeof(uint32_t), s));
+  if (v) {   // (a clear that is not needed, or not over yet, could erase a report from another stream)
+    CK(cudaMemsetAsync(workspace, 0, sizeof(uint32_t), s));
+    CK(cudaStreamSynchronize(s));
+  }
   *err_word = v;
   return DFM_OK;
 }

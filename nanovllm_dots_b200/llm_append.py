@@ -85,6 +85,7 @@ class B200AppendAttention:
             raise RuntimeError("unsupported append-attention shape")
         self.workspace = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
         self.workspace[:256].zero_()
+        torch.cuda.current_stream(self.device).synchronize()   # graphs may be replayed on any stream
         self._index = self.device.index
         self._dtype = _DTYPES[dtype]
         self._call = _lib.packed("dllm_append_attention", _lib.c_void_p, _lib.c_size_t, _lib.c_void_p)
@@ -192,11 +193,11 @@ class B200AppendAttention:
                          tree_masks, out, stream)
 
     def check_errors(self) -> None:
-        """Synchronise and raise if a kernel reported a device-side error."""
+        """Wait for the device (calls and replayed graphs may be on any stream) and
+        raise if a kernel reported an error."""
+        torch.cuda.synchronize(self.device)
         v = _lib.c_uint32(0)
         s = torch.cuda.current_stream(self.device)
-        if s.cuda_stream != self._stream:
-            self._follow(s.cuda_stream)
         with torch.cuda.device(self.device):
             _lib.check(self.L.dllm_read_error(_lib.ptr(self.workspace), _lib.c_void_p(s.cuda_stream), v),
                        "dllm_read_error")

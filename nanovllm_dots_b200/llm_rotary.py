@@ -125,6 +125,7 @@ class B200Rotary:
         self.L = _lib.lib()
         self.turns = _turns(inv).to(self.device)
         self.err = torch.zeros(64, dtype=torch.int32, device=self.device)
+        torch.cuda.current_stream(self.device).synchronize()   # calls may come on any stream
         self._index, self._inter = self.device.index, layout == "interleaved"
         self._call = _lib.packed("dllm_rotary", _lib.c_void_p)
         self._turns, self._err = self.turns.data_ptr(), self.err.data_ptr()
@@ -219,7 +220,9 @@ class B200Rotary:
         return self._run(q, positions, out, stream, (k, v, slot_mapping, k_cache, v_cache))
 
     def check_errors(self) -> None:
-        """Synchronise and raise if a slot past the cache was met."""
+        """Wait for the device (calls and replayed graphs may be on any stream) and
+        raise if a slot past the cache was met."""
+        torch.cuda.synchronize(self.device)
         v = _lib.c_uint32(0)
         s = torch.cuda.current_stream(self.device)
         with torch.cuda.device(self.device):

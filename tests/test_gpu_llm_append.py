@@ -614,3 +614,22 @@ def test_special_values_of_v_reach_their_own_dims(name, lens, opts, rows, D, dty
     plain = expect == 0
     assert torch.equal(got[plain], want[plain])
     assert torch.equal(got[~plain].double().nan_to_num(7.0), expect[~plain].nan_to_num(7.0))
+
+
+def test_errors_of_a_graph_on_another_stream_are_reported():
+    """A bad block id met by a graph that is replayed on a busy stream."""
+    c = Case([(5, 600), (3, 20)]).device()
+    c.tabled[0, 1] = 10_000
+    att, out = c.attention(), torch.empty_like(c.qd)
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        c.call(att, out=out)
+    for _ in range(2):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(100_000_000)
+            g.replay()
+        with pytest.raises(RuntimeError, match="page"):
+            att.check_errors()
+        att.check_errors()

@@ -138,3 +138,32 @@ def test_no_tokens_graph_and_stream():
     other = r.rotate(x, pos, stream=s)
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(other, want)
+
+
+@pytest.mark.parametrize("how", ["stream argument", "current stream", "replayed graph"])
+def test_errors_on_other_streams_are_reported(how):
+    """A slot past the cache met on a stream that is still busy when the error is asked for."""
+    r = B200Rotary(128, device=DEV)
+    qkv = data(4, 4, 128, torch.bfloat16).to(DEV)
+    K = torch.zeros(2, 16, 1, 128, dtype=torch.bfloat16, device=DEV)
+    V = torch.zeros_like(K)
+    pos, slots = torch.arange(4, dtype=torch.int32, device=DEV), torch.tensor([0, 32, 5, 31], dtype=torch.int32, device=DEV)
+    args = (qkv[:, :2], qkv[:, 2:3], qkv[:, 3:], pos, slots, K, V)
+    out = torch.empty(4, 2, 128, dtype=torch.bfloat16, device=DEV)
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    if how == "replayed graph":
+        with torch.cuda.graph(g):
+            r.rotate_store(*args, out=out)
+    for _ in range(3):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(100_000_000)
+            if how == "replayed graph":
+                g.replay()
+            elif how == "current stream":
+                r.rotate_store(*args, out=out)
+        if how == "stream argument":
+            r.rotate_store(*args, out=out, stream=s)
+        with pytest.raises(RuntimeError, match="page"):
+            r.check_errors()
+        r.check_errors()
