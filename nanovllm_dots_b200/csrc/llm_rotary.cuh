@@ -6,10 +6,10 @@
 // with the pair (d, d + rot_dim / 2) in the half layout and (2d, 2d + 1) in the
 // interleaved one; dims past rot_dim are copied.  w_i comes in turns per
 // position as a 64-bit binary fraction, so the angle modulo one turn is one
-// wrapping 64-bit multiplication, off by at most |position| * 2^-65 turns: a
-// 32-bit float angle is off by 0.06 rad at position 10^6.  What is left of a
-// turn is split into a quarter (exact) and an eighth-turn remainder for
-// sincospif.
+// wrapping 64-bit multiplication, off by at most |position| * 2^-65 turns, of
+// which the upper 32 bits are used (another 2^-32): a 32-bit float angle is off by
+// 0.06 rad at position 10^6.  What is left of a turn is split into a quarter
+// (exact) and an eighth-turn remainder for sincospif.
 #pragma once
 
 #include <cuda_fp16.h>

@@ -92,19 +92,40 @@ def rotary_frequencies(rot_dim: int, theta: float, scaling: RotaryScaling | None
     return inv / s.factor * (1 - keep) + inv * keep, factor
 
 
+def _two_pi(bits: int) -> int:
+    """2 pi * 2^bits as an integer (Machin: pi = 16 arctan(1/5) - 4 arctan(1/239))."""
+    one = 1 << (bits + 16)
+
+    def arctan(n):
+        term, total, k = one // n, 0, 1
+        while term:
+            total += term // k if k % 4 == 1 else -(term // k)
+            term //= n * n
+            k += 2
+        return total
+
+    return (32 * arctan(5) - 8 * arctan(239)) >> 16
+
+
+_TWO_PI = _two_pi(192)
+
+
 def _turns(inv: torch.Tensor) -> torch.Tensor:
-    """Frequencies as turns a position, a binary fraction of 2^64 in int64."""
+    """Frequencies as turns a position, a binary fraction of 2^64 in int64: each
+    float64 frequency by 2 pi in integer arithmetic, rounded once."""
     out = []
     for w in inv.tolist():
-        bits = round(math.ldexp(math.fmod(w / (2 * math.pi), 1.0), 64)) & ((1 << 64) - 1)
+        n, d = w.as_integer_ratio()
+        scaled, by = n << (64 + 192), d * _TWO_PI
+        bits = (2 * scaled + by) // (2 * by) & ((1 << 64) - 1)
         out.append(bits - (1 << 64) if bits >> 63 else bits)
     return torch.tensor(out, dtype=torch.int64)
 
 
 class B200Rotary:
     """Rotary of one model: head size, layout and frequencies.  Rotated values
-    are computed in fp32 and rounded once; the angle is exact to 2^-31 turns at
-    every int32 position."""
+    are computed in fp32 and rounded once; the angle is that of the frequencies
+    in float64 to 2^-31 turns, at every int32 position."""
 
     def __init__(self, head_dim: int, *, theta: float = 10000.0, rot_dim: int | None = None,
                  layout: str = "half", scaling: RotaryScaling | None = None,

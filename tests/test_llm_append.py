@@ -7,6 +7,7 @@ import math
 import os
 import shutil
 import subprocess
+from fractions import Fraction
 
 import pytest
 import torch
@@ -170,6 +171,31 @@ def test_turns_keep_the_angle_at_far_positions():
             gap = abs(math.remainder(got - math.fmod(pos * w, 2 * math.pi), 2 * math.pi))
             # the fraction of 2^64 is rounded: half a unit a position, in radians
             assert gap <= pos * (w * 2.0 ** -51 + math.pi * 2.0 ** -64) + 1e-12
+
+
+def exact_two_pi():
+    """2 pi as a fraction, from Euler's pi = 20 arctan(1/7) + 8 arctan(3/79)."""
+    def arctan(x):
+        total, power, k = Fraction(0), x, 1
+        while abs(power) > Fraction(1, 1 << 220):
+            total += power / k if k % 4 == 1 else -power / k
+            power, k = power * x * x, k + 2
+        return total
+
+    return 2 * (20 * arctan(Fraction(1, 7)) + 8 * arctan(Fraction(3, 79)))
+
+
+@pytest.mark.parametrize("rot,theta,scaling", [(128, 1e6, None), (64, 10000.0, None), (2, 5e4, None),
+                                               (64, 1e6, RotaryScaling("yarn", 16.0, 4096)),
+                                               (128, 5e5, RotaryScaling("bands", 8.0, 8192))])
+def test_turns_are_rounded_to_the_last_bit(rot, theta, scaling):
+    """Against rational arithmetic: half a unit of 2^-64 turns a position, which is
+    |position| 2^-65 turns of the angle."""
+    inv, _ = rotary_frequencies(rot, theta, scaling)
+    period = exact_two_pi()
+    for w, t in zip(inv.tolist(), _turns(inv).tolist()):
+        off = Fraction(t % (1 << 64)) - Fraction(w) / period * (1 << 64)
+        assert abs(off) <= Fraction(1, 2) + Fraction(1, 1 << 100)
 
 
 def test_tree_masks():
