@@ -134,7 +134,8 @@ typedef struct DllmRotary {
   const uint64_t* turns;        /* [rot_dim / 2] turns a position, as a binary fraction of 2^64 */
   const int32_t* positions;     /* [tokens] */
   const void* q;                /* [tokens, q_heads, head_dim] */
-  void* q_out;                  /* the same shape; may be q with q's strides, else no overlap */
+  void* q_out;                  /* the same shape; may be q with q's strides, else no overlap with
+                                 * anything; the caches overlap no other tensor either */
   const void* k;                /* [tokens, kv_heads, head_dim]; NULL skips the store */
   const void* v;
   void* k_cache;                /* [num_slots, kv_heads, head_dim] */

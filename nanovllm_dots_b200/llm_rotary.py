@@ -147,6 +147,7 @@ class B200Rotary:
         self.turns = _turns(inv).to(self.device)
         self.err = torch.zeros(64, dtype=torch.int32, device=self.device)
         torch.cuda.current_stream(self.device).synchronize()   # calls may come on any stream
+        self._size = {_lib.DLLM_BF16: 2, _lib.DLLM_FP16: 2, _lib.DLLM_FP32: 4}
         self._index, self._inter = self.device.index, layout == "interleaved"
         self._call = _lib.packed("dllm_rotary", _lib.c_void_p)
         self._turns, self._err = self.turns.data_ptr(), self.err.data_ptr()
@@ -172,8 +173,33 @@ class B200Rotary:
             raise RuntimeError(f"{name}: expected a contiguous int32 [{tokens}] on {self.device}")
         return t.data_ptr()
 
+    def _check_apart(self, read, out, T, size, kc, vc, room):
+        """Raises where the store's outputs share memory with each other or with what
+        the call reads (out may be q).  Tensors come with address, token and head
+        strides and heads: where their spans cross, slices of one packed row are
+        apart by their places in it, and else every row is looked at."""
+        D = self.head_dim
+        if abs(kc - vc) < room:
+            raise RuntimeError("k_cache and v_cache overlap")
+        lo, hi = min(kc, vc), max(kc, vc) + room
+        for t, p, ts, hs, n in read if out is None else (*read, out):
+            if p < hi and p + ((T - 1) * ts + (n - 1) * hs + D) * size > lo and \
+                    (meets(t, kc, kc + room) or meets(t, vc, vc + room)):
+                raise RuntimeError("q, k, v or out overlaps a cache")
+        if out is None:
+            return
+        t, p, ts, hs, n = out
+        row, wide = ts * size, ((n - 1) * hs + D) * size
+        for other, p2, ts2, hs2, n2 in read[1:]:
+            wide2 = ((n2 - 1) * hs2 + D) * size
+            if p2 + (T - 1) * ts2 * size + wide2 <= p or p + (T - 1) * row + wide <= p2 or \
+                    (ts == ts2 and row and wide <= (p2 - p) % row <= row - wide2):
+                continue
+            if shared(t, other):
+                raise RuntimeError("out: overlaps k or v")
+
     def _run(self, q, positions, out, stream, store):
-        dtype = _DTYPES.get(q.dtype)
+        dtype, given = _DTYPES.get(q.dtype), out is not None
         if dtype is None:
             raise RuntimeError(f"q: unsupported type {q.dtype}")
         T = q.shape[0]
@@ -213,7 +239,17 @@ class B200Rotary:
                     raise RuntimeError(f"{name}: expected a contiguous {q.dtype} [num_blocks, block_size, "
                                        f"{kvh}, {self.head_dim}] on {self.device}, and both caches alike")
             slots = shape[0] * shape[1]
-            kp, vp, kcp, vcp = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+            kp, vp, qp = k.data_ptr(), v.data_ptr(), q.data_ptr()
+            kcp, vcp = k_cache.data_ptr(), v_cache.data_ptr()
+            D, size = self.head_dim, self._size[dtype]
+            room, lo, hi = slots * kvh * D * size, min(kcp, vcp), max(kcp, vcp)
+            end, t1 = hi + room, T - 1
+            if T and (given or hi - lo < room or
+                      (qp < end and qp + (t1 * qt + (heads - 1) * qh + D) * size > lo) or
+                      (kp < end and kp + (t1 * kt + (kvh - 1) * kh + D) * size > lo) or
+                      (vp < end and vp + (t1 * vt + (kvh - 1) * vh + D) * size > lo)):
+                self._check_apart(((q, qp, qt, qh, heads), (k, kp, kt, kh, kvh), (v, vp, vt, vh, kvh)),
+                                  (out, out.data_ptr(), ot, oh, heads) if given else None, T, size, kcp, vcp, room)
         if T == 0 or heads == 0 and store is None:
             return out
         a = _pack(dtype, T, heads, kvh, self.head_dim, self.rot_dim, self._inter, self.factor,
@@ -237,7 +273,8 @@ class B200Rotary:
         block_size, kv_heads, head_dim] at int32 slot_mapping [tokens] (block *
         block_size + offset; -1 stores nothing).  Two tokens must not share a
         slot.  A slot past the cache is not stored and reported by
-        ``check_errors``."""
+        ``check_errors``.  The caches share no memory with each other nor with q,
+        k or v, and out none with k, v and the caches."""
         return self._run(q, positions, out, stream, (k, v, slot_mapping, k_cache, v_cache))
 
     def check_errors(self) -> None:
@@ -255,7 +292,7 @@ class B200Rotary:
 
 
 def _span(t):
-    """First and last byte of a tensor's elements."""
+    """First byte of a tensor's elements and the one behind the last."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
@@ -265,6 +302,31 @@ def overlap(a, b) -> bool:
         return False
     (a0, a1), (b0, b1) = _span(a), _span(b)
     return a0 < b1 and b0 < a1
+
+
+def _starts(t):
+    """First bytes of the rows of [tokens, heads, dims], sorted, and a row's length."""
+    size = t.element_size()
+    token, head = (torch.arange(n, device="cpu") for n in t.shape[:2])
+    at = (token[:, None] * t.stride(0) + head * t.stride(1)) * size
+    return (at.flatten() + t.data_ptr()).sort().values, t.shape[2] * size
+
+
+def meets(t, lo: int, hi: int) -> bool:
+    """Whether a row of [tokens, heads, dims] reaches into the bytes [lo, hi)."""
+    at, room = _starts(t)
+    return bool(((at < hi) & (at + room > lo)).any())
+
+
+def shared(a, b) -> bool:
+    """Whether two tensors [tokens, heads, dims] have elements in common, which
+    spans that cross do not say: heads of a packed row may take turns."""
+    if not overlap(a, b):
+        return False
+    (x, wx), (y, wy) = _starts(a), _starts(b)
+    # rows of y before the end of a row of x, of which the last reaches into it
+    i = torch.searchsorted(y, x + wx) - 1
+    return bool(((i >= 0) & (y[i.clamp(min=0)] + wy > x)).any())
 
 
 def _apart(t) -> bool:

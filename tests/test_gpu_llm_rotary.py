@@ -167,3 +167,41 @@ def test_errors_on_other_streams_are_reported(how):
         with pytest.raises(RuntimeError, match="page"):
             r.check_errors()
         r.check_errors()
+
+
+def test_store_refuses_memory_that_its_outputs_share():
+    """out over k, v or a cache, caches over each other or over what is read; slices of one
+    packed projection, out=q among them, are apart."""
+    T, D = 40, 64
+    r = B200Rotary(D, device=DEV)
+    packed = data(T, 16, D, torch.bfloat16).to(DEV)
+    pos, slots = positions(T).to(DEV), torch.arange(T, dtype=torch.int32, device=DEV)
+    pool = torch.zeros(6, 48, 2, D, dtype=torch.bfloat16, device=DEV)
+    K, V, more = pool[:2], pool[2:4], pool[4:]
+    q, k, v = packed[:, :12], packed[:, 12:14], packed[:, 14:]
+
+    def call(q=q, k=k, v=v, K=K, V=V, out=None):
+        return r.rotate_store(q, k, v, pos, slots, K, V, out=out)
+
+    want = call().clone()
+    kept = K.clone(), V.clone()
+    rows = more.view(-1, 2, D)[:T]
+    for bad in (dict(out=packed[:, 1:13]), dict(out=packed[:, 2:14]), dict(out=packed[:, 4:16]),
+                dict(V=K), dict(V=pool[1:3]), dict(k=K.view(-1, 2, D)[:T]), dict(v=V.view(-1, 2, D)[:T]),
+                dict(q=V.view(-1, 2, D)[:T]), dict(q=rows, out=K.view(-1, 2, D)[:T]),
+                dict(q=rows, out=pool.view(-1, 2, D)[90:90 + T])):
+        with pytest.raises(RuntimeError, match="overlap|share no memory"):
+            call(**bad)
+    torch.cuda.synchronize()
+    assert torch.equal(K, kept[0]) and torch.equal(V, kept[1])
+    K.zero_(), V.zero_()
+    assert torch.equal(call(out=torch.empty_like(want)), want)
+    assert call(out=q) is q and torch.equal(q, want)          # in place, next to k and v
+    assert torch.equal(K, kept[0]) and torch.equal(V, kept[1])
+    mixed = packed[:, :12].view(T, 2, 6, D)                    # heads of q, k and v interleaved
+    qi, ki, vi = (mixed[:, :, i] for i in range(3))
+    got = call(q=qi, k=ki, v=vi)
+    again = call(q=qi.clone(), k=ki.clone(), v=vi.clone())
+    assert torch.equal(got, again)
+    assert torch.equal(call(q=qi, k=ki, v=vi, out=qi), again)
+    r.check_errors()

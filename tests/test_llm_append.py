@@ -14,7 +14,7 @@ import torch
 
 from nanovllm_dots_b200 import _lib
 from nanovllm_dots_b200.llm_append import B200AppendAttention, tree_masks
-from nanovllm_dots_b200.llm_rotary import B200Rotary, RotaryScaling, _turns, rotary_frequencies
+from nanovllm_dots_b200.llm_rotary import B200Rotary, RotaryScaling, _turns, meets, rotary_frequencies, shared
 from oracle import llm_append_oracle as O
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -196,6 +196,38 @@ def test_turns_are_rounded_to_the_last_bit(rot, theta, scaling):
     for w, t in zip(inv.tolist(), _turns(inv).tolist()):
         off = Fraction(t % (1 << 64)) - Fraction(w) / period * (1 << 64)
         assert abs(off) <= Fraction(1, 2) + Fraction(1, 1 << 100)
+
+
+def test_shared_memory_is_found_element_by_element():
+    """Against the sets of the elements' addresses, for views of one buffer at random."""
+    import random
+
+    r = random.Random(0)
+    room = torch.zeros(4000, dtype=torch.bfloat16)
+
+    def view():
+        n, heads, dims = r.randint(0, 5), r.randint(1, 4), r.choice((2, 4, 8))
+        ts, hs = r.choice((0, 8, 24, 40, 96, 97)), r.choice((0, 2, 8, 10, 24))
+        return room.as_strided((n, heads, dims), (ts, hs, 1), r.randint(0, 300))
+
+    def bytes_of(t):
+        return {t.data_ptr() + 2 * (i * t.stride(0) + j * t.stride(1) + d) for i in range(t.shape[0])
+                for j in range(t.shape[1]) for d in range(t.shape[2])}
+
+    seen = set()
+    for _ in range(3000):
+        a, b = view(), view()
+        want = bool(bytes_of(a) & bytes_of(b))
+        assert shared(a, b) == want == shared(b, a)
+        lo = room.data_ptr() + 2 * r.randint(0, 400)
+        hi = lo + 2 * r.randint(1, 60)
+        inside = any(lo <= x < hi for x in bytes_of(a))
+        assert meets(a, lo, hi) == inside
+        seen.add((want, inside))
+    assert len(seen) == 4
+    packed = torch.zeros(7, 16, 8)           # a packed projection, and one interleaved by heads
+    assert not shared(packed[:, :12], packed[:, 12:14]) and shared(packed[:, :13], packed[:, 12:14])
+    assert not shared(packed[:, 0::2], packed[:, 1::2]) and shared(packed[:, 0::2], packed[:, 0::4])
 
 
 def test_tree_masks():
