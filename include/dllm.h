@@ -187,7 +187,7 @@ typedef struct DllmAppend {
   const uint64_t* tree_masks;   /* [tokens] or NULL */
   const float* slopes;          /* [num_heads] or NULL */
   void* out;                    /* [tokens, num_heads, head_dim], 32-byte aligned; may be a
-                                 * q of the same strides, else no overlap */
+                                 * q of the same strides, else no overlap with anything */
 } DllmAppend;
 
 /* Workspace bytes for up to these bounds, 0 if the shape is not supported.

@@ -133,6 +133,9 @@ class B200AppendAttention:
             raise RuntimeError("out: expected 32-byte alignment")
         elif overlap(q, out) and not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):
             raise RuntimeError("out: overlaps q without being q")
+        elif T and any(c.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < c.data_ptr() + c.nbytes
+                       for c in (k_cache, v_cache)):
+            raise RuntimeError("out: overlaps a cache")
         i32, width = torch.int32, rows[1]
         plain = tree is None
         a = _pack(

@@ -633,3 +633,19 @@ def test_errors_of_a_graph_on_another_stream_are_reported():
         with pytest.raises(RuntimeError, match="page"):
             att.check_errors()
         att.check_errors()
+
+
+def test_out_over_a_cache_is_refused():
+    c = Case([(20, 300), (3, 40)], 8, 8, D=64, bs=16).device()
+    att = c.attention()
+    want, K, V = c.call(att), c.Kd.clone(), c.Vd.clone()
+    T = c.q.shape[0]
+    for cache in (c.Kd, c.Vd):
+        for at in (0, cache.numel() - T * 512):
+            with pytest.raises(RuntimeError, match="overlaps a cache"):
+                c.call(att, out=cache.flatten()[at:at + T * 512].view(T, 8, 64))
+    both = torch.zeros(c.Kd.numel() + T * 512, dtype=BF, device=DEV)      # right behind a cache is free
+    both[:c.Kd.numel()] = c.Kd.flatten()
+    c.Kd, out = both[:c.Kd.numel()].view_as(c.Kd), both[c.Kd.numel():].view(T, 8, 64)
+    assert torch.equal(c.call(att, out=out), want)
+    assert torch.equal(c.Kd.nan_to_num(9.0), K.nan_to_num(9.0)) and torch.equal(c.Vd.nan_to_num(9.0), V.nan_to_num(9.0))
