@@ -181,10 +181,10 @@ class B200Rotary:
         D = self.head_dim
         if abs(kc - vc) < room:
             raise RuntimeError("k_cache and v_cache overlap")
-        lo, hi = min(kc, vc), max(kc, vc) + room
         for t, p, ts, hs, n in read if out is None else (*read, out):
-            if p < hi and p + ((T - 1) * ts + (n - 1) * hs + D) * size > lo and \
-                    (meets(t, kc, kc + room) or meets(t, vc, vc + room)):
+            end = p + ((T - 1) * ts + (n - 1) * hs + D) * size
+            if (p < kc + room and end > kc and meets(t, kc, kc + room)) or \
+                    (p < vc + room and end > vc and meets(t, vc, vc + room)):
                 raise RuntimeError("q, k, v or out overlaps a cache")
         if out is None:
             return
@@ -241,13 +241,13 @@ class B200Rotary:
             slots = shape[0] * shape[1]
             kp, vp, qp = k.data_ptr(), v.data_ptr(), q.data_ptr()
             kcp, vcp = k_cache.data_ptr(), v_cache.data_ptr()
-            D, size = self.head_dim, self._size[dtype]
-            room, lo, hi = slots * kvh * D * size, min(kcp, vcp), max(kcp, vcp)
-            end, t1 = hi + room, T - 1
-            if T and (given or hi - lo < room or
-                      (qp < end and qp + (t1 * qt + (heads - 1) * qh + D) * size > lo) or
-                      (kp < end and kp + (t1 * kt + (kvh - 1) * kh + D) * size > lo) or
-                      (vp < end and vp + (t1 * vt + (kvh - 1) * vh + D) * size > lo)):
+            D, size, t1 = self.head_dim, self._size[dtype], T - 1
+            room = slots * kvh * D * size
+            kce, vce, qe = kcp + room, vcp + room, qp + (t1 * qt + (heads - 1) * qh + D) * size
+            ke, ve = kp + (t1 * kt + (kvh - 1) * kh + D) * size, vp + (t1 * vt + (kvh - 1) * vh + D) * size
+            if T and (given or kcp < vce and vcp < kce or qp < kce and kcp < qe or qp < vce and vcp < qe or
+                      kp < kce and kcp < ke or kp < vce and vcp < ke or vp < kce and kcp < ve or
+                      vp < vce and vcp < ve):
                 self._check_apart(((q, qp, qt, qh, heads), (k, kp, kt, kh, kvh), (v, vp, vt, vh, kvh)),
                                   (out, out.data_ptr(), ot, oh, heads) if given else None, T, size, kcp, vcp, room)
         if T == 0 or heads == 0 and store is None:
