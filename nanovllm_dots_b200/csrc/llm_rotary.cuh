@@ -145,7 +145,7 @@ constexpr int RO_MAX_PAIRS = 256;    // of a head in the table
 template <typename T, bool INTER, int TB>
 __global__ void __launch_bounds__(RO_THREADS, 6) llm_rotary_kernel(RotaryParams p) {
   constexpr int VP = 16 / sizeof(T);
-  __shared__ float2 table[TB][RO_MAX_PAIRS];
+  __shared__ float4 table[TB][RO_MAX_PAIRS / 2];   // cosine and sine of two pairs: read 16 bytes at a time
   pdl_trigger();
   pdl_wait();
   const int half = p.rot / 2, heads = p.heads + (p.slots ? 2 * p.kv_heads : 0);
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(RO_THREADS, 6) llm_rotary_kernel(RotaryParams 
     const int tok = TB > 1 ? p.by_pairs(i) : 0, e = i - tok * half;
     float c, s;
     rotary_sincos(p.turns[e], p.positions[t0 + tok], p.factor, c, s);
-    table[tok][e] = make_float2(c, s);
+    reinterpret_cast<float2*>(table[tok])[e] = make_float2(c, s);
   }
   __syncthreads();
   for (int item = threadIdx.x; item < items; item += RO_THREADS) {
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(RO_THREADS, 6) llm_rotary_kernel(RotaryParams 
     if (turn) {
       T* x = reinterpret_cast<T*>(&va);
       T* y = reinterpret_cast<T*>(&vb);
-      const float4* cs = reinterpret_cast<const float4*>(&table[t][l * VP]);
+      const float4* cs = &table[t][l * VP / 2];
 #pragma unroll
       for (int i = 0; i < VP; i += 2) {
         const float4 c = cs[i / 2];
