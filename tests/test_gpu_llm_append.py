@@ -649,3 +649,37 @@ def test_out_over_a_cache_is_refused():
     c.Kd, out = both[:c.Kd.numel()].view_as(c.Kd), both[c.Kd.numel():].view(T, 8, 64)
     assert torch.equal(c.call(att, out=out), want)
     assert torch.equal(c.Kd.nan_to_num(9.0), K.nan_to_num(9.0)) and torch.equal(c.Vd.nan_to_num(9.0), V.nan_to_num(9.0))
+
+
+LONG = [[(3, 70000)], [(1, 40000), (64, 33333), (1, 0)], [(200, 20000)], [(1, 9000), (2, 12345), (40, 6000)] * 7]
+
+
+@pytest.mark.parametrize("D,bs,H,KVH", [(64, 256, 4, 1), (128, 256, 12, 2), (64, 16, 4, 4), (128, 48, 6, 2)])
+@pytest.mark.parametrize("lens,opts", [(x, {}) for x in LONG] + [
+    (LONG[0], dict(window=30011)), (LONG[1], dict(causal=False)), (LONG[3], dict(window=5000)),
+    ([(25, 40000), (64, 17000), (7, 999)], dict(tree=True)), (LONG[1], dict(softcap=10.0))])
+def test_every_key_counts_once(lens, opts, D, bs, H, KVH):
+    """Zero queries weigh all keys alike; the values say which 16 keys they belong to (a
+    one at that number modulo D), so that the output counts the keys of each: a box of
+    16 that is left out, read twice or taken from elsewhere changes a dim by one part
+    in as many boxes as share it, several times the rounding of the result.  (Sums of
+    ones are exact, the probabilities of the fp32 pipe 1e-7 off.)"""
+    opts = dict(opts)
+    if "tree" in opts:
+        opts["tree"] = trees(lens, 6)
+    c = Case(lens, H, KVH, D, bs, **opts)
+    c.q.zero_()
+    ref = []
+    for i, (m, p) in enumerate(lens):
+        k = torch.arange(m + p)
+        live = c.see[i].any(0)
+        code = torch.nn.functional.one_hot(k // 16 % D, D)
+        c.V[c.table[i, k[live] // bs].long(), k[live] % bs] = code[live, None].to(BF).expand(-1, KVH, D)
+        see = c.see[i].double()
+        ref.append(see @ code.double() / see.sum(1, keepdim=True))
+        assert -(-(m + p) // 16) / D < 1 / (2 * O.HALF_STEP[BF]) - 1      # (a box is seen in the result)
+    att = c.attention()
+    got = c.device().call(att)
+    att.check_errors()
+    ref = torch.cat(ref)[:, None].expand(-1, H, D)
+    check(got, ref, ref * (O.HALF_STEP[BF] + 2.0 ** -21))
