@@ -131,3 +131,59 @@ def test_serving_loop():
     s.append.check_errors()
     s.rotary.check_errors()
     s.decode.check_errors()
+
+
+@pytest.mark.parametrize("decode_first", [True, False])
+def test_installed_module_over_a_packed_projection(decode_first):
+    """The two hooks on a module of the engine's shape: its forward gets the projection's slices
+    ([tokens, heads * D], the values still inside the packed row), prefills two chunks of
+    two prompts over the paged cache and decodes one token each.  Calls outside the
+    hooks' conditions reach the module's own forward."""
+    from types import SimpleNamespace as NS
+
+    from nanovllm_dots_b200.llm_append import install_append_attention
+    from nanovllm_dots_b200.llm_attention import install_decode_attention
+
+    s, own = Loop(), []
+    module = NS(num_heads=H, num_kv_heads=KVH, head_dim=D, is_causal=True, k_cache=s.K, v_cache=s.V,
+                forward=lambda q, k, v: own.append(q.shape))
+    ctx = NS()
+
+    def store(k, v, k_cache, v_cache, slots):
+        k_cache.view(-1, KVH, D)[slots.long()] = k
+        v_cache.view(-1, KVH, D)[slots.long()] = v
+
+    hooks = [lambda: install_decode_attention(module, lambda: ctx, s.decode),
+             lambda: install_append_attention(module, lambda: ctx, s.append, store)]
+    for hook in hooks if decode_first else hooks[::-1]:
+        hook()
+
+    def forward(counts, prefill):
+        packed = s.project(counts)
+        base = [len(k) for k in s.kept]
+        pos = [base[i] + j for i, m in enumerate(counts) for j in range(m)]
+        d = packed.to(DEV).view(sum(counts), -1)
+        q, k, v = d.split([H * D, KVH * D, KVH * D], dim=1)
+        at = torch.tensor(pos, dtype=torch.int32, device=DEV)
+        q, k = (s.rotary.rotate(x.view(x.shape[0], -1, D), at).flatten(1) for x in (q, k))
+        ctx.slot_mapping = torch.cat([s.slots(i, base[i], m) for i, m in enumerate(counts)]).to(torch.int32).to(DEV)
+        i = 0
+        for n, m in enumerate(counts):
+            s.kept[n] += [(packed[i + j, H:H + KVH], packed[i + j, H + KVH:], pos[i + j]) for j in range(m)]
+            i += m
+        ctx.is_prefill = prefill
+        ctx.cu_seqlens_q, ctx.context_lens, ctx.block_tables = s.lens(counts)
+        ctx.cu_seqlens_k = torch.nn.functional.pad(ctx.context_lens.cumsum(0, dtype=torch.int32), (1, 0))
+        got = module.forward(q, k if prefill else k.contiguous(), v if prefill else v.contiguous())
+        s.check(got, q.view(-1, H, D), packed, counts, pos,
+                [O.visible(m, len(s.kept[i])) for i, m in enumerate(counts)])
+
+    for counts, prefill in (([300, 40], True), ([77, 200], True), ([1, 1], False), ([3, 1], True)):
+        forward(counts, prefill)
+    s.append.check_errors()
+    s.decode.check_errors()
+    assert not own
+    ctx.is_prefill, ctx.block_tables = True, None
+    q = torch.zeros(5, H * D, dtype=BF, device=DEV)
+    module.forward(q, q[:, :KVH * D], q[:, :KVH * D])
+    assert own == [q.shape]
