@@ -52,7 +52,8 @@ int dllm_decode_attention(const void* q, const void* k, const void* v, void* k_c
                           int32_t block_size, int32_t max_blocks, float softmax_scale, void* out,
                           void* workspace, size_t workspace_bytes, void* stream);
 
-/* Read and clear the device error word of a workspace; synchronises `stream`. */
+/* Read and clear the device error word of a workspace; synchronises `stream`.
+ * Calls on other streams are seen if the caller has waited for them. */
 int dllm_read_error(void* workspace, void* stream, uint32_t* err_word);
 
 /* ---------------------------------------------------------------------------
@@ -162,10 +163,12 @@ int dllm_rotary(const DllmRotary* args, void* stream);
  * mask, whatever their order; the other masks and slopes are not used then.
  * Scores are s = scale q.k, softcap tanh(s / softcap) if softcap > 0, minus
  * slopes[h] |p - k| if slopes; the output is softmax(s) v, and zeros for a
- * token that sees no key.  An infinity or NaN in a K row reaches the tokens
- * that see it, one in a V row its own dims of theirs (as an infinity or NaN),
- * and no other; keys that no token sees are not read beyond the pages of those
- * that are.  Rows of q and out past cu_seqlens_q[n] are not touched.
+ * token that sees no key.  Scores, softmax and sums are fp32; each softmax
+ * weight is rounded to dtype before it meets its row of V (half a step), the
+ * result once more.  An infinity or NaN in a K row reaches the tokens that see
+ * it, one in a V row its own dims of theirs (as an infinity or NaN), and no
+ * other; keys that no token sees are not read beyond the pages of those that
+ * are.  Rows of q and out past cu_seqlens_q[n] are not touched.
  * ------------------------------------------------------------------------- */
 typedef struct DllmAppend {
   int32_t dtype;                /* of q, caches and out: DLLM_BF16 or DLLM_FP16 */
@@ -202,8 +205,9 @@ size_t dllm_append_workspace_size(int32_t tokens, int32_t n, int32_t num_heads,
  * nearly 2^31 positions, or of more key tiles in all than 30 bits count, and a
  * softcap below 1e-37 scale or above 1e18 scale are refused
  * (DFM_ERR_UNSUPPORTED).  Lengths that make no sense, a block id out of range
- * or a tree of more than 64 tokens set a device error bit (dllm_read_error); such a sequence's rows are zeros, or untouched where
- * cu_seqlens_q itself is wrong, and such a block reads as zeros. */
+ * or a tree of more than 64 tokens set a device error bit (dllm_read_error);
+ * such a sequence's rows are zeros, or untouched where cu_seqlens_q itself is
+ * wrong, and such a block reads as zeros. */
 int dllm_append_attention(const DllmAppend* args, void* workspace, size_t workspace_bytes,
                           void* stream);
 

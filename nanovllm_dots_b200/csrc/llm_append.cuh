@@ -35,11 +35,18 @@
 // Two full row tiles: a stream's chain of maximum (750 clocks), probabilities (1500)
 // and the products of P and of the next scores (1250 of latency and of the other
 // stream's): 3500 clocks a key tile, of which the tensor cores are busy 2048 with
-// D = 128.  8192 tokens behind 8192: 516 us, 1.2 PFLOP/s (595 us and 1.04 under the
-// power cap; the same loads and products without a softmax 440).  All 512 TMEM columns are
-// taken (S, S, O, O), so scores cannot be computed ahead of P; key tiles of 64 in two
-// buffers, which could, take the tensor cores twice as long a score (676 us);
-// two threads a row instead of one: 568.
+// D = 128.  8192 tokens behind 8192: 526 us, 1.17 PFLOP/s (605 us and 1.02 under the
+// power cap; the same loads and products without a softmax 440).  With D = 128 all 512
+// TMEM columns are taken (S, S, O, O), so scores cannot be computed ahead of P, which
+// the 128 columns left with D = 64 would allow; key tiles of 64 in two buffers, which
+// could, take the tensor cores twice as long a score (676 us); two threads a row
+// instead of one: 568.
+//
+// P is rounded to the type of V, which the product asks of both (half a step, relative
+// to each probability); scores, maxima, sums and O are fp32, and the sum takes P
+// before its rounding.  For given lengths a row's result depends on its own query and
+// the keys that it sees, bit for bit: what a warp decides together only chooses the
+// way there.
 //
 // Keys nobody in the unit may see are not loaded (their pages may be gone) and
 // their rows of V are set to zero.  In a tile with masks, an infinity or a NaN in a

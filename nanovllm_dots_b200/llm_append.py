@@ -46,9 +46,10 @@ class B200AppendAttention:
     sequences.
 
     The workspace serves one call at a time.  Calls on one stream follow each
-    other; a call on another stream waits for the last one's stream.  A captured
-    graph keeps using the workspace: replay graphs of one object, and call it,
-    on one stream at a time, or give each an object of its own.
+    other; a call on another stream waits for the last one's stream, which has to
+    exist until then.  A captured graph keeps using the workspace: replay graphs of
+    one object, and call it, on one stream at a time, or give each an object of its
+    own, as threads need that call at the same time.
     """
 
     def __init__(self, num_heads: int, head_dim: int, scale: float, num_kv_heads: int, *,
