@@ -177,7 +177,8 @@ class B200Rotary:
         """Raises where the store's outputs share memory with each other or with what
         the call reads (out may be q).  Tensors come with address, token and head
         strides and heads: where their spans cross, slices of one packed row are
-        apart by their places in it, and else every row is looked at."""
+        apart by their places in it, heads that take turns by theirs, and else every
+        row is looked at (milliseconds)."""
         D = self.head_dim
         if abs(kc - vc) < room:
             raise RuntimeError("k_cache and v_cache overlap")
@@ -193,7 +194,9 @@ class B200Rotary:
         for other, p2, ts2, hs2, n2 in read[1:]:
             wide2 = ((n2 - 1) * hs2 + D) * size
             if p2 + (T - 1) * ts2 * size + wide2 <= p or p + (T - 1) * row + wide <= p2 or \
-                    (ts == ts2 and row and wide <= (p2 - p) % row <= row - wide2):
+                    (ts == ts2 and row and wide <= (p2 - p) % row <= row - wide2) or \
+                    (hs == hs2 and hs and ts % hs == ts2 % hs == 0 and
+                     D * size <= (p2 - p) % (hs * size) <= (hs - D) * size):
                 continue
             if shared(t, other):
                 raise RuntimeError("out: overlaps k or v")

@@ -205,3 +205,36 @@ def test_store_refuses_memory_that_its_outputs_share():
     assert torch.equal(got, again)
     assert torch.equal(call(q=qi, k=ki, v=vi, out=qi), again)
     r.check_errors()
+
+
+def test_usual_layouts_are_told_apart_by_their_strides(monkeypatch):
+    """In place in a packed row, in one whose heads are interleaved, and in a buffer with
+    the heads in front: no row by row search."""
+    from nanovllm_dots_b200 import llm_rotary
+
+    def search(*_):
+        raise AssertionError("searched row by row")
+
+    monkeypatch.setattr(llm_rotary, "shared", search)
+    monkeypatch.setattr(llm_rotary, "meets", search)
+    T, D = 300, 64
+    r = B200Rotary(D, device=DEV)
+    pos, slots = positions(T).to(DEV), torch.arange(T, dtype=torch.int32, device=DEV)
+    x = data(T, 12, D, torch.bfloat16).to(DEV)
+    K = torch.zeros(2, 160, 4, D, dtype=torch.bfloat16, device=DEV)
+    V = torch.zeros_like(K)
+    want = r.rotate_store(x[:, :4], x[:, 4:8], x[:, 8:], pos, slots, K, V)
+    kept = K.clone()
+    for layout in ("packed", "interleaved", "heads in front"):
+        buffer = torch.empty(12 * T * D, dtype=torch.bfloat16, device=DEV)
+        if layout == "packed":
+            q, k, v = buffer.view(T, 12, D).split(4, dim=1)
+        elif layout == "interleaved":
+            q, k, v = buffer.view(T, 4, 3, D).unbind(2)
+        else:
+            q, k, v = buffer.view(12, T, D).transpose(0, 1).split(4, dim=1)
+        for to, at in ((q, 0), (k, 4), (v, 8)):
+            to.copy_(x[:, at:at + 4])
+        K.zero_()
+        assert r.rotate_store(q, k, v, pos, slots, K, V, out=q) is q
+        assert torch.equal(q, want) and torch.equal(K, kept)

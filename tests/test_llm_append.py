@@ -230,6 +230,46 @@ def test_shared_memory_is_found_element_by_element():
     assert not shared(packed[:, 0::2], packed[:, 1::2]) and shared(packed[:, 0::2], packed[:, 0::4])
 
 
+def test_store_check_refuses_exactly_what_shares_memory():
+    """The strides' short cuts and the search behind them against sets of addresses."""
+    import random
+    from types import SimpleNamespace as NS
+
+    r, room = random.Random(1), torch.zeros(6000, dtype=torch.bfloat16)
+    seen = {True: 0, False: 0}
+    for _ in range(6000):
+        T, D = r.randint(1, 4), r.choice((2, 4))
+        ts, hs = r.choice((12, 24, 48, 96, 40)), r.choice((D, 2 * D, 3 * D, 12, 24, 96))
+
+        def view(heads):
+            t, h = (ts, hs) if r.random() < 0.7 else (r.choice((8, 24, 50)), r.choice((D, 6, 16)))
+            return room.as_strided((T, heads, D), (t, h, 1), r.randint(0, 250))
+
+        q, k, v, out = view(3), view(2), view(2), view(3)
+        if r.random() < 0.3:
+            out = q
+        # mostly behind the views, sometimes among them
+        kc, vc = (room.data_ptr() + 2 * r.choice((r.randint(0, 300), r.randint(700, 2500))) for _ in range(2))
+        n = 2 * r.randint(8, 200)
+
+        def of(t):
+            return {t.data_ptr() + 2 * (i * t.stride(0) + j * t.stride(1) + d) + b for i in range(T)
+                    for j in range(t.shape[1]) for d in range(D) for b in range(2)}
+
+        caches = [set(range(c, c + n)) for c in (kc, vc)]
+        bad = bool(caches[0] & caches[1]) or any(of(t) & c for t in (q, k, v, out) for c in caches) or \
+            bool(of(out) & (of(k) | of(v)))
+        at = lambda t: (t, t.data_ptr(), t.stride(0), t.stride(1), t.shape[1])  # noqa: E731
+        try:
+            B200Rotary._check_apart(NS(head_dim=D), (at(q), at(k), at(v)), at(out), T, 2, kc, vc, n)
+            refused = False
+        except RuntimeError:
+            refused = True
+        assert refused == bad
+        seen[bad] += 1
+    assert min(seen.values()) > 300, seen
+
+
 def test_tree_masks():
     got = tree_masks([[-1, 0, 0, -1, 2], [-1]])
     assert got.tolist() == [0b1, 0b11, 0b101, 0b1000, 0b10101, 0b1]
