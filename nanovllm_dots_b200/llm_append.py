@@ -64,8 +64,9 @@ class B200AppendAttention:
             raise RuntimeError(f"unsupported append-attention type {dtype}")
         if block_size < 16 or block_size % 16:
             raise RuntimeError(f"block_size {block_size}: expected a multiple of 16")
-        if not scale > 0 or softcap < 0 or window < 0 or max_blocks < 1:
-            raise RuntimeError("expected a positive scale and max_blocks, no negative softcap or window")
+        if not 0 < scale < 3e38 or not 0 <= softcap < 3e38 or not 0 <= window < 1 << 31 or max_blocks < 1:
+            raise RuntimeError("expected a positive scale and max_blocks, no negative softcap or window, "
+                               "all finite and the window below 2^31")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim

@@ -144,6 +144,14 @@ def test_classes_refuse_what_they_cannot_do():
             B200AppendAttention(12, 128, kw.pop("scale"), 2, max_tokens=8, max_seqs=1, device="cuda:0", **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e39), dict(softcap=math.nan),
+                                dict(softcap=math.inf), dict(softcap=1e39), dict(window=1 << 31), dict(window=1 << 70)])
+def test_options_beyond_their_fields_are_refused_at_once(kw):
+    kw = {"scale": 0.1, **kw}
+    with pytest.raises(RuntimeError, match="expected a positive scale"):
+        B200AppendAttention(12, 128, kw.pop("scale"), 2, max_tokens=8, max_seqs=1, max_blocks=1, device="cuda:0", **kw)
+
+
 def test_frequencies():
     plain, one = rotary_frequencies(128, 1e6)
     assert one == 1.0 and plain.dtype == torch.float64
