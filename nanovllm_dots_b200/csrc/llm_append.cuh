@@ -1250,7 +1250,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           float xa[32], xb[32];
           auto ld = [&](float (&x)[32], int c) { ap_load(tS + c * 32, x); };
           bool stored = kBias || !full;
-          bool raw = false, some_raw = false;   // this row, some row leaves its cap to the second pass
+          bool raw = false;   // this row leaves its cap to the second pass
           float near_top = 0.f;
           if (!stored) {
             float big = 0.f;
@@ -1271,7 +1271,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               // stored back and read again)
               raw = !ap_far(big, p);
               stored = __any_sync(0xffffffffu, valid && !raw);
-              some_raw = __any_sync(0xffffffffu, valid && raw);
               near_top = ap_cap_one(top, p);
               top = -INFINITY;
             }
@@ -1434,9 +1433,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
             }
           };
-          if (!kLateCap || !full) second_pass(std::integral_constant<int, 0>{});
-          else if (!stored) second_pass(std::integral_constant<int, kLateCap ? 1 : 0>{});
-          else second_pass(std::integral_constant<int, kLateCap ? 2 : 0>{});
+          if (kLateCap && full && !stored) second_pass(std::integral_constant<int, kLateCap ? 1 : 0>{});
+          else if (kLateCap && __any_sync(0xffffffffu, valid && raw)) second_pass(std::integral_constant<int, kLateCap ? 2 : 0>{});
+          else second_pass(std::integral_constant<int, 0>{});
           float a, b;
           f2_split(f2_add(sum0, sum1), a, b);
           l += a + b;
